@@ -240,6 +240,63 @@ int kd_gated_delta_rule(const void* qkv, int64_t ldqkv, const void* ab, int64_t 
 int kd_gated_norm(const void* x, int64_t ldx, const void* z, int64_t ldz, const void* weight, int64_t T, int heads,
                   int head_dim, float eps, void* out, int64_t ldo, cudaStream_t stream);
 
+/* ---------------------------------------------------------------------------------------------- cache of states
+ * Keys and values of earlier tokens kept in blocks of KD_KV_BLOCK tokens, so that a state that is asked about again runs
+ * only its new rows. One layer's pool: codes k, v e4m3 [blocks][heads_kv][KD_KV_BLOCK][head_dim] (contiguous) and one
+ * float32 scale per (block, head) for each, a power of two with exponent in [-100, 120]: value = code * scale. Block
+ * tables int32 [requests][width] name each request's blocks in order (-1: none). No counterpart in the reference, which
+ * computes every request from its first token (decider.py:110-123). */
+#define KD_KV_BLOCK 64
+#define KD_KV_TABLE_FULL (-1) /* free_count[1]: a request's blocks exceed the table's width */
+#define KD_KV_MALFORMED (-2)  /* free_count[1]: lengths, bounds, count or block ids outside their ranges */
+
+/* Blocks, positions and slots of new rows. Request i holds lens[i] tokens and gets the rows [cu[i], cu[i+1]); free_blocks
+ * int32 [capacity] is a stack of free block ids (capacity: blocks in the pool), free_count[0] its height. The request's
+ * further blocks are taken from the top in request order and written to its table row; kv_len[i] = lens[i] + new rows
+ * (kv_len may be lens), seqpos[t] the row's position in its request, slots[t] = block * KD_KV_BLOCK + place. Rows
+ * outside every request (padding) get position 0 and slot -1. All or nothing: when blocks are missing nothing is taken,
+ * every slot is -1 and kv_len = lens. free_count[1]: 0, the number of missing blocks, or KD_KV_TABLE_FULL /
+ * KD_KV_MALFORMED. At most 16,384 requests. */
+int kd_kv_assign(const int32_t* lens, const int32_t* cu, int num_requests, int64_t rows, int32_t* table,
+                 int64_t ld_table, int table_width, const int32_t* free_blocks, int capacity, int32_t* free_count,
+                 int32_t* kv_len, int64_t* seqpos, int64_t* slots, cudaStream_t stream);
+
+/* The inverse: the blocks that hold none of request i's first keep[i] tokens (of lens[i]) return to the stack, the last
+ * request's last block first, and their table entries become -1. lens is not written. free_count[1]: 0, or
+ * KD_KV_MALFORMED (an entry outside the pool, a stack without room: nothing is given back). A block named by two
+ * requests would be given back twice: no two may share one. */
+int kd_kv_release(int32_t* table, int64_t ld_table, int table_width, const int32_t* lens, const int32_t* keep,
+                  int num_requests, int32_t* free_blocks, int capacity, int32_t* free_count, cudaStream_t stream);
+
+/* The rows' keys and values (bf16 [rows][heads_kv][head_dim], row strides in elements) into their blocks. Per block and
+ * head the scale is the least power of two that keeps the largest finite magnitude within 448 scale units; a block that
+ * held earlier tokens of the request (its first new row is not the block's first) keeps the larger of its scale and the
+ * new rows' own, and where it grows its earlier codes are brought to it, each rounded once to nearest even. Values
+ * saturate at 448 * scale (infinities too). A token with a NaN in its key or value is stored as a NaN key (code 0x7f) and
+ * a zero value: exactly the query rows that see it become NaN. A request's rows take consecutive places, as
+ * kd_kv_assign makes them; requests whose first slot is negative, and rows outside every request, are not written. No
+ * two requests may write one block in one call. head_dim 64, 128, 256 or 512. */
+int kd_kv_store_e4m3(const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t rows, const int32_t* cu,
+                     int num_requests, const int64_t* slots, int num_heads_kv, int head_dim, void* k_codes,
+                     void* v_codes, float* k_scale, float* v_scale, int64_t num_blocks, cudaStream_t stream);
+
+/* *bytes (a host int64): the scratch kd_attention_cache needs on the current device, 16-byte aligned, one area per
+ * launch in flight. */
+int kd_attention_cache_workspace(int num_requests, int64_t total_q, int num_heads_q, int num_heads_kv, int head_dim,
+                                 int64_t* bytes);
+
+/* Attention of new rows over their requests' cached tokens, the visibility rule and the gate of kd_attention_varlen with
+ * Lk = kv_len[i] (new rows stored first: a causal row sees itself). q (total_q, heads_q, head_dim) bf16; cu_q int32
+ * [requests + 1], kv_len int32 [requests] and the table are read when the kernel runs; max_q bounds every request's
+ * rows. out rows outside every request are left as they were; a row that sees no key is 0. A table entry outside the
+ * pool hides its block's tokens. out = bf16(o * sigmoid(gate)) with a gate (one rounding). head_dim 64, 128, 256, 512. */
+int kd_attention_cache(const void* q, int64_t ldq, const void* k_codes, const void* v_codes, const float* k_scale,
+                       const float* v_scale, int64_t num_blocks, const int32_t* table, int64_t ld_table,
+                       int table_width, const int32_t* cu_q, const int32_t* kv_len, int num_requests, int max_q,
+                       int64_t total_q, void* out, int64_t ldo, const void* gate, int64_t ldg, int num_heads_q,
+                       int num_heads_kv, int head_dim, float scale, int window_left, int window_right, void* workspace,
+                       int64_t workspace_bytes, int* status, cudaStream_t stream);
+
 /* The head: out[m, :] = norm(h[markers[m], :]) (final norm at the readout markers).
  * Replaces families/qwen/packed.py:173-176 and families/gemma/packed.py:297-303. */
 int kd_marker_norm(const void* h, int hidden, const int64_t* markers, int64_t M, const void* weight, int norm_mode,

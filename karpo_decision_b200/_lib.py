@@ -16,6 +16,7 @@ KD_OK = 0
 KD_DEVICE_TIMEOUT = 1
 EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU, EPI_GEGLU = 0, 1, 2, 3
 NORM_NONE, NORM_WEIGHT, NORM_ONE_PLUS = 0, 1, 2
+KV_BLOCK, KV_TABLE_FULL, KV_MALFORMED = 64, -1, -2
 
 P = c_void_p
 #: Every exported entry point: name -> argument types (all return int).
@@ -50,6 +51,12 @@ SIGNATURES: dict[str, list] = {
     "kd_gated_delta_rule": [P, c_int64, P, c_int64, P, P, P, c_int, c_int64, c_int, c_int, c_int, c_int, P, c_int64,
                             P, P],
     "kd_gated_norm": [P, c_int64, P, c_int64, P, c_int64, c_int, c_int, c_float, P, c_int64, P],
+    "kd_kv_assign": [P, P, c_int, c_int64, P, c_int64, c_int, P, c_int, P, P, P, P, P],
+    "kd_kv_release": [P, c_int64, c_int, P, P, c_int, P, c_int, P, P],
+    "kd_kv_store_e4m3": [P, c_int64, P, c_int64, c_int64, P, c_int, P, c_int, c_int, P, P, P, P, c_int64, P],
+    "kd_attention_cache_workspace": [c_int, c_int64, c_int, c_int, c_int, P],
+    "kd_attention_cache": [P, c_int64, P, P, P, P, c_int64, P, c_int64, c_int, P, P, c_int, c_int, c_int64, P, c_int64,
+                           P, c_int64, c_int, c_int, c_int, c_float, c_int, c_int, P, c_int64, P, P],
     "kd_marker_norm": [P, c_int, P, c_int64, P, c_int, c_float, P, P],
     "kd_readout": [P, c_int64, c_int, P, c_int, c_float, P, P],
 }

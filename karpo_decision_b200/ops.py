@@ -4,14 +4,21 @@ stream. Each op is one entry point of libkd_b200; none has a fallback.
 
 from __future__ import annotations
 
+import ctypes
+import functools
+from typing import NamedTuple
+
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import EPI_GEGLU, EPI_RESIDUAL, EPI_STORE, EPI_SWIGLU, NORM_NONE, NORM_ONE_PLUS, NORM_WEIGHT, call
+from ._lib import (EPI_GEGLU, EPI_RESIDUAL, EPI_STORE, EPI_SWIGLU, KV_BLOCK, KV_MALFORMED, KV_TABLE_FULL, NORM_NONE,
+                   NORM_ONE_PLUS, NORM_WEIGHT, call)
 
-__all__ = ["EPI_GEGLU", "EPI_RESIDUAL", "EPI_STORE", "EPI_SWIGLU", "NORM_NONE", "NORM_ONE_PLUS", "NORM_WEIGHT",
-           "add_rmsnorm", "attention_varlen", "check_status", "embed", "gather_rows", "gemm", "gemm_fp8", "marker_norm",
+__all__ = ["EPI_GEGLU", "EPI_RESIDUAL", "EPI_STORE", "EPI_SWIGLU", "KV_BLOCK", "KV_MALFORMED", "KV_TABLE_FULL",
+           "KVBlocks", "NORM_NONE", "NORM_ONE_PLUS", "NORM_WEIGHT",
+           "add_rmsnorm", "attention_cache", "attention_varlen", "check_status", "embed", "gather_rows", "gemm",
+           "gemm_fp8", "kv_assign", "kv_blocks", "kv_release", "kv_store_e4m3", "marker_norm",
            "norm_add", "qkv_norm_rope", "qkv_projection", "quantize_rows_e4m3", "readout", "rmsnorm", "rmsnorm_e4m3",
            "rope_gather", "rope_table", "rope_table_axes",
            "sched_pair", "status_word"]
@@ -397,4 +404,170 @@ def gated_norm(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, heads: in
         out = torch.empty(t, heads * head_dim, dtype=torch.bfloat16, device=x.device)
     call("kd_gated_norm", x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0), weight.data_ptr(), t, heads,
          head_dim, float(eps), out.data_ptr(), out.stride(0), _stream(x))
+    return out
+
+
+# ------------------------------------------------------------------------------------------------ cache of states
+
+
+class KVBlocks(NamedTuple):
+    """One layer's pool of cached keys and values: e4m3 codes (blocks, Hkv, 64, hd) and float32 power-of-two scales
+    (blocks, Hkv); value = code * scale."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def kv_blocks(blocks: int, kv_heads: int, head_dim: int, device: torch.device) -> KVBlocks:
+    """An empty pool of ``blocks`` blocks of 64 tokens."""
+    def codes() -> torch.Tensor:
+        return torch.zeros(blocks, kv_heads, KV_BLOCK, head_dim, dtype=torch.float8_e4m3fn, device=device)
+
+    def scales() -> torch.Tensor:
+        return torch.ones(blocks, kv_heads, dtype=torch.float32, device=device)
+
+    return KVBlocks(codes(), codes(), scales(), scales())
+
+
+def _pool(cache: KVBlocks) -> tuple[int, int, int]:
+    """(blocks, Hkv, hd) of a well-formed pool."""
+    k, v, ks, vs = cache
+    _require(k.dim() == 4 and k.shape[2] == KV_BLOCK and k.shape == v.shape, "cache codes: (blocks, Hkv, 64, head_dim)")
+    _require(k.dtype == v.dtype == torch.float8_e4m3fn and k.is_contiguous() and v.is_contiguous(),
+             "cache codes: contiguous e4m3")
+    _require(ks.shape == vs.shape == k.shape[:2] and ks.dtype == vs.dtype == torch.float32 and ks.is_contiguous()
+             and vs.is_contiguous(), "cache scales: contiguous float32 (blocks, Hkv)")
+    _require(k.is_cuda and k.device == v.device == ks.device == vs.device, "cache: on one CUDA device")
+    return k.shape[0], k.shape[1], k.shape[3]
+
+
+def _int32s(t: torch.Tensor, n: int, name: str, device: torch.device) -> None:
+    _require(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n, f"{name}: {n} contiguous int32")
+    _require(t.device == device, f"{name}: on {device}")
+
+
+def _block_table(table: torch.Tensor, n: int, device: torch.device) -> None:
+    _require(table.dim() == 2 and table.dtype == torch.int32 and (table.stride(1) == 1 or table.shape[1] <= 1),
+             "table: int32 (requests, width) with contiguous rows")
+    _require(table.shape[0] == n and (n <= 1 or table.stride(0) >= table.shape[1]),
+             f"table: {n} rows that do not overlap")
+    _require(table.device == device, f"table: on {device}")
+
+
+def kv_assign(lens: torch.Tensor, cu: torch.Tensor, table: torch.Tensor, free: torch.Tensor, count: torch.Tensor,
+              rows: int, out: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Blocks for the new rows [cu[i], cu[i + 1]) of requests holding ``lens`` tokens: takes them from the top of the
+    stack ``free`` (``count`` int32[2]: its height, the outcome), extends ``table`` in place and returns (kv_len int32
+    (n,), seqpos int64 (rows,), slots int64 (rows,)), or writes them to ``out`` (whose kv_len may be ``lens``). When
+    blocks are missing nothing is taken, every slot is -1 and ``count[1]`` says how many (or KV_TABLE_FULL /
+    KV_MALFORMED)."""
+    n, dev = lens.numel(), lens.device
+    _require(lens.is_cuda, "lens must be on a CUDA device")
+    _int32s(lens, n, "lens", dev)
+    _int32s(cu, n + 1, "cu", dev)
+    _block_table(table, n, dev)
+    _int32s(free, free.numel(), "free", dev)
+    _int32s(count, 2, "count", dev)
+    if out is None:
+        out = (torch.empty(n, dtype=torch.int32, device=dev), torch.empty(rows, dtype=torch.int64, device=dev),
+               torch.empty(rows, dtype=torch.int64, device=dev))
+    kv_len, seqpos, slots = out
+    _int32s(kv_len, n, "kv_len", dev)
+    _require(seqpos.dtype == slots.dtype == torch.int64 and seqpos.is_contiguous() and slots.is_contiguous()
+             and seqpos.numel() == slots.numel() == rows, "seqpos, slots: contiguous int64, one per row")
+    _require(seqpos.device == dev and slots.device == dev, f"seqpos, slots: on {dev}")
+    with torch.cuda.device(dev):
+        call("kd_kv_assign", lens.data_ptr(), cu.data_ptr(), n, rows, table.data_ptr(),
+             max(table.stride(0), table.shape[1]), table.shape[1], free.data_ptr(), free.numel(), count.data_ptr(),
+             kv_len.data_ptr(), seqpos.data_ptr(), slots.data_ptr(), _stream(lens))
+    return out
+
+
+def kv_release(table: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor, free: torch.Tensor, count: torch.Tensor
+               ) -> None:
+    """Gives the blocks past each request's first ``keep`` tokens (of ``lens``) back to the stack, undoing a
+    ``kv_assign`` exactly; ``lens`` is not written. No two requests may share a block given back."""
+    n, dev = lens.numel(), lens.device
+    _require(lens.is_cuda, "lens must be on a CUDA device")
+    _int32s(lens, n, "lens", dev)
+    _int32s(keep, n, "keep", dev)
+    _block_table(table, n, dev)
+    _int32s(free, free.numel(), "free", dev)
+    _int32s(count, 2, "count", dev)
+    with torch.cuda.device(dev):
+        call("kd_kv_release", table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1], lens.data_ptr(),
+             keep.data_ptr(), n, free.data_ptr(), free.numel(), count.data_ptr(), _stream(lens))
+
+
+def _head_rows(t: torch.Tensor, name: str, heads: int, head_dim: int) -> int:
+    """Row stride of (rows, heads, head_dim) bf16 with the heads packed within a row."""
+    _require(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == head_dim and t.dtype == torch.bfloat16,
+             f"{name}: bf16 (rows, {heads}, {head_dim})")
+    _require(t.stride(2) == 1 and (heads == 1 or t.stride(1) == head_dim), f"{name}: heads must be packed within a row")
+    return t.stride(0) if t.shape[0] > 1 else heads * head_dim
+
+
+def kv_store_e4m3(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, slots: torch.Tensor, cache: KVBlocks) -> None:
+    """Writes the rows' keys and values (T, Hkv, hd) into the blocks ``slots`` (from ``kv_assign``) names, quantized to
+    e4m3 with a power-of-two scale per (block, head); a half-filled block's scale grows as its new rows need."""
+    blocks, heads, hd = _pool(cache)
+    dev = cache.k.device
+    ldk, ldv = _head_rows(k, "k", heads, hd), _head_rows(v, "v", heads, hd)
+    rows = k.shape[0]
+    _require(v.shape[0] == rows and k.device == dev and v.device == dev, "k, v: the same rows, on the cache's device")
+    _int32s(cu, cu.numel(), "cu", dev)
+    _require(cu.numel() >= 1, "cu: at least one bound")
+    _require(slots.dtype == torch.int64 and slots.is_contiguous() and slots.numel() == rows and slots.device == dev,
+             "slots: contiguous int64, one per row")
+    with torch.cuda.device(dev):
+        call("kd_kv_store_e4m3", k.data_ptr(), ldk, v.data_ptr(), ldv, rows, cu.data_ptr(), cu.numel() - 1,
+             slots.data_ptr(), heads, hd, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+             cache.v_scale.data_ptr(), blocks, _stream(k))
+
+
+@functools.lru_cache(maxsize=4096)
+def _cache_workspace(device: int, n: int, rows: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of scratch of an ``attention_cache`` launch (on the current device, ``device``)."""
+    size = ctypes.c_int64()
+    call("kd_attention_cache_workspace", n, rows, heads, kv_heads, head_dim, ctypes.addressof(size))
+    return size.value
+
+
+def attention_cache(q: torch.Tensor, cache: KVBlocks, table: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
+                    max_q: int, scale: float, window: tuple[int, int], gate: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the new rows ``q`` (Tq, Hq, hd) over their requests' cached tokens (``kv_len`` of them, the new ones
+    included, in the blocks ``table`` names), with ``attention_varlen``'s end-aligned window; returns (Tq, Hq * hd),
+    gated by sigmoid(gate) when given. Rows of ``out`` outside every request are left as they were."""
+    blocks, hkv, hd = _pool(cache)
+    dev = cache.k.device
+    _require(q.dim() == 3, "q: bf16 (rows, heads, head_dim)")
+    tq, hq = q.shape[0], q.shape[1]
+    ldq = _head_rows(q, "q", hq, hd)
+    n = kv_len.numel()
+    _int32s(kv_len, n, "kv_len", dev)
+    _int32s(cu_q, n + 1, "cu_q", dev)
+    _block_table(table, n, dev)
+    _require(q.device == dev, f"q: on {dev}")
+    if out is None:
+        out = torch.empty(tq, hq * hd, dtype=torch.bfloat16, device=dev)
+    _require(out.shape == (tq, hq * hd) and out.dtype == torch.bfloat16 and out.stride(1) == 1 and out.device == dev,
+             f"out: bf16 ({tq}, {hq * hd}) with contiguous rows")
+    if gate is not None:
+        _require(gate.shape == (tq, hq * hd) and gate.dtype == torch.bfloat16 and gate.stride(1) == 1
+                 and gate.device == dev, f"gate: bf16 ({tq}, {hq * hd}) with contiguous rows")
+    if n == 0 or tq == 0:
+        return out
+    _require(hkv > 0 and hq % hkv == 0, "query heads must be a multiple of key/value heads")
+    with torch.cuda.device(dev):
+        size = _cache_workspace(dev.index, n, tq, hq, hkv, hd)
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+        call("kd_attention_cache", q.data_ptr(), ldq, cache.k.data_ptr(), cache.v.data_ptr(),
+             cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), blocks, table.data_ptr(),
+             max(table.stride(0), table.shape[1]), table.shape[1], cu_q.data_ptr(), kv_len.data_ptr(), n, int(max_q),
+             tq, out.data_ptr(), out.stride(0) if tq > 1 else hq * hd, _ptr(gate),
+             0 if gate is None else gate.stride(0) if tq > 1 else hq * hd, hq, hkv, hd, float(scale), int(window[0]),
+             int(window[1]), scratch.data_ptr(), size, status_word(dev).data_ptr(), _stream(q))
     return out

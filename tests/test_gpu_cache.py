@@ -1,0 +1,461 @@
+"""The state cache's operators on the GPU against their float64 restatement (tests/cache_reference.py): block tables and
+slot maps, the e4m3 block write, attention over the blocks, and the three of them together."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import cache_reference as ref
+from karpo_decision_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+BLOCK = ops.KV_BLOCK
+
+
+def ints(x, device=DEV):
+    return torch.tensor(x, dtype=torch.int32, device=device)
+
+
+def bounds(new):
+    return [0, *np.cumsum(new).tolist()]
+
+
+def dealt(lens, new, width, spare, seed=0):
+    """(table rows, free list, count): the requests' blocks dealt from a shuffled pool, the rest on the stack."""
+    g = np.random.default_rng(seed)
+    have = [-(-x // BLOCK) for x in lens]
+    total = sum(have) + spare
+    order = g.permutation(total).tolist()
+    rows, at = [], 0
+    for h in have:
+        rows.append(order[at:at + h] + [-1] * (width - h))
+        at += h
+    free = order[at:]
+    return rows, free + [-7] * (total - len(free)), len(free)
+
+
+# ------------------------------------------------------------------------------------------------ block tables
+
+
+CASES = {
+    "one token": ([4000], [1]),
+    "one new block": ([64], [1]),
+    "empty request": ([0], [0]),
+    "from nothing": ([0], [129]),
+    "mixed": ([0, 63, 64, 65, 1, 500, 0, 127], [1, 1, 1, 0, 63, 64, 0, 130]),
+    "one long": ([10], [70001]),
+    "many": ([(7 * i) % 301 for i in range(1500)], [(13 * i) % 40 for i in range(1500)]),
+}
+
+
+@pytest.mark.parametrize("name", CASES)
+@pytest.mark.parametrize("pad", [0, 5])
+def test_assign_and_its_inverse(name, pad):
+    lens, new = CASES[name]
+    width = max(-(-(a + b) // BLOCK) for a, b in zip(lens, new)) + 1
+    need = sum(-(-(a + b) // BLOCK) - -(-a // BLOCK) for a, b in zip(lens, new))
+    rows, free, count = dealt(lens, new, width, need + 3)
+    table, stack, height = ints(rows), ints(free), ints([count, 9])
+    got = ops.kv_assign(ints(lens), ints(bounds(new)), table, stack, height, sum(new) + pad)
+    kv_len, seqpos, slots, want_table, left, outcome = ref.assign(lens, new, rows, free, count, width)
+    assert [x.tolist() for x in got] == [kv_len, seqpos + [0] * pad, slots + [-1] * pad]
+    assert table.tolist() == want_table and height.tolist() == [left, outcome] and outcome == 0
+    ops.kv_release(table, got[0], ints(lens), stack, height)
+    assert table.tolist() == rows and height.tolist() == [count, 0] and stack.tolist() == free
+
+
+def test_assign_takes_nothing_when_blocks_are_missing():
+    lens, new = [70, 0, 10], [200, 65, 4]
+    rows, free, count = dealt(lens, new, 8, 4)  # 3 + 2 + 0 new blocks, 4 free
+    table, stack, height = ints(rows), ints(free), ints([count, 0])
+    kv_len, seqpos, slots = ops.kv_assign(ints(lens), ints(bounds(new)), table, stack, height, sum(new))
+    assert height.tolist() == [4, 1] and table.tolist() == rows and stack.tolist() == free
+    assert kv_len.tolist() == lens and set(slots.tolist()) == {-1}
+    assert seqpos.tolist() == ref.assign(lens, new, rows, free, count, 8)[1]
+
+
+@pytest.mark.parametrize("lens,cu,width,outcome", [
+    ([600], [0, 10], 9, ops.KV_TABLE_FULL),     # 10 blocks in a table of 9
+    ([-1, 5], [0, 4, 8], 9, ops.KV_MALFORMED),  # a negative length
+    ([5, 5], [0, 4, 2], 9, ops.KV_MALFORMED),   # bounds that fall
+    ([5], [0, 12], 9, ops.KV_MALFORMED),        # bounds past the rows
+])
+def test_assign_refuses_on_the_device(lens, cu, width, outcome):
+    table, stack, height = ints([[0] * width] * len(lens)), ints(list(range(20))), ints([20, 0])
+    before = table.clone()
+    kv_len, _, slots = ops.kv_assign(ints(lens), ints(cu), table, stack, height, 10)
+    assert height.tolist() == [20, outcome] and torch.equal(table, before)
+    assert kv_len.tolist() == lens and set(slots.tolist()) == {-1}
+
+
+def test_assign_in_place_and_release_to_a_length():
+    """kv_len may be lens; a release keeps each request's first tokens and the blocks that hold them."""
+    lens, new, keep = ints([100, 0, 64]), [300, 70, 1], [130, 0, 500]
+    rows, free, count = dealt([100, 0, 64], new, 9, 12)
+    table, stack, height = ints(rows), ints(free), ints([count, 0])
+    seqpos = torch.empty(371, dtype=torch.int64, device=DEV)
+    slots = torch.empty_like(seqpos)
+    ops.kv_assign(lens, ints(bounds(new)), table, stack, height, 371, out=(lens, seqpos, slots))
+    assert lens.tolist() == [400, 70, 65]
+    full = table.tolist()
+    taken = count - height[0].item()
+    ops.kv_release(table, lens, ints(keep), stack, height)
+    kept = [-(-130 // BLOCK), 0, 2]  # a `keep` past the length gives nothing back
+    assert table.tolist() == [row[:k] + [-1] * (9 - k) for row, k in zip(full, kept)]
+    dropped = [row[j] for row, k, h in zip(full, kept, (7, 2, 2)) for j in range(k, h)]
+    assert height.tolist() == [count - taken + len(dropped), 0]
+    assert stack.tolist()[count - taken:count - taken + len(dropped)] == dropped[::-1]
+
+
+@pytest.mark.parametrize("entry", [-1, 20])
+def test_release_of_a_block_outside_the_pool_gives_nothing_back(entry):
+    table, stack, height = ints([[3, entry, 5]]), ints(list(range(20))), ints([8, 0])
+    before, held = table.clone(), stack.clone()
+    ops.kv_release(table, ints([150]), ints([0]), stack, height)
+    assert height.tolist() == [8, ops.KV_MALFORMED] and torch.equal(table, before) and torch.equal(stack, held)
+
+
+def test_release_onto_a_full_stack_gives_nothing_back():
+    table, stack, height = ints([[3, 4, 5]]), ints(list(range(6))), ints([4, 0])
+    ops.kv_release(table, ints([150]), ints([0]), stack, height)
+    assert height.tolist() == [4, ops.KV_MALFORMED] and table.tolist() == [[3, 4, 5]]
+
+
+# ------------------------------------------------------------------------------------------------ the write
+
+
+def pool(blocks, heads, hd, seed, junk=True):
+    """A pool of random codes and scales 2^-6 .. 2^2; with ``junk`` some codes are NaN, as unwritten memory holds."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    k, v = (torch.randint(0, 256, (blocks, heads, BLOCK, hd), generator=g, device=DEV, dtype=torch.uint8)
+            for _ in range(2))
+    if not junk:
+        k, v = (torch.where(x & 0x7f == 0x7f, x & 0x80, x) for x in (k, v))
+    ks, vs = (torch.randint(-6, 3, (blocks, heads), generator=g, device=DEV) for _ in range(2))
+    ones = torch.ones(blocks, heads, device=DEV)
+    return ops.KVBlocks(k.view(torch.float8_e4m3fn), v.view(torch.float8_e4m3fn), torch.ldexp(ones, ks),
+                        torch.ldexp(ones, vs))
+
+
+def placed(lens, new, seed=0, spare=3):
+    """(blocks in the pool, table, slots) of requests holding ``lens`` tokens that get ``new`` rows."""
+    width = max(1, max(-(-(a + b) // BLOCK) for a, b in zip(lens, new)))
+    grown = [a + b for a, b in zip(lens, new)]
+    rows, free, _ = dealt(grown, new, width, spare, seed)
+    slots = [rows[i][p // BLOCK] * BLOCK + p % BLOCK for i, (a, b) in enumerate(zip(lens, new)) for p in range(a, a + b)]
+    return len(free), rows, slots
+
+
+def check_store(k, v, cu, slots, cache, rows):
+    before = [x.clone() for x in cache]
+    ops.kv_store_e4m3(k, v, ints(cu), torch.tensor(slots, dtype=torch.int64, device=DEV), cache)
+    kd, vd = k.double().cpu(), v.double().cpu()
+    for got, scale, was, was_scale, x, other, is_key in (
+            (cache.k, cache.k_scale, before[0], before[2], kd, vd, True),
+            (cache.v, cache.v_scale, before[1], before[3], vd, kd, False)):
+        values, scales = ref.store(x, other, cu, slots, was.double().cpu(), was_scale.double().cpu(), is_key)
+        assert torch.equal(scale.double().cpu(), scales)
+        assert torch.equal(got.double().cpu().nan_to_num(1e9), values.nan_to_num(1e9))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("heads", [1, 5])
+@pytest.mark.parametrize("lens,new", [([0], [1]), ([63], [2]), ([64], [64]), ([10, 0, 70, 5], [200, 0, 1, 64]),
+                                      ([1] * 70, [3] * 70)])
+def test_store_matches_its_definition(hd, heads, lens, new):
+    blocks, _, slots = placed(lens, new, seed=hd)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(hd + heads)
+    rows = sum(new)
+    k = (torch.randn(rows, heads, hd, generator=g, device=DEV) *
+         torch.exp2(3 * torch.randn(rows, heads, 1, generator=g, device=DEV))).bfloat16()
+    v = torch.randn(rows, heads, hd, generator=g, device=DEV).bfloat16()
+    check_store(k, v, bounds(new), slots, pool(blocks, heads, hd, 3), rows)
+
+
+@pytest.mark.parametrize("fill", [0.0, 448.0, 449.0, 447.0, 2.0 ** -110, 3.3e38, 2.0 ** -133, math.inf, math.nan])
+def test_store_of_special_values(fill):
+    """Zeros, the largest magnitude that still fits a scale, one past it, the ends of bf16's range, infinities, NaN."""
+    lens, new = [0, 30], [5, 7]
+    blocks, _, slots = placed(lens, new)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    k = torch.randn(12, 2, 64, generator=g, device=DEV).bfloat16()
+    v = torch.randn(12, 2, 64, generator=g, device=DEV).bfloat16()
+    k[2, 0, 5] = fill
+    v[7, 1, 9] = -fill
+    if fill in (0.0, 2.0 ** -133):
+        k[:5] = fill
+    cache = pool(blocks, 2, 64, 4, junk=False)
+    check_store(k, v, bounds(new), slots, cache, 12)
+
+
+def test_store_grows_a_scale_and_keeps_what_it_can():
+    """A half-filled block's old codes move to the larger scale: exact where they stay normal, rounded where not."""
+    cache = ops.kv_blocks(2, 1, 64, DEV)
+    slots = list(range(64))
+    k = torch.randn(64, 1, 64, generator=torch.Generator().manual_seed(0)).to(DEV).bfloat16()
+    k[32:] *= 2.0 ** 14
+    check_store(k[:32], k[:32], [0, 32], slots[:32], cache, 32)
+    check_store(k[32:], k[32:], [0, 32], slots[32:], cache, 32)
+
+
+def test_store_reads_strided_rows_and_leaves_the_rest():
+    """k and v as columns of one projection; rows behind the last request and requests without slots are not written."""
+    lens, new = [10, 20, 0], [70, 3, 9]
+    blocks, _, slots = placed(lens, new)
+    slots[70:73] = [-1] * 3  # the second request got no blocks
+    g = torch.Generator(device=DEV)
+    g.manual_seed(5)
+    qkv = torch.randn(100, 8 * 64, generator=g, device=DEV).bfloat16()
+    k, v = (qkv[:, a:a + 128].unflatten(1, (2, 64)) for a in (128, 256))
+    check_store(k, v, bounds(new), slots + [0] * 18, pool(blocks, 2, 64, 6), 100)
+
+
+# ------------------------------------------------------------------------------------------------ attention
+
+
+def make(lens, new, hq, hkv, hd, seed=0, spread=1.0, pad=0):
+    """Requests' cached tokens in a pool whose unwritten places hold anything, NaN codes too."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    blocks, rows, _ = placed(lens, [0] * len(lens), seed)
+    cache = pool(blocks, hkv, hd, seed + 1)
+    for codes, scale, apart in ((cache.k, cache.k_scale, 1.0), (cache.v, cache.v_scale, spread)):
+        for i, n in enumerate(lens):
+            for j in range(-(-n // BLOCK)):
+                live = min(BLOCK, n - j * BLOCK)
+                x = torch.randn(hkv, live, hd, generator=g, device=DEV) * 60.0
+                codes[rows[i][j], :, :live] = x.clamp(-448, 448).to(torch.float8_e4m3fn)
+                scale[rows[i][j]] = 2.0 ** -6 * torch.exp2(torch.round(
+                    apart * torch.randn(hkv, generator=g, device=DEV)))
+    q = (1.5 * torch.randn(sum(new) + pad, hq, hd, generator=g, device=DEV)).bfloat16()
+    gate = torch.randn(sum(new) + pad, hq * hd, generator=g, device=DEV).bfloat16()
+    return cache, ints(rows), q, gate
+
+
+def tolerance(want, spread, size, hd, keys):
+    """What the definition's value may move by (derived, not fitted); spread = sum p |v| / sum p, size = the largest
+    sum |q k| * scale:
+    - the output's rounding to bf16: 2^-8 |o|;
+    - the probabilities' rounding to f16: 2^-11 relative each, so 2^-11 spread; those below f16's normal numbers, 2^-29
+      of the row's largest scaled probability, lose at most 2^-40 of it each: keys * 2^-40 of 448 block units, which the
+      largest one's own term in spread covers unless its codes are all under 2^-6;
+    - a score's error d moves every probability by at most 2 d relative: d <= (hd / 8) 2^-23 size for the products'
+      float32 sums (hd / 16 products of 16 terms, each added with an error of one unit) and 2^-22 size for its scaling,
+      the subtraction of the maximum and the exponential;
+    - the float32 sums over keys: keys / 16 additions of 2^-23 relative at most, in numerator and denominator."""
+    d = (hd / 8 * 2.0 ** -23 + 2.0 ** -22) * size
+    return 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -14 + keys / 8 * 2.0 ** -23 + 2 * d) * spread + 1e-30
+
+
+def check_attention(lens, new, hq, hkv, hd, window=(-1, 0), gated=False, seed=0, table=None, **kw):
+    cache, rows, q, gate = make(lens, new, hq, hkv, hd, seed, **kw)
+    table = rows if table is None else table(rows)
+    scale = hd ** -0.5
+    cu = bounds(new)
+    got = ops.attention_cache(q, cache, table, ints(cu), ints(lens), max(new), scale, window,
+                              gate=gate if gated else None)
+    ops.check_status(DEV)
+    want, spread, size = ref.attention(q, cache.k.double(), cache.v.double(), cache.k_scale, cache.v_scale, table, cu, lens,
+                                 scale, window, gate if gated else None)
+    n = cu[-1]
+    err = (got[:n].double() - want[:n]).abs()
+    tol = tolerance(want[:n], spread[:n], size, hd, max(lens))
+    assert torch.isfinite(got[:n]).all()
+    worst = (err / tol).max().item() if n else 0.0
+    assert worst <= 1.0, f"error {worst:.3f} of the tolerance"
+    return got
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (4, 4), (6, 2), (16, 2), (5, 1)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_attention_of_single_tokens(hd, hq, hkv, gated):
+    check_attention([1, 64, 65, 130, 1000, 3, 2049], [1] * 7, hq, hkv, hd, gated=gated)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (8, 2), (3, 1)])
+@pytest.mark.parametrize("window", [(-1, 0), (-1, -1), (20, 0), (0, 0), (63, 5), (200, -1)])
+def test_attention_of_questions(hd, hq, hkv, window):
+    """Ragged questions about states of all lengths, causal, windowed and whole; a request without new rows."""
+    check_attention([40, 129, 700, 64, 1500], [40, 17, 33, 0, 70], hq, hkv, hd, window, gated=hq == 8)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+def test_attention_of_a_whole_prompt(hd):
+    check_attention([391], [391], 4, 2, hd)
+    check_attention([1111, 300], [1111, 300], 2, 2, hd, window=(127, 0), gated=True)
+
+
+def test_attention_of_one_long_state():
+    check_attention([70001], [1], 8, 2, 128)
+    check_attention([33000], [65], 8, 2, 128, gated=True)
+
+
+def test_attention_of_many_requests():
+    g = np.random.default_rng(3)
+    lens = g.integers(1, 400, 300).tolist()
+    check_attention(lens, [1] * 300, 8, 4, 64)
+    check_attention(lens, [min(n, 3) for n in lens], 8, 4, 128, window=(100, 0))
+
+
+def test_rows_that_see_nothing_are_zero():
+    """No cached token, fewer cached tokens than rows (the first rows lie before key 0), a state whose blocks are all
+    absent; the gate does not matter there."""
+    got = check_attention([0, 3, 70], [5, 9, 2], 4, 2, 128, gated=True,
+                          table=lambda t: torch.cat([t[:2], torch.full_like(t[2:], -1)]))
+    assert not got[:5].any() and not got[5:11].any() and not got[14:].any() and got[11:14].any()
+
+
+def test_absent_blocks_are_not_seen():
+    """Table entries outside the pool, negative and too large, in the middle of a state."""
+    def holes(t):
+        t = t.clone()
+        t[0, 1], t[0, 4], t[1, 0] = -1, 10 ** 9, -5
+        return t
+
+    check_attention([500, 130], [3, 40], 4, 2, 128, table=holes)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [30, 41]])
+def test_scales_far_apart(new):
+    """Blocks whose value scales differ by up to 2^40 or so: the largest values need not have the largest probability."""
+    check_attention([640, 333], new, 8, 2, 128, spread=8.0)
+
+
+def test_a_nan_token_reaches_only_rows_that_see_it():
+    cache = ops.kv_blocks(8, 2, 128, DEV)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(2)
+    k, v, q = (torch.randn(200, 2, 128, generator=g, device=DEV).bfloat16() for _ in range(3))
+    v[120, 1, 7] = math.nan
+    table = ints([[5, 0, 7, 2]])
+    t = torch.arange(200, device=DEV)
+    ops.kv_store_e4m3(k, v, ints([0, 200]), table[0].long()[t // 64] * 64 + t % 64, cache)
+    out = ops.attention_cache(q, cache, table, ints([0, 200]), ints([200]), 200, 0.1, (40, 0)).float()
+    assert torch.isfinite(out[:, :128]).all()
+    nan = out[:, 128:].isnan()
+    assert nan[120:161].all() and not nan[:120].any() and not nan[161:].any()
+
+
+def test_strides_and_rows_behind_the_last_request():
+    """q, gate and out as columns of wider buffers, a table with a row stride, rows of padding left as they were."""
+    lens, new = [300, 77], [5, 20]
+    cache, table, q, gate = make(lens, new, 4, 2, 64, pad=7)
+    wide = torch.zeros(2, 40, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    qs = torch.zeros(32, 768, dtype=torch.bfloat16, device=DEV)
+    gs, outs = torch.zeros_like(qs), torch.full_like(qs, 5.0)
+    qs[:, 256:512], gs[:, 512:] = q.reshape(32, 256), gate
+    args = (ints(bounds(new)), ints(lens), 20, 0.125, (-1, 0))
+    want = ops.attention_cache(q, cache, table, *args, gate=gate)
+    got = ops.attention_cache(qs[:, 256:512].unflatten(1, (4, 64)), cache, wide[:, :table.shape[1]], *args,
+                              gate=gs[:, 512:], out=outs[:, 256:512])
+    assert torch.equal(got[:25], want[:25])
+    assert (outs[25:] == 5).all() and (outs[:, :256] == 5).all() and (outs[:, 512:] == 5).all()
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 9, 60]])
+def test_repeated_calls_are_equal_and_streams_do_not_mix(new):
+    """Bit-equal results from launches in flight on two streams at once, again and again."""
+    cache, table, q, gate = make([900, 64, 5000], new, 8, 2, 128)
+    args = (cache, table, ints(bounds(new)), ints([900, 64, 5000]), max(new), 0.1, (-1, 0))
+    want = ops.attention_cache(q, *args, gate=gate)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(ops.attention_cache(q, *args, gate=gate))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in got)
+
+
+# ------------------------------------------------------------------------------------------------ together
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_states_grown_in_pieces(hd):
+    """Assign, store and attend over the same tokens in different pieces, as a captured graph would run each step: the
+    outputs stay within rounding of the definition on the cache as it stood, and giving blocks back leaves the stack
+    full."""
+    hq, hkv, total = 4, 2, [150, 70, 333]
+    g = torch.Generator(device=DEV)
+    g.manual_seed(8)
+    q = [torch.randn(n, hq, hd, generator=g, device=DEV).bfloat16() for n in total]
+    k = [torch.randn(n, hkv, hd, generator=g, device=DEV).bfloat16() for n in total]
+    v = [torch.randn(n, hkv, hd, generator=g, device=DEV).bfloat16() for n in total]
+    cache = pool(16, hkv, hd, 9)
+    table, stack, height = ints([[-1] * 6] * 3), ints(list(range(16))), ints([16, 0])
+    lens, done = ints([0, 0, 0]), [0, 0, 0]
+    for step in ([100, 1, 200], [1, 0, 1], [1, 69, 100], [48, 0, 32]):
+        new = list(step)
+        pick = [slice(d, d + s) for d, s in zip(done, new)]
+        rows = [torch.cat([x[i][pick[i]] for i in range(3)]) for x in (q, k, v)]
+        cu = ints(bounds(new))
+        kv_len, seqpos, slots = ops.kv_assign(lens, cu, table, stack, height, sum(new))
+        ops.kv_store_e4m3(rows[1], rows[2], cu, slots, cache)
+        out = ops.attention_cache(rows[0], cache, table, cu, kv_len, max(new), hd ** -0.5, (-1, 0))
+        done = [d + s for d, s in zip(done, new)]
+        assert kv_len.tolist() == done
+        want, spread, size = ref.attention(rows[0], cache.k.double(), cache.v.double(), cache.k_scale, cache.v_scale, table,
+                                     bounds(new), done, hd ** -0.5, (-1, 0))
+        tol = tolerance(want, spread, size, hd, 333)
+        assert ((out.double() - want).abs() <= tol).all()
+        lens = kv_len
+    # what the cache holds is the rows within e4m3's rounding: half a step, 2^-4 relative, and under a block's smallest
+    # normal code (2^-6) half of its 2^-9 steps, each a second time where a scale grew
+    for i, n in enumerate(total):
+        pos = torch.arange(n, device=DEV)
+        ids = table[i].long()[pos // BLOCK]
+        for codes, scale, x in ((cache.k, cache.k_scale, k[i]), (cache.v, cache.v_scale, v[i])):
+            held = codes[ids, :, pos % BLOCK].double() * scale[ids].double()[:, :, None]
+            step = 2.0 ** -9 * scale[ids].double()[:, :, None]
+            assert ((held - x.double()).abs() <= 2 * (2.0 ** -4 * x.double().abs() + step)).all()
+    ops.kv_release(table, lens, ints([0, 0, 0]), stack, height)
+    assert height.tolist() == [16, 0] and sorted(stack.tolist()) == list(range(16)) and (table == -1).all()
+
+
+def test_a_captured_step_follows_the_lengths_on_the_device():
+    """One graph of assign, store and attend, replayed as the requests grow by a token each."""
+    hq, hkv, hd, n = 4, 2, 64, 3
+    cache = ops.kv_blocks(24, hkv, hd, DEV)
+    table, stack, height = ints([[-1] * 6] * n), ints(list(range(24))), ints([24, 0])
+    lens, cu = ints([0] * n), ints([0, 1, 2, 3])
+    q = torch.zeros(n, hq, hd, dtype=torch.bfloat16, device=DEV)
+    k, v = (torch.zeros(n, hkv, hd, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    seqpos, slots = (torch.zeros(n, dtype=torch.int64, device=DEV) for _ in range(2))
+
+    def step():
+        ops.kv_assign(lens, cu, table, stack, height, n, out=(lens, seqpos, slots))
+        ops.kv_store_e4m3(k, v, cu, slots, cache)
+        return ops.attention_cache(q, cache, table, cu, lens, 1, hd ** -0.5, (-1, 0))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    ops.kv_release(table, lens, ints([0] * n), stack, height)
+    lens.zero_()
+    g = torch.Generator(device=DEV)
+    g.manual_seed(4)
+    for i in range(130):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=g, device=DEV))
+        graph.replay()
+        if i in (0, 1, 62, 63, 64, 65, 129):
+            assert lens.tolist() == [i + 1] * n and seqpos.tolist() == [i] * n and height[1].item() == 0
+            want, spread, size = ref.attention(q, cache.k.double(), cache.v.double(), cache.k_scale, cache.v_scale, table,
+                                         [0, 1, 2, 3], [i + 1] * n, hd ** -0.5, (-1, 0))
+            tol = tolerance(want, spread, size, hd, 130)
+            assert ((out.double() - want).abs() <= tol).all()
