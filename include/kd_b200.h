@@ -280,10 +280,10 @@ int kd_kv_store_e4m3(const void* k, int64_t ldk, const void* v, int64_t ldv, int
                      int num_requests, const int64_t* slots, int num_heads_kv, int head_dim, void* k_codes,
                      void* v_codes, float* k_scale, float* v_scale, int64_t num_blocks, cudaStream_t stream);
 
-/* *bytes (a host int64): the scratch kd_attention_cache needs on the current device, 16-byte aligned, one area per
- * launch in flight. */
-int kd_attention_cache_workspace(int num_requests, int64_t total_q, int num_heads_q, int num_heads_kv, int head_dim,
-                                 int64_t* bytes);
+/* *bytes (a host int64): the scratch kd_attention_cache needs on the current device for these sizes, 16-byte aligned,
+ * one area per launch in flight. */
+int kd_attention_cache_workspace(int num_requests, int max_q, int64_t total_q, int num_heads_q, int num_heads_kv,
+                                 int head_dim, int64_t* bytes);
 
 /* Attention of new rows over their requests' cached tokens, the visibility rule and the gate of kd_attention_varlen with
  * Lk = kv_len[i] (new rows stored first: a causal row sees itself). q (total_q, heads_q, head_dim) bf16; cu_q int32

@@ -54,7 +54,7 @@ SIGNATURES: dict[str, list] = {
     "kd_kv_assign": [P, P, c_int, c_int64, P, c_int64, c_int, P, c_int, P, P, P, P, P],
     "kd_kv_release": [P, c_int64, c_int, P, P, c_int, P, c_int, P, P],
     "kd_kv_store_e4m3": [P, c_int64, P, c_int64, c_int64, P, c_int, P, c_int, c_int, P, P, P, P, c_int64, P],
-    "kd_attention_cache_workspace": [c_int, c_int64, c_int, c_int, c_int, P],
+    "kd_attention_cache_workspace": [c_int, c_int, c_int64, c_int, c_int, c_int, P],
     "kd_attention_cache": [P, c_int64, P, P, P, P, c_int64, P, c_int64, c_int, P, P, c_int, c_int, c_int64, P, c_int64,
                            P, c_int64, c_int, c_int, c_int, c_float, c_int, c_int, P, c_int64, P, P],
     "kd_marker_norm": [P, c_int, P, c_int64, P, c_int, c_float, P, P],

@@ -20,16 +20,11 @@
 // Probabilities are rounded to f16 relative to the largest *scaled* probability p 2^e_v met (11 bits, exponents down
 // to 2^-39 of it), so the blocks' value scales need no product of their own; the sum of the probabilities stays in
 // float32, unrounded.
-#include <cuda_fp16.h>
-
-#include "common.cuh"
-#include "kd_internal.h"
+#include "cache_attention.cuh"
 
 namespace kd {
 namespace ca {
 
-constexpr int BN = KD_KV_BLOCK;  // keys per tile: one block
-constexpr int RT = 16;           // query rows per tile
 constexpr float P_SCALE = 32768.f;  // f16 probabilities hold p * 2^15 (at most 2^15; subnormal below 2^-29)
 
 template <int HD>
@@ -49,49 +44,6 @@ struct Cfg {
   static constexpr int PARTIAL = RT * (HD + 3);  // floats of one group's partial: O, then (m, M, l) per row
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
-
-struct Args {
-  const __nv_bfloat16* q;
-  __nv_bfloat16* out;
-  const __nv_bfloat16* gate;
-  int64_t ldq, ldo, ldg;
-  const int32_t* table;
-  int64_t ldt;
-  int width;
-  const int32_t* cu;
-  const int32_t* kv_len;
-  int n;
-  int64_t total_q;
-  const float* k_scale;
-  const float* v_scale;
-  int blocks;
-  int hq, hkv, group;
-  float scale_log2;
-  int left, right;
-  int64_t* tile_cu;   // [n + 1] key tiles of the requests before (of one key/value head)
-  int32_t* item_cu;   // [n + 1] 16-row tiles of the requests before
-  float* partials;
-  int* status;
-};
-
-struct Request {
-  int q0, lq, lk;
-  int nrt;          // 16-row tiles
-  int first, tiles; // key tiles that any row may see
-};
-
-KD_DEVICE Request request(const Args& a, int i) {
-  Request r;
-  r.q0 = a.cu[i];
-  const int end = a.cu[i + 1];
-  r.lq = r.q0 < 0 || end > a.total_q ? 0 : max(end - r.q0, 0);
-  r.lk = (int)min((int64_t)max(a.kv_len[i], 0), (int64_t)a.width * BN);
-  r.nrt = (int)(((int64_t)r.lq * a.group + RT - 1) / RT);
-  const int kmin = a.left >= 0 ? max(0, r.lk - r.lq - a.left) : 0;
-  r.first = kmin / BN;
-  r.tiles = r.lq > 0 && r.lk > kmin ? (r.lk - 1) / BN - r.first + 1 : 0;
-  return r;
-}
 
 // A position in the list of key tiles: request > key/value head > 16-row tile > key tile. `advance(g)` moves forward to
 // the item holding tile g.
@@ -135,30 +87,6 @@ struct Cursor {
   }
 };
 
-// CTAs that take part: every one of them has a tile, so no partial of an item is missing.
-KD_DEVICE int64_t shares(int64_t total, int ctas) { return total < ctas ? (total > 0 ? total : 1) : ctas; }
-
-KD_DEVICE float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// 2^e for whole e, clamped to the normal float32 exponents.
-KD_DEVICE float pow2i(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
-// The exponent of a scale (a power of two).
-KD_DEVICE int exponent_of(float s) { return (int)((__float_as_uint(s) >> 23) & 255u) - 127; }
-
-// Four e4m3 codes to two f16 pairs (exact).
-KD_DEVICE void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 a, b;\n\t"
-      "mov.b32 {a, b}, %2;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-      : "=r"(lo), "=r"(hi)
-      : "r"(w));
-}
-
 KD_DEVICE void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -178,11 +106,6 @@ KD_DEVICE void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint3
       "%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-KD_DEVICE uint32_t pack_f16x2(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 KD_DEVICE void group_sync(int id, int threads) {
@@ -508,7 +431,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
         float factor[2], alpha_o[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float mul = q_scale[u] * ti.k_scale * a.scale_log2;
+          const float mul = score_factor(q_scale[u], ti.k_scale, a.scale_log2);
           float mx = -INFINITY;
 #pragma unroll
           for (int j = 0; j < 8; ++j)
@@ -718,6 +641,10 @@ __global__ void __launch_bounds__(128) join_kernel(Args a, int ctas) {
   }
 }
 
+// Whether the requests' rows per key/value head fit one 16-row tile: the kernel of this file. Both kernels are right for
+// any rows.
+static bool few_rows(int max_q, int group) { return (int64_t)max_q * group <= RT; }
+
 // Bytes of scratch: the two request arrays, then one partial per (item + CTA, key group).
 template <int HD>
 int64_t few_rows_items(int n, int64_t total_q, int hkv, int group) {
@@ -772,19 +699,25 @@ int launch(Args a, const void* k_codes, const void* v_codes, uint8_t* ws, int64_
 
 using namespace kd;
 
-extern "C" int kd_attention_cache_workspace(int num_requests, int64_t total_q, int num_heads_q, int num_heads_kv,
-                                            int head_dim, int64_t* bytes) {
-  if (!bytes || num_requests < 0 || total_q < 0 || num_heads_q <= 0 || num_heads_kv <= 0 || num_heads_q % num_heads_kv)
+extern "C" int kd_attention_cache_workspace(int num_requests, int max_q, int64_t total_q, int num_heads_q,
+                                            int num_heads_kv, int head_dim, int64_t* bytes) {
+  if (!bytes || num_requests < 0 || max_q < 0 || total_q < 0 || num_heads_q <= 0 || num_heads_kv <= 0 ||
+      num_heads_q % num_heads_kv)
     return set_error(KD_ERR_ARGUMENT, "attention_cache_workspace: sizes, heads or a null pointer");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512)
+    return set_error(KD_ERR_ARGUMENT, "attention_cache_workspace: head_dim must be 64, 128, 256 or 512");
   int dev = 0;
   if (int rc = record_cuda_error(cudaGetDevice(&dev), "attention_cache_workspace: device")) return rc;
-  const int ctas = num_sms(dev), group = num_heads_q / num_heads_kv;
+  const int sms = num_sms(dev), group = num_heads_q / num_heads_kv;
+  if (!ca::few_rows(max_q, group)) {
+    *bytes = ca::row_tiles_workspace(head_dim, num_requests, sms);
+    return KD_OK;
+  }
   switch (head_dim) {
-    case 64: *bytes = ca::workspace_bytes<64>(num_requests, total_q, num_heads_kv, group, ctas); break;
-    case 128: *bytes = ca::workspace_bytes<128>(num_requests, total_q, num_heads_kv, group, ctas); break;
-    case 256: *bytes = ca::workspace_bytes<256>(num_requests, total_q, num_heads_kv, group, ctas); break;
-    case 512: *bytes = ca::workspace_bytes<512>(num_requests, total_q, num_heads_kv, group, ctas); break;
-    default: return set_error(KD_ERR_ARGUMENT, "attention_cache_workspace: head_dim must be 64, 128, 256 or 512");
+    case 64: *bytes = ca::workspace_bytes<64>(num_requests, total_q, num_heads_kv, group, sms); break;
+    case 128: *bytes = ca::workspace_bytes<128>(num_requests, total_q, num_heads_kv, group, sms); break;
+    case 256: *bytes = ca::workspace_bytes<256>(num_requests, total_q, num_heads_kv, group, sms); break;
+    default: *bytes = ca::workspace_bytes<512>(num_requests, total_q, num_heads_kv, group, sms); break;
   }
   return KD_OK;
 }
@@ -796,8 +729,7 @@ extern "C" int kd_attention_cache(const void* q, int64_t ldq, const void* k_code
                                   const void* gate, int64_t ldg, int num_heads_q, int num_heads_kv, int head_dim,
                                   float scale, int window_left, int window_right, void* workspace,
                                   int64_t workspace_bytes, int* status, cudaStream_t stream) {
-  (void)max_q;
-  if (num_requests < 0 || total_q < 0 || total_q > 0x3fffffff || num_blocks < 0 || table_width < 0 ||
+  if (num_requests < 0 || max_q < 0 || total_q < 0 || total_q > 0x3fffffff || num_blocks < 0 || table_width < 0 ||
       ld_table < table_width)
     return set_error(KD_ERR_ARGUMENT, "attention_cache: negative sizes, or a table narrower than its width");
   if (num_requests == 0 || total_q == 0) return KD_OK;
@@ -846,11 +778,13 @@ extern "C" int kd_attention_cache(const void* q, int64_t ldq, const void* k_code
   a.item_cu = nullptr;
   a.partials = nullptr;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512)
+    return set_error(KD_ERR_ARGUMENT, "attention_cache: head_dim must be 64, 128, 256 or 512");
+  if (!ca::few_rows(max_q, a.group)) return ca::row_tiles(head_dim, a, k_codes, v_codes, ws, workspace_bytes, stream);
   switch (head_dim) {
     case 64: return ca::launch<64>(a, k_codes, v_codes, ws, workspace_bytes, stream);
     case 128: return ca::launch<128>(a, k_codes, v_codes, ws, workspace_bytes, stream);
     case 256: return ca::launch<256>(a, k_codes, v_codes, ws, workspace_bytes, stream);
-    case 512: return ca::launch<512>(a, k_codes, v_codes, ws, workspace_bytes, stream);
-    default: return set_error(KD_ERR_ARGUMENT, "attention_cache: head_dim must be 64, 128, 256 or 512");
+    default: return ca::launch<512>(a, k_codes, v_codes, ws, workspace_bytes, stream);
   }
 }

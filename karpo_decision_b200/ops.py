@@ -528,10 +528,10 @@ def kv_store_e4m3(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, slots: tor
 
 
 @functools.lru_cache(maxsize=4096)
-def _cache_workspace(device: int, n: int, rows: int, heads: int, kv_heads: int, head_dim: int) -> int:
+def _cache_workspace(device: int, n: int, max_q: int, rows: int, heads: int, kv_heads: int, head_dim: int) -> int:
     """Bytes of scratch of an ``attention_cache`` launch (on the current device, ``device``)."""
     size = ctypes.c_int64()
-    call("kd_attention_cache_workspace", n, rows, heads, kv_heads, head_dim, ctypes.addressof(size))
+    call("kd_attention_cache_workspace", n, max_q, rows, heads, kv_heads, head_dim, ctypes.addressof(size))
     return size.value
 
 
@@ -562,7 +562,7 @@ def attention_cache(q: torch.Tensor, cache: KVBlocks, table: torch.Tensor, cu_q:
         return out
     _require(hkv > 0 and hq % hkv == 0, "query heads must be a multiple of key/value heads")
     with torch.cuda.device(dev):
-        size = _cache_workspace(dev.index, n, tq, hq, hkv, hd)
+        size = _cache_workspace(dev.index, n, int(max_q), tq, hq, hkv, hd)
         scratch = torch.empty(size, dtype=torch.uint8, device=dev)
         call("kd_attention_cache", q.data_ptr(), ldq, cache.k.data_ptr(), cache.v.data_ptr(),
              cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), blocks, table.data_ptr(),

@@ -48,7 +48,7 @@ def test_store_refusals():
 def test_attention_refusals():
     #     q  ldq  k  v  ks vs blk tab ldt w  cu kv n mq tq  out ldo gate ldg hq hkv hd scale l  r  ws bytes st stream
     ok = [P, 512, P, P, P, P, 5, P, 8, 8, P, P, 2, 1, 10, P, 512, P, 512, 4, 2, 128, 0.1, -1, 0, P, 1 << 40, P, None]
-    for at, bad in ((1, 511), (1, 256), (6, 0), (6, -1), (6, 2 ** 31), (8, 7), (9, -1), (9, 2 ** 25), (12, -1), (14, -1),
+    for at, bad in ((1, 511), (1, 256), (6, 0), (6, -1), (6, 2 ** 31), (8, 7), (9, -1), (9, 2 ** 25), (12, -1), (13, -1), (14, -1),
                     (14, 2 ** 30), (16, 500), (18, 130), (19, 3), (19, 0), (20, 0), (21, 96), (22, 0.0), (22, -1.0),
                     (22, math.nan), (0, None), (0, P + 2), (2, P + 8), (3, None), (4, None), (5, None), (7, None),
                     (10, None), (11, None), (15, None), (17, P + 4), (25, None), (25, P + 8), (26, 16), (27, None)):
@@ -56,7 +56,8 @@ def test_attention_refusals():
         args[at] = bad
         assert "attention_cache" in refused("kd_attention_cache", *args), (at, bad)
     size = ctypes.c_int64()
-    for bad in ((-1, 10, 4, 2, 128), (1, -1, 4, 2, 128), (1, 10, 3, 2, 128), (1, 10, 4, 0, 128)):
+    for bad in ((-1, 1, 10, 4, 2, 128), (1, -1, 10, 4, 2, 128), (1, 1, -1, 4, 2, 128), (1, 1, 10, 3, 2, 128),
+                (1, 1, 10, 4, 0, 128), (1, 1, 10, 4, 2, 96)):
         assert "workspace" in refused("kd_attention_cache_workspace", *bad, ctypes.addressof(size))
 
 

@@ -329,6 +329,32 @@ def test_scales_far_apart(new):
     check_attention([640, 333], new, 8, 2, 128, spread=8.0)
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_zero_queries_and_zero_blocks(rows):
+    """Every score 0 (a zero query, blocks of zeros with the smallest scale): the mean of the values, not NaN."""
+    cache = ops.kv_blocks(4, 1, 128, DEV)
+    cache.k_scale.fill_(2.0 ** -100)
+    cache.v.fill_(2.0)
+    q = torch.zeros(rows, 2, 128, dtype=torch.bfloat16, device=DEV)
+    out = ops.attention_cache(q, cache, ints([[2, 0, 1]]), ints([0, rows]), ints([150]), rows, 0.1, (-1, 0))
+    assert (out == 2).all()
+
+
+@pytest.mark.parametrize("new", [[3, 1], [60, 41]])
+def test_scales_at_the_ends_of_their_range(new):
+    """Value scales 2^-100 beside 2^100: small probabilities of large values, and the reverse."""
+    cache, table, q, _ = make([640, 333], new, 4, 2, 64)
+    for i, n in enumerate((640, 333)):
+        cache.v_scale[table[i, :-(-n // BLOCK)].long()] = 2.0 ** -100
+    cache.v_scale[table[0, 3].long()] = 2.0 ** 100
+    cache.v_scale[table[1, 0].long()] = 2.0 ** 20
+    cu, scale = bounds(new), 0.125
+    got = ops.attention_cache(q, cache, table, ints(cu), ints([640, 333]), max(new), scale, (-1, 0))
+    want, spread, size = ref.attention(q, cache.k.double(), cache.v.double(), cache.k_scale, cache.v_scale, table, cu,
+                                       [640, 333], scale, (-1, 0))
+    assert ((got.double() - want).abs() <= tolerance(want, spread, size, 64, 640)).all()
+
+
 def test_a_nan_token_reaches_only_rows_that_see_it():
     cache = ops.kv_blocks(8, 2, 128, DEV)
     g = torch.Generator(device=DEV)
