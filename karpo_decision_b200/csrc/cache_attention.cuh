@@ -80,6 +80,11 @@ KD_DEVICE void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
       : "r"(w));
 }
 
+// Two values as packed e4m3 codes, round to nearest even, saturating at +-448; NaN stays NaN.
+KD_DEVICE uint32_t e4m3_pair(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+
 // scale * log2(e) times the power-of-two scales of a query row and a block's keys: finite and not 0, so that it times a
 // masked -inf or a score of 0 is no NaN.
 KD_DEVICE float score_factor(float q_scale, float k_scale, float scale_log2) {

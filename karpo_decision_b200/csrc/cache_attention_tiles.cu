@@ -2,12 +2,16 @@
 // formulas and the visibility rule of cache_attention.cu, on the 5th-generation tensor cores.
 //
 // The rows of a request that share a key/value head (row r is token r / group, query head r % group of the head) are cut
-// into tiles of 128, so a group's heads read the codes together. S = Q K^T and O += P V are tcgen05.mma in f16 with S, P
-// and O in tensor memory, as in attention.cu; what differs is where K and V come from. Converter warps load a block's
-// codes (16 bytes a thread and piece, the next tile's loads in flight while a tile is converted, the tiles after it on
-// their way into L2), turn them into f16 exactly (two per instruction) and write the 128-byte swizzled tiles that the
-// descriptors name: the codes cross HBM and L2 once as bytes, and the conversion hides under the products. The blocks'
-// scales never touch the elements: the key scale joins the softmax scale, the value scale the probabilities.
+// into tiles of 128, so a group's heads read the codes together. S = Q K^T and O += P V are tcgen05.mma with S, P and O in
+// tensor memory, as in attention.cu; what differs is the operands. The keys' codes go to the tensor cores as they are
+// (kind::f8f6f4, tiles by TMA): a query row is split into two e4m3 rows, its rounding and the rest, q 2^-e = hi + lo with
+// the row's largest magnitude in (224, 448]. That is exact for every bf16 element within 2^-10 of the row's largest and
+// off by at most 2^-10 (2^-18 of the largest) below, and two products at the 8-bit rate cost what one in 16 bits does.
+// The values meet probabilities, which need more range than e4m3 has: converter warps load a block's value codes (16
+// bytes a thread and piece, the next tile's loads in flight while one is converted, later tiles on their way into L2) and
+// write them as f16 (exact, two per instruction) into the 128-byte swizzled tiles that the descriptors name. So the codes
+// cross HBM and L2 as bytes. The blocks' scales never touch the elements: the key scale joins the softmax scale, the
+// value scale the probabilities.
 //
 // Work is shared by weight, not by tile lists: every (request, key/value head, row tile, value slice) has a weight close
 // to its visible keys whose prefix sums have a closed form, CTA c of P takes the c-th part of the total, and a part of an
@@ -15,8 +19,8 @@
 // host knowing a length. An item in one CTA's part is finished there; the others leave float32 partials (at most two per
 // CTA) that a second launch joins.
 //
-// Warps: 0-3 softmax and epilogue (one row a thread: its TMEM lane; they also bring the item's query rows into shared
-// memory as f16), 4 work fetch, 5 MMA issue, 6.. conversion.
+// Warps: 0-3 softmax and epilogue (one row a thread: its TMEM lane; they also split the item's query rows), 4 work fetch
+// and the keys' TMA loads, 5 MMA issue, 6.. conversion of values.
 #include "cache_attention.cuh"
 
 namespace kd {
@@ -27,27 +31,30 @@ using namespace ca;
 template <int HD, int DV>
 struct Cfg {
   static constexpr int BM = 128;
-  static constexpr int CHUNKS = HD / 64;      // 128-byte swizzle chunks along the head dim (Q, K)
-  static constexpr int V_CHUNKS = DV / 64;
-  static constexpr int SLICES = HD / DV;      // value slices, separate items
-  static constexpr int Q_CHUNK = BM * 128;
-  static constexpr int KV_CHUNK = BN * 128;
-  static constexpr int Q_BYTES = Q_CHUNK * CHUNKS;
-  static constexpr int K_BYTES = KV_CHUNK * CHUNKS;
-  static constexpr int V_BYTES = KV_CHUNK * V_CHUNKS;
-  static constexpr int STAGE_BYTES = K_BYTES + V_BYTES;
-  static constexpr int STAGES = HD <= 256 ? 2 : 1;
-  static constexpr int SMEM = Q_BYTES + STAGES * STAGE_BYTES + 1024;
+  static constexpr int ROW = HD < 128 ? HD : 128;  // bytes of a key or query row within a swizzle chunk
+  static constexpr int CHUNKS = HD / ROW;          // swizzle chunks along the head dim (Q, K)
+  static constexpr int V_CHUNKS = DV / 64;         // 64 f16 values each
+  static constexpr int SLICES = HD / DV;           // value slices, separate items
+  static constexpr int Q_CHUNK = BM * ROW, K_CHUNK = BN * ROW, V_CHUNK = BN * 128;
+  static constexpr int Q_BYTES = Q_CHUNK * CHUNKS;  // of hi, and of lo
+  static constexpr int K_BYTES = K_CHUNK * CHUNKS;
+  static constexpr int V_BYTES = V_CHUNK * V_CHUNKS;
+  static constexpr int KST = HD <= 256 ? 3 : 2, VST = HD <= 256 ? 3 : 1;  // ring stages
+  static constexpr int SMEM = 2 * Q_BYTES + KST * K_BYTES + VST * V_BYTES + 1024;
   static constexpr int O_COL = 0, S_COL = DV;
   static constexpr int TMEM_COLS = DV + 2 * BN <= 256 ? 256 : 512;
   static constexpr int NS = (TMEM_COLS - DV) / BN < 4 ? (TMEM_COLS - DV) / BN : 4;  // score buffers
-  static constexpr int CTAS_PER_SM = (2 * (SMEM + 1024) <= 227 * 1024 && 2 * TMEM_COLS <= 512) ? 2 : 1;
+  static constexpr int CTAS_PER_SM = (2 * (SMEM + 2048) <= 227 * 1024 && 2 * TMEM_COLS <= 512) ? 2 : 1;
   static constexpr int CONV_WARPS = HD <= 128 ? 2 : 4;
   static constexpr int CONV = 32 * CONV_WARPS;
   static constexpr int THREADS = 192 + CONV;
   static constexpr int PARTIAL = BM * (DV + 3);  // floats: O, then (m, M, l) per row
   static_assert(NS >= 2 && S_COL + NS * BN <= TMEM_COLS, "tensor memory budget");
   static_assert(SMEM + 1024 <= 227 * 1024, "shared memory budget");
+  // Registers per thread when two CTAs share the SM (256 threads at 128 each): the softmax warps take what the others
+  // leave (4 x 32 x (168 + 88) = 256 x 128).
+  static constexpr bool SPLIT_REGISTERS = CTAS_PER_SM == 2;
+  static_assert(!SPLIT_REGISTERS || THREADS == 256, "two warpgroups");
 };
 
 constexpr float THRESHOLD = 4.0f;   // log2 units a row's maximum may grow before its sums are rescaled
@@ -194,16 +201,51 @@ KD_DEVICE void prefetch_block(const uint8_t* p, int bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
+// Shared-memory descriptor of a K-major tile of 8-bit elements in rows of ROW bytes with ROW-byte swizzling.
+template <int ROW>
+KD_DEVICE uint64_t kmajor_desc(uint32_t addr) {
+  if constexpr (ROW == 128) {
+    return sw128_kmajor_desc(addr);
+  } else {
+    uint64_t d = 0;
+    d |= (uint64_t)((addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)1u << 16;
+    d |= (uint64_t)(512u >> 4) << 32;  // 8 rows x 64 B
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)4u << 61;           // 64-byte swizzle
+    return d;
+  }
+}
+// Offset of 16-byte piece c of row r in such a tile (chunks of `chunk` bytes).
+template <int ROW>
+KD_DEVICE int swizzled(int r, int c, int chunk) {
+  if constexpr (ROW == 128) {
+    return (c >> 3) * chunk + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+  } else {
+    return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+  }
+}
+
+template <int N>
+KD_DEVICE void set_registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+KD_DEVICE void set_registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 template <int HD, int DV>
 __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM)
-    row_tiles_kernel(Args a, const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ v_codes) {
+    row_tiles_kernel(const __grid_constant__ CUtensorMap map_k, Args a, const uint8_t* __restrict__ v_codes) {
   using C = Cfg<HD, DV>;
-  constexpr int ST = C::STAGES, NS = C::NS, SL = C::SLICES;
+  constexpr int KST = C::KST, VST = C::VST, NS = C::NS, SL = C::SLICES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_q = smem;
-  uint8_t* s_kv = smem + C::Q_BYTES;  // stage s: K at s * STAGE_BYTES, V right after
-  __shared__ uint64_t q_full, k_full[ST], v_full[ST], k_empty[ST], v_empty[ST], s_full[NS], p_full[NS], pv_done[NS];
+  uint8_t* s_k = smem + 2 * C::Q_BYTES;
+  uint8_t* s_v = s_k + KST * C::K_BYTES;
+  __shared__ uint64_t q_full, k_full[KST], v_full[VST], k_empty[KST], v_empty[VST], s_full[NS], p_full[NS], pv_done[NS];
   __shared__ uint64_t item_full[2], item_empty[2];
   __shared__ Work works[2];
   __shared__ uint32_t tmem_slot;
@@ -213,10 +255,12 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
   if (tid == 0) {
     mbar_init(&q_full, 128);
-    for (int s = 0; s < ST; ++s) {
-      mbar_init(&k_full[s], C::CONV_WARPS);
-      mbar_init(&v_full[s], C::CONV_WARPS);
+    for (int s = 0; s < KST; ++s) {
+      mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < VST; ++s) {
+      mbar_init(&v_full[s], C::CONV_WARPS);
       mbar_init(&v_empty[s], 1);
     }
     for (int b = 0; b < NS; ++b) {
@@ -285,52 +329,96 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
+  if (warp >= 4) {
+  if constexpr (C::SPLIT_REGISTERS) set_registers_down<88>();  // one instruction for the whole warpgroup
   if (warp == 4) {
-    // ------------------------------------------------------------ work fetch
-    if (elect_one()) {
-      const int64_t lo = s_lo, hi = s_hi;
-      Item it;
-      bool more = lo < hi;
-      if (more) find<SL>(a, s_req, s_start, lo, it);
-      uint32_t k = 0;
-      while (true) {
-        Work w;
-        w.i = -1;
-        while (more && it.begin < hi) {
-          const Tiles v = visible(a, it.s, it.tile);
-          const int64_t x0 = max(lo, it.begin), x1 = min(hi, it.end);
-          int t0, t1;
-          portion(it, x0, x1, v.n, t0, t1);
-          const bool whole = x0 == it.begin && x1 == it.end;
-          if (whole || t0 < t1) {
-            w.q0 = it.s.q0;
-            w.lq = it.s.lq;
-            w.lk = it.s.lk;
-            w.h = it.h;
-            w.slice = it.slice;
-            w.r0 = it.tile * 128;
-            w.rows = (int)min((int64_t)128, (int64_t)it.s.lq * a.group - w.r0);
-            w.first = v.first + t0;
-            w.n = t1 - t0;
-            w.i = it.i;
-            // an item begun by an earlier CTA leaves this one's first partial, one begun here its second
-            w.slot = whole ? -1 : 2 * (int)blockIdx.x + (it.begin < lo ? 0 : 1);
-            more = next<SL>(a, it);
-            break;
-          }
+    // ------------------------------------------------------------ work fetch, keys
+    const int64_t lo = s_lo, hi = s_hi;
+    Item it;
+    bool more = lo < hi;
+    if (more) find<SL>(a, s_req, s_start, lo, it);
+    if (lane == 0) tma_prefetch_desc(&map_k);
+    uint32_t g = 0;  // key tiles so far
+    bool ok = true;
+    int64_t issued[KST];  // the last use of each stage that a copy was issued for
+#pragma unroll
+    for (int s = 0; s < KST; ++s) issued[s] = -1;
+    for (uint32_t k = 0; ok; ++k) {
+      Work w;
+      w.i = -1;
+      w.n = 0;
+      while (more && it.begin < hi) {
+        const Tiles v = visible(a, it.s, it.tile);
+        const int64_t x0 = max(lo, it.begin), x1 = min(hi, it.end);
+        int t0, t1;
+        portion(it, x0, x1, v.n, t0, t1);
+        const bool whole = x0 == it.begin && x1 == it.end;
+        if (whole || t0 < t1) {
+          w.q0 = it.s.q0;
+          w.lq = it.s.lq;
+          w.lk = it.s.lk;
+          w.h = it.h;
+          w.slice = it.slice;
+          w.r0 = it.tile * 128;
+          w.rows = (int)min((int64_t)128, (int64_t)it.s.lq * a.group - w.r0);
+          w.first = v.first + t0;
+          w.n = t1 - t0;
+          w.i = it.i;
+          // an item begun by an earlier CTA leaves this one's first partial, one begun here its second
+          w.slot = whole ? -1 : 2 * (int)blockIdx.x + (it.begin < lo ? 0 : 1);
           more = next<SL>(a, it);
+          break;
         }
-        if (!mbar_wait(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, a.status)) goto done;
-        works[k & 1] = w;
-        mbar_arrive(&item_full[k & 1]);
-        ++k;
-        if (w.i < 0) break;
+        more = next<SL>(a, it);
       }
+      if (lane == 0) {
+        ok = mbar_wait(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, a.status);
+        if (ok) {
+          works[k & 1] = w;
+          mbar_arrive(&item_full[k & 1]);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok || w.i < 0) break;
+      int z_next = block_of(a, w, lane), z_now = -1;
+      for (int j = 0; j < w.n && ok; ++j) {
+        if ((j & 31) == 0) {
+          z_now = z_next;
+          z_next = block_of(a, w, j + 32 + lane);
+        }
+        const int z = __shfl_sync(0xffffffffu, z_now, j & 31);
+        const uint32_t G = g + j;
+        const int st = G % KST;
+        if (lane == 0) {
+          ok = mbar_wait(&k_empty[st], ((G / KST) & 1) ^ 1, a.status);
+          if (ok) {
+            // an absent block's keys are masked: whatever the stage holds will do
+            if (z >= 0) {
+              issued[st] = G / KST;
+              mbar_arrive_expect_tx(&k_full[st], C::K_BYTES);
+              for (int c = 0; c < C::CHUNKS; ++c)
+                tma_load_3d(&map_k, &k_full[st], s_k + st * C::K_BYTES + c * C::K_CHUNK, c * C::ROW, 0, z);
+            } else {
+              mbar_arrive(&k_full[st]);
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+      }
+      g += w.n;
+    }
+    if (!ok && lane == 0) {
+      // another role gave up: wait (bounded) for the copies in flight before the shared memory goes away
+      const uint64_t start = globaltimer();
+      for (int s = 0; s < KST; ++s)
+        while (issued[s] >= 0 && !mbar_try_wait(smem_u32(&k_full[s]), (uint32_t)issued[s] & 1) &&
+               globaltimer() - start < 1000000000ull) {
+        }
     }
   } else if (warp == 5) {
     // ------------------------------------------------------------ MMA issue
     if (elect_one()) {
-      constexpr uint32_t idesc_s = mma_idesc(0, C::BM, BN);     // f16, K-major A and B
+      constexpr uint32_t idesc_s = mma_idesc(0, C::BM, BN);     // e4m3, K-major A and B
       constexpr uint32_t idesc_o = mma_idesc(0, C::BM, DV, 1);  // f16, A from TMEM, MN-major B (V)
       const uint32_t sq = smem_u32(s_q);
       uint32_t g = 0, nq = 0;  // key tiles and items so far
@@ -345,18 +433,20 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         ++nq;
         auto issue_s = [&](int j) -> bool {
           const uint32_t G = g + j;
-          const int st = G % ST;
+          const int st = G % KST;
           if (G >= NS && !mbar_wait(&pv_done[G % NS], ((G - NS) / NS) & 1, a.status)) return false;
-          if (!mbar_wait(&k_full[st], (G / ST) & 1, a.status)) return false;
+          if (!mbar_wait(&k_full[st], (G / KST) & 1, a.status)) return false;
           tc_fence_after();
-          const uint32_t sk = smem_u32(s_kv + st * C::STAGE_BYTES);
+          const uint32_t sk = smem_u32(s_k + st * C::K_BYTES);
           const uint32_t d = tmem + C::S_COL + (G % NS) * BN;
 #pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const int c = kk / 4, w = (kk % 4) * 32;
-            mma_f16_ss(d, sw128_kmajor_desc(sq + c * C::Q_CHUNK + w), sw128_kmajor_desc(sk + c * C::KV_CHUNK + w),
-                       idesc_s, kk > 0);
-          }
+          for (int half = 0; half < 2; ++half)  // hi, then lo
+#pragma unroll
+            for (int kk = 0; kk < HD / 32; ++kk) {
+              const int c = kk * 32 / C::ROW, w = kk * 32 % C::ROW;
+              mma_f8_ss(d, kmajor_desc<C::ROW>(sq + half * C::Q_BYTES + c * C::Q_CHUNK + w),
+                        kmajor_desc<C::ROW>(sk + c * C::K_CHUNK + w), idesc_s, (half | kk) > 0);
+            }
           mma_commit(&k_empty[st]);
           mma_commit(&s_full[G % NS]);
           return true;
@@ -365,15 +455,15 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         for (int j = 0; j < n; ++j) {
           if (j + 1 < n && !issue_s(j + 1)) goto done;
           const uint32_t G = g + j;
-          const int st = G % ST;
+          const int st = G % VST;
           if (!mbar_wait(&p_full[G % NS], (G / NS) & 1, a.status)) goto done;
-          if (!mbar_wait(&v_full[st], (G / ST) & 1, a.status)) goto done;
+          if (!mbar_wait(&v_full[st], (G / VST) & 1, a.status)) goto done;
           tc_fence_after();
-          const uint32_t sv = smem_u32(s_kv + st * C::STAGE_BYTES + C::K_BYTES);
+          const uint32_t sv = smem_u32(s_v + st * C::V_BYTES);
           const uint32_t p = tmem + C::S_COL + (G % NS) * BN;
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk)
-            mma_f16_ts(tmem + C::O_COL, p + kk * 8, sw128_mnmajor_desc(sv + kk * 2048, C::KV_CHUNK), idesc_o,
+            mma_f16_ts(tmem + C::O_COL, p + kk * 8, sw128_mnmajor_desc(sv + kk * 2048, C::V_CHUNK), idesc_o,
                        (j | kk) != 0);
           mma_commit(&v_empty[st]);
           mma_commit(&pv_done[G % NS]);
@@ -381,15 +471,15 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         g += n;
       }
     }
-  } else if (warp >= 6) {
-    // ------------------------------------------------------------ conversion of K and V tiles
+  } else {
+    // ------------------------------------------------------------ conversion of value tiles
     // A warp's pass covers 8 rows x 64 columns: lanes 0-3 the four 16-code pieces of one row, lanes 4-7 of the next,
-    // whose f16 pieces fall on the other eight banks' groups (the swizzle is the row's parity there).
-    constexpr int KP = 8 * C::CHUNKS / C::CONV_WARPS, VP = 8 * C::V_CHUNKS / C::CONV_WARPS;  // passes a warp
-    constexpr int AHEAD = 6;  // tiles between L2 prefetch and use
+    // whose f16 pieces fall on the other banks (the swizzle flips with the row's parity).
+    constexpr int VP = 8 * C::V_CHUNKS / C::CONV_WARPS;  // passes a warp
+    constexpr int AHEAD = 6;                             // tiles between L2 prefetch and use
     const int cw = warp - 6;
     const int sub = lane >> 2, quarter = lane & 3;
-    uint4 kr[KP], vr[VP];
+    uint4 vr[VP];
     uint32_t g = 0;
     for (uint32_t k = 0;; ++k) {
       if (!mbar_wait(&item_full[k & 1], (k >> 1) & 1, a.status)) goto done;
@@ -404,14 +494,6 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         const int x = __shfl_sync(0xffffffffu, z_now, j & 31), y = __shfl_sync(0xffffffffu, z_next, j & 31);
         return j >= w.n ? -1 : (j >> 5) == batch ? x : y;
       };
-      auto load_k = [&](int z) {
-        const uint8_t* p = k_codes + (int64_t)max(z, 0) * (BN * HD);
-#pragma unroll
-        for (int s = 0; s < KP; ++s) {
-          const int pass = s * C::CONV_WARPS + cw, row = (pass & 7) * 8 + sub, c = pass >> 3;
-          kr[s] = z >= 0 ? load_codes(p + row * HD + c * 64 + quarter * 16) : make_uint4(0, 0, 0, 0);
-        }
-      };
       auto load_v = [&](int z, int keys) {  // keys: rows of the block that hold tokens; the rest may hold NaN codes
         const uint8_t* p = v_codes + (int64_t)max(z, 0) * (BN * HD) + w.slice * DV;
 #pragma unroll
@@ -420,59 +502,45 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
           vr[s] = z >= 0 && row < keys ? load_codes(p + row * HD + c * 64 + quarter * 16) : make_uint4(0, 0, 0, 0);
         }
       };
-      auto put = [&](const uint4& x, uint8_t* tile, int pass) {
-        const int row = (pass & 7) * 8 + sub, c = pass >> 3;
-        uint8_t* dst = tile + c * C::KV_CHUNK + row * 128;
-        uint4 lo, hi;
-        codes_to_f16(x.x, lo.x, lo.y);
-        codes_to_f16(x.y, lo.z, lo.w);
-        codes_to_f16(x.z, hi.x, hi.y);
-        codes_to_f16(x.w, hi.z, hi.w);
-        *reinterpret_cast<uint4*>(dst + (((2 * quarter) ^ (row & 7)) << 4)) = lo;
-        *reinterpret_cast<uint4*>(dst + (((2 * quarter + 1) ^ (row & 7)) << 4)) = hi;
-      };
       const int last_key = w.lk - w.first * BN;  // keys from the item's first tile to the request's last token
-      load_k(id(0));
-      for (int j = 0; j <= w.n; ++j) {  // keys one tile ahead of values
+      load_v(id(0), last_key);
+      for (int j = 0; j < w.n; ++j) {
         if (j >= 32 && (j & 31) == 0) {
           z_now = z_next;
           ++batch;
           z_next = block_of(a, w, j + 32 + lane);
         }
-        if (cw < 2) {
+        if (cw == 0) {
           const int z = id(j + AHEAD);
-          if (lane == 0 && z >= 0)
-            prefetch_block((cw ? v_codes : k_codes) + (int64_t)z * (BN * HD), BN * HD);
+          if (lane == 0 && z >= 0) prefetch_block(v_codes + (int64_t)z * (BN * HD), BN * HD);
         }
-        const int zj = id(j), zj1 = id(j + 1);
-        if (j < w.n) {
-          const uint32_t G = g + j;
-          const int st = G % ST;
-          if (!mbar_wait(&k_empty[st], ((G / ST) & 1) ^ 1, a.status)) goto done;
-          uint8_t* tile = s_kv + st * C::STAGE_BYTES;
+        const int z1 = id(j + 1);
+        const uint32_t G = g + j;
+        const int st = G % VST;
+        if (!mbar_wait(&v_empty[st], ((G / VST) & 1) ^ 1, a.status)) goto done;
+        uint8_t* tile = s_v + st * C::V_BYTES;
 #pragma unroll
-          for (int s = 0; s < KP; ++s) put(kr[s], tile, s * C::CONV_WARPS + cw);
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&k_full[st]);
-          load_k(zj1);
+        for (int s = 0; s < VP; ++s) {
+          const int pass = s * C::CONV_WARPS + cw, row = (pass & 7) * 8 + sub, c = pass >> 3;
+          uint8_t* dst = tile + c * C::V_CHUNK + row * 128;
+          uint4 lo, hi;
+          codes_to_f16(vr[s].x, lo.x, lo.y);
+          codes_to_f16(vr[s].y, lo.z, lo.w);
+          codes_to_f16(vr[s].z, hi.x, hi.y);
+          codes_to_f16(vr[s].w, hi.z, hi.w);
+          *reinterpret_cast<uint4*>(dst + (((2 * quarter) ^ (row & 7)) << 4)) = lo;
+          *reinterpret_cast<uint4*>(dst + (((2 * quarter + 1) ^ (row & 7)) << 4)) = hi;
         }
-        if (j >= 1) {
-          const uint32_t G = g + j - 1;
-          const int st = G % ST;
-          if (!mbar_wait(&v_empty[st], ((G / ST) & 1) ^ 1, a.status)) goto done;
-          uint8_t* tile = s_kv + st * C::STAGE_BYTES + C::K_BYTES;
-#pragma unroll
-          for (int s = 0; s < VP; ++s) put(vr[s], tile, s * C::CONV_WARPS + cw);
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&v_full[st]);
-        }
-        load_v(zj, last_key - j * BN);
+        load_v(z1, last_key - (j + 1) * BN);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[st]);
       }
       g += w.n;
     }
+  }
   } else {
+    if constexpr (C::SPLIT_REGISTERS) set_registers_up<168>();
     // ------------------------------------------------------------ queries, softmax, epilogue (warps 0-3)
     const int r = tid;  // the row within the tile = TMEM lane
     const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
@@ -488,38 +556,48 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
       const int gr = w.r0 + (live ? r : 0);
       const int tok = gr / a.group, head = w.h * a.group + gr - tok * a.group;
       float q_scale = 1.f;
+      bool bad = false;  // an infinity or a NaN among the row's queries: NaN wherever it sees a key
       if (n > 0) {
-        // The row's queries as f16, scaled by a power of two to its largest magnitude (exact but for what lies 2^-24
-        // below it). The last item's products have read theirs: its last scores were waited for.
+        // The row's queries as hi + lo. The last item's products have read theirs: its last scores were waited for.
         const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)(w.q0 + tok) * a.ldq + (int64_t)head * HD);
-        uint32_t big = 0;
+        uint32_t top = 0;  // the largest magnitude as a bf16 pattern
         if (live) {
 #pragma unroll 4
           for (int c = 0; c < HD / 8; ++c) {
             const uint4 x = src[c];
             const uint32_t v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t lo = v[e] & 0x7fffu, hi = (v[e] >> 16) & 0x7fffu;
-              big = max(big, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-            }
+            for (int e = 0; e < 4; ++e) top = max(top, max(v[e] & 0x7fffu, (v[e] >> 16) & 0x7fffu));
           }
         }
-        const int e = max((int)(big >> 7) - 127, -120);
+        bad = top >= 0x7f80u;
+        // the least e with the largest magnitude within 448 = 1.75 * 2^8
+        const int e = min(max((int)(top >> 7) - 127 - 8 + ((top & 0x7fu) > 0x60u ? 1 : 0), -120), 120);
         q_scale = pow2i(e);
         const float inv = pow2i(-e);
-#pragma unroll 4
-        for (int c = 0; c < HD / 8; ++c) {
-          const uint4 x = live ? src[c] : make_uint4(0, 0, 0, 0);
-          const uint32_t v[4] = {x.x, x.y, x.z, x.w};
-          uint32_t o[4];
+#pragma unroll 2
+        for (int c = 0; c < HD / 16; ++c) {
+          uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float2 f = unpack_bf16x2(v[y]);
-            o[y] = pack_f16x2(f.x * inv, f.y * inv);
+          for (int half = 0; half < 2; ++half) {
+            const uint4 x = live ? src[2 * c + half] : make_uint4(0, 0, 0, 0);
+            const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float2 f = unpack_bf16x2(v[2 * y]), h = unpack_bf16x2(v[2 * y + 1]);
+              const float4 q4 = make_float4(f.x * inv, f.y * inv, h.x * inv, h.y * inv);
+              const uint32_t w0 = e4m3_pair(q4.x, q4.y), w1 = e4m3_pair(q4.z, q4.w);
+              hi[2 * half + y] = w0 | (w1 << 16);
+              uint32_t h0, h1;
+              codes_to_f16(hi[2 * half + y], h0, h1);
+              const float2 b0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+              const float2 b1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+              lo[2 * half + y] = e4m3_pair(q4.x - b0.x, q4.y - b0.y) | (e4m3_pair(q4.z - b1.x, q4.w - b1.y) << 16);
+            }
           }
-          *reinterpret_cast<uint4*>(s_q + (c >> 3) * C::Q_CHUNK + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
-              make_uint4(o[0], o[1], o[2], o[3]);
+          const int at = swizzled<C::ROW>(r, c, C::Q_CHUNK);
+          *reinterpret_cast<uint4*>(s_q + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(s_q + C::Q_BYTES + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         fence_async_smem();
         mbar_arrive(&q_full);
@@ -633,6 +711,7 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         tc_fence_after();
       }
       if (warp_live) {
+        if (bad && l != 0.f) l = __int_as_float(0x7fffffff);
         const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
         const int64_t row = w.q0 + tok, col = (int64_t)head * HD + w.slice * DV;
         if (w.slot < 0) {
@@ -706,11 +785,12 @@ done:
 }
 
 // Joins the partials of an item that spans several CTAs' shares. blockIdx.x: the share whose beginning lies inside the
-// item, the first such one of the item; blockIdx.y: 8 of its 128 rows, a warp each. The partials lie in key order.
+// item, the first such one of the item; blockIdx.y: 32 of its 128 rows, a warp for each fourth. The lanes read the
+// partials' statistics together and weigh them; the sums then run in key order with their loads in flight.
 template <int HD, int DV>
 __global__ void __launch_bounds__(256) join_tiles_kernel(Args a, int ctas) {
   using C = Cfg<HD, DV>;
-  constexpr int V = DV / 32;
+  constexpr int V = DV / 32;  // columns a lane holds
   const int c = blockIdx.x + 1, lane = threadIdx.x & 31;
   const int64_t total = a.tile_cu[a.n];
   const int np = parts(total, a.group, ctas);
@@ -727,39 +807,94 @@ __global__ void __launch_bounds__(256) join_tiles_kernel(Args a, int ctas) {
   Item it;
   find<C::SLICES>(a, lo, a.tile_cu[lo], x, it);
   if (it.begin >= x || (c > 1 && total * (c - 1) / np > it.begin)) return;
-  const int r = blockIdx.y * 8 + threadIdx.x / 32;
-  const int gr = it.tile * 128 + r;
-  if (gr >= (int64_t)it.s.lq * a.group) return;
-  const int tok = gr / a.group, head = it.h * a.group + gr - tok * a.group;
+  const int rows = (int)min((int64_t)128, (int64_t)it.s.lq * a.group - it.tile * 128);
   const Tiles v = visible(a, it.s, it.tile);
-  float m = -INFINITY, big = -INFINITY, l = 0.f, o[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) o[e] = 0.f;
-  for (int p = c - 1; p < np; ++p) {
-    const int64_t x0 = total * p / np, x1 = total * (p + 1) / np;
-    if (x0 >= it.end) break;
-    int t0, t1;
-    portion(it, max(x0, it.begin), min(x1, it.end), v.n, t0, t1);
-    if (t0 >= t1) continue;
-    const float* part = a.partials + (int64_t)(2 * p + (it.begin < x0 ? 0 : 1)) * C::PARTIAL;
-    const float pm = part[C::BM * DV + 3 * r], pb = part[C::BM * DV + 3 * r + 1], pl = part[C::BM * DV + 3 * r + 2];
-    const float m_new = fmaxf(m, pm), big_new = fmaxf(big, pb);
-    const float base = m_new == -INFINITY ? 0.f : m_new, vbase = big_new == -INFINITY ? 0.f : big_new;
-    l = l * fast_exp2(m - base) + pl * fast_exp2(pm - base);
-    const float f0 = fast_exp2(big - vbase), f1 = fast_exp2(pb - vbase);
-#pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = o[e] * f0 + part[r * DV + lane * V + e] * f1;
-    m = m_new;
-    big = big_new;
+  int last = c;  // the last share that meets the item
+  {
+    // share p holds weight y when floor(p total / np) <= y: the one holding the item's last weight
+    last = (int)((it.end * np - 1) / total);
+    if (last >= np) last = np - 1;
   }
-  const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
-  const float fin = l == 0.f ? 0.f : fast_exp2(fminf(vbase - base, 126.f)) / (l * P_SCALE);
-  const int64_t row = it.s.q0 + tok, col = (int64_t)head * HD + it.slice * DV + lane * V;
+  const int first = c - 1, n = last - first + 1;
+  for (int r = blockIdx.y * 32 + threadIdx.x / 32; r < min(rows, (int)blockIdx.y * 32 + 32); r += 8) {
+    const int gr = it.tile * 128 + r;
+    const int tok = gr / a.group, head = it.h * a.group + gr - tok * a.group;
+    float m = -INFINITY, big = -INFINITY, l = 0.f, o[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    float y = l == 0.f ? 0.f : o[e] * fin;
-    if (a.gate && l != 0.f) y = x_sigmoid(y, __bfloat162float(a.gate[row * a.ldg + col + e]));
-    a.out[row * a.ldo + col + e] = __float2bfloat16_rn(y);
+    for (int e = 0; e < V; ++e) o[e] = 0.f;
+    for (int p0 = 0; p0 < n; p0 += 32) {
+      const int p = first + p0 + lane;
+      float pm = -INFINITY, pb = -INFINITY, pl = 0.f;
+      const float* part = a.partials;
+      if (p <= last) {
+        const int64_t x0 = total * p / np, x1 = total * (p + 1) / np;
+        int t0, t1;
+        portion(it, max(x0, it.begin), min(x1, it.end), v.n, t0, t1);
+        part += (int64_t)(2 * p + (it.begin < x0 ? 0 : 1)) * C::PARTIAL;
+        if (t0 < t1) {
+          pm = part[C::BM * DV + 3 * r];
+          pb = part[C::BM * DV + 3 * r + 1];
+          pl = part[C::BM * DV + 3 * r + 2];
+        }
+      }
+      float m_new = pm, big_new = pb;
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) {
+        m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, s));
+        big_new = fmaxf(big_new, __shfl_xor_sync(0xffffffffu, big_new, s));
+      }
+      m_new = fmaxf(m_new, m);
+      big_new = fmaxf(big_new, big);
+      const float base = m_new == -INFINITY ? 0.f : m_new, vbase = big_new == -INFINITY ? 0.f : big_new;
+      float sum = pl * fast_exp2(pm - base);
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+      l = l * fast_exp2(m - base) + sum;
+      const float f0 = fast_exp2(big - vbase), f1 = pb == -INFINITY && pl == 0.f ? -1.f : fast_exp2(pb - vbase);
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] *= f0;
+      m = m_new;
+      big = big_new;
+      const int count = min(32, n - p0);
+      const uint64_t mine = reinterpret_cast<uint64_t>(part + r * DV);
+#pragma unroll 4
+      for (int q = 0; q < count; ++q) {
+        const float f = __shfl_sync(0xffffffffu, f1, q);
+        const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, mine, q)) + lane * V;
+        if (f < 0.f) continue;  // no key of the row (the partial may hold nothing)
+        if constexpr (V >= 4) {
+#pragma unroll
+          for (int e = 0; e < V; e += 4) {
+            const float4 y = *reinterpret_cast<const float4*>(src + e);
+            o[e] += y.x * f;
+            o[e + 1] += y.y * f;
+            o[e + 2] += y.z * f;
+            o[e + 3] += y.w * f;
+          }
+        } else {
+          const float2 y = *reinterpret_cast<const float2*>(src);
+          o[0] += y.x * f;
+          o[1] += y.y * f;
+        }
+      }
+    }
+    const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
+    const float fin = l == 0.f ? 0.f : fast_exp2(fminf(vbase - base, 126.f)) / (l * P_SCALE);
+    const int64_t row = it.s.q0 + tok, col = (int64_t)head * HD + it.slice * DV + lane * V;
+    float y[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) y[e] = l == 0.f ? 0.f : o[e] * fin;
+    if (a.gate && l != 0.f) {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const float2 s = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(a.gate + row * a.ldg + col + e));
+        y[e] = x_sigmoid(y[e], s.x);
+        y[e + 1] = x_sigmoid(y[e + 1], s.y);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < V; e += 2)
+      *reinterpret_cast<uint32_t*>(a.out + row * a.ldo + col + e) = pack_bf16x2(y[e], y[e + 1]);
   }
 }
 
@@ -772,7 +907,7 @@ int64_t workspace(int n, int sms) {
 }
 
 template <int HD, int DV>
-int launch(Args a, const uint8_t* k_codes, const uint8_t* v_codes, uint8_t* ws, int64_t ws_bytes, cudaStream_t stream) {
+int launch(Args a, const void* k_codes, const uint8_t* v_codes, uint8_t* ws, int64_t ws_bytes, cudaStream_t stream) {
   using C = Cfg<HD, DV>;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -789,9 +924,14 @@ int launch(Args a, const uint8_t* k_codes, const uint8_t* v_codes, uint8_t* ws, 
     if (e != cudaSuccess) return record_cuda_error(e, "attention_cache: cudaFuncSetAttribute");
     configured[dev] = true;
   }
-  kernel<<<ctas, C::THREADS, C::SMEM, stream>>>(a, k_codes, v_codes);
+  CUtensorMap mk;
+  const auto sw = C::ROW == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  if (int rc = make_tma_3d(&mk, k_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, HD, BN, (uint64_t)a.blocks * a.hkv, HD,
+                           (uint64_t)BN * HD, C::ROW, BN, 1, sw))
+    return rc;
+  kernel<<<ctas, C::THREADS, C::SMEM, stream>>>(mk, a, v_codes);
   if (int rc = record_cuda_error(cudaGetLastError(), "attention_cache: launch")) return rc;
-  join_tiles_kernel<HD, DV><<<dim3(ctas - 1 > 0 ? ctas - 1 : 1, 16), 256, 0, stream>>>(a, ctas);
+  join_tiles_kernel<HD, DV><<<dim3(ctas - 1 > 0 ? ctas - 1 : 1, 4), 256, 0, stream>>>(a, ctas);
   return record_cuda_error(cudaGetLastError(), "attention_cache: join launch");
 }
 
@@ -810,13 +950,12 @@ int64_t row_tiles_workspace(int head_dim, int n, int sms) {
 
 int row_tiles(int head_dim, const Args& a, const void* k_codes, const void* v_codes, uint8_t* ws, int64_t ws_bytes,
               cudaStream_t stream) {
-  const uint8_t* k = static_cast<const uint8_t*>(k_codes);
   const uint8_t* v = static_cast<const uint8_t*>(v_codes);
   switch (head_dim) {
-    case 64: return ct::launch<64, 64>(a, k, v, ws, ws_bytes, stream);
-    case 128: return ct::launch<128, 128>(a, k, v, ws, ws_bytes, stream);
-    case 256: return ct::launch<256, 256>(a, k, v, ws, ws_bytes, stream);
-    default: return ct::launch<512, 256>(a, k, v, ws, ws_bytes, stream);
+    case 64: return ct::launch<64, 64>(a, k_codes, v, ws, ws_bytes, stream);
+    case 128: return ct::launch<128, 128>(a, k_codes, v, ws, ws_bytes, stream);
+    case 256: return ct::launch<256, 256>(a, k_codes, v, ws, ws_bytes, stream);
+    default: return ct::launch<512, 256>(a, k_codes, v, ws, ws_bytes, stream);
   }
 }
 
