@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
         float factor[2], alpha_o[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float mul = score_factor(q_scale[u], ti.k_scale, a.scale_log2);
+          const float mul = score_factor(q_scale[u] * a.scale_log2, ti.k_scale);
           float mx = -INFINITY;
 #pragma unroll
           for (int j = 0; j < 8; ++j)
@@ -710,7 +710,7 @@ extern "C" int kd_attention_cache_workspace(int num_requests, int max_q, int64_t
   if (int rc = record_cuda_error(cudaGetDevice(&dev), "attention_cache_workspace: device")) return rc;
   const int sms = num_sms(dev), group = num_heads_q / num_heads_kv;
   if (!ca::few_rows(max_q, group)) {
-    *bytes = ca::row_tiles_workspace(head_dim, num_requests, sms);
+    *bytes = ca::row_tiles_workspace(head_dim, sms);
     return KD_OK;
   }
   switch (head_dim) {

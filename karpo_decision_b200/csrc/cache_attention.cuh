@@ -33,6 +33,7 @@ struct Args {
   int left, right;
   int64_t* tile_cu;   // [n + 1] few rows: key tiles of the requests before (of one key/value head); many: their weights
   int32_t* item_cu;   // [n + 1] few rows: 16-row tiles of the requests before
+  void* splits;       // many rows: an item begun by a CTA and finished by later ones, per CTA
   float* partials;
   int* status;
 };
@@ -85,10 +86,10 @@ KD_DEVICE uint32_t e4m3_pair(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
-// scale * log2(e) times the power-of-two scales of a query row and a block's keys: finite and not 0, so that it times a
-// masked -inf or a score of 0 is no NaN.
-KD_DEVICE float score_factor(float q_scale, float k_scale, float scale_log2) {
-  return fminf(fmaxf(q_scale * k_scale * scale_log2, 1.1754944e-38f), 3.4028235e38f);
+// The softmax scale * log2(e) * a query row's power of two (`row`), times a block's key scale: finite and not 0, so that
+// it times a masked -inf or a score of 0 is no NaN.
+KD_DEVICE float score_factor(float row, float k_scale) {
+  return fminf(fmaxf(row * k_scale, 1.1754944e-38f), 3.4028235e38f);
 }
 
 KD_DEVICE uint32_t pack_f16x2(float lo, float hi) {
@@ -96,8 +97,24 @@ KD_DEVICE uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// Launches the joining kernel so that its blocks are in place when the kernel before it in the stream ends (it waits for
+// that itself, by griddepcontrol.wait).
+template <typename K>
+int launch_after(K kernel, dim3 grid, int threads, cudaStream_t stream, const Args& a, int ctas) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return record_cuda_error(cudaLaunchKernelEx(&cfg, kernel, a, ctas), "attention_cache: join launch");
+}
+
 // The kernel for many rows per key/value head (cache_attention_tiles.cu).
-int64_t row_tiles_workspace(int head_dim, int n, int sms);
+int64_t row_tiles_workspace(int head_dim, int sms);
 int row_tiles(int head_dim, const Args& a, const void* k_codes, const void* v_codes, uint8_t* ws, int64_t ws_bytes,
               cudaStream_t stream);
 

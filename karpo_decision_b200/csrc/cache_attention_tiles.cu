@@ -19,8 +19,10 @@
 // host knowing a length. An item in one CTA's part is finished there; the others leave float32 partials (at most two per
 // CTA) that a second launch joins.
 //
-// Warps: 0-3 softmax and epilogue (one row a thread: its TMEM lane; they also split the item's query rows), 4 work fetch
-// and the keys' TMA loads, 5 MMA issue, 6.. conversion of values.
+// Warps: 0-3 softmax and epilogue, a thread a row (they also split the item's query rows), 4 work fetch and the keys' TMA
+// loads, 5 MMA issue, 6.. conversion of values.
+#include <type_traits>
+
 #include "cache_attention.cuh"
 
 namespace kd {
@@ -39,36 +41,51 @@ struct Cfg {
   static constexpr int Q_BYTES = Q_CHUNK * CHUNKS;  // of hi, and of lo
   static constexpr int K_BYTES = K_CHUNK * CHUNKS;
   static constexpr int V_BYTES = V_CHUNK * V_CHUNKS;
-  static constexpr int KST = HD <= 256 ? 3 : 2, VST = HD <= 256 ? 3 : 1;  // ring stages
-  static constexpr int SMEM = 2 * Q_BYTES + KST * K_BYTES + VST * V_BYTES + 1024;
-  static constexpr int O_COL = 0, S_COL = DV;
-  static constexpr int TMEM_COLS = DV + 2 * BN <= 256 ? 256 : 512;
-  static constexpr int NS = (TMEM_COLS - DV) / BN < 4 ? (TMEM_COLS - DV) / BN : 4;  // score buffers
-  static constexpr int CTAS_PER_SM = (2 * (SMEM + 2048) <= 227 * 1024 && 2 * TMEM_COLS <= 512) ? 2 : 1;
+  // Tensor-memory columns: O, NS score buffers (P overwrites its scores) and, for heads of 256, the queries (4 elements a
+  // column): an A operand from shared memory costs 4 KB per 32 of head dim beside 2 KB of keys, more than the tensor core
+  // waits for. Heads of 512 leave no room for them.
+  static constexpr bool Q_TMEM = HD == 256;
+  static constexpr int NS = HD == 64 ? 3 : HD == 512 ? 4 : 2;
+  static constexpr int O_COL = 0, S_COL = DV, HI_COL = S_COL + NS * BN, LO_COL = HI_COL + HD / 4;
+  static constexpr int USED_COLS = HI_COL + (Q_TMEM ? HD / 2 : 0), TMEM_COLS = USED_COLS <= 256 ? 256 : 512;
+  static constexpr int QS_BYTES = Q_TMEM ? 0 : 2 * Q_BYTES;  // queries in shared memory
+  static constexpr int KST = HD <= 128 ? 3 : HD == 256 ? 4 : 2, VST = HD <= 128 ? 3 : HD == 256 ? 4 : 1;  // ring stages
+  static constexpr int TILES = QS_BYTES + KST * K_BYTES + VST * V_BYTES + (Q_TMEM ? BM * ROW : 0);  // of 1,024 bytes
+  static constexpr int SMEM = TILES + 3072;
+  static constexpr int CTAS_PER_SM = (2 * (SMEM + 1024) <= 227 * 1024 && 2 * TMEM_COLS <= 512) ? 2 : 1;
+  static constexpr int SOFT = 4;  // softmax warps, a thread a row
   static constexpr int CONV_WARPS = HD <= 128 ? 2 : 4;
   static constexpr int CONV = 32 * CONV_WARPS;
-  static constexpr int THREADS = 192 + CONV;
+  static constexpr int THREADS = 32 * (SOFT + 2) + CONV;
   static constexpr int PARTIAL = BM * (DV + 3);  // floats: O, then (m, M, l) per row
-  static_assert(NS >= 2 && S_COL + NS * BN <= TMEM_COLS, "tensor memory budget");
-  static_assert(SMEM + 1024 <= 227 * 1024, "shared memory budget");
+  static_assert(KST + NS <= 8, "the ring of tile infos");
+  static_assert(USED_COLS <= 512, "tensor memory budget");
+  static_assert(SMEM <= 227 * 1024, "shared memory budget");
   // Registers per thread when two CTAs share the SM (256 threads at 128 each): the softmax warps take what the others
-  // leave (4 x 32 x (168 + 88) = 256 x 128).
+  // leave (128 x (168 + 88) = 256 x 128).
   static constexpr bool SPLIT_REGISTERS = CTAS_PER_SM == 2;
   static_assert(!SPLIT_REGISTERS || THREADS == 256, "two warpgroups");
 };
 
 constexpr float THRESHOLD = 4.0f;   // log2 units a row's maximum may grow before its sums are rescaled
-constexpr float P_SCALE = 2048.f;   // f16 probabilities hold p * 2^11: at most 2^15 with the threshold
+constexpr float P_EXPONENT = 11.f, P_SCALE = 2048.f;  // f16 probabilities hold p * 2^11: at most 2^15 with the threshold
 constexpr int ITEM_TILES = 4;       // an item's own cost (queries, epilogue) in key tiles
 constexpr int MIN_TILES = 6;        // the least share of a CTA in key tiles: less costs more to join than it saves
 
-// A request's row tiles and their weights w(j) = min(base + step j, cap) + own (units: keys x group): the keys tile j
-// sees, up to the window's width.
+// Quotients of non-negative numbers: in 32 bits where both fit (a 64-bit division costs some 600 cycles here, and the
+// first key tile waits for several).
+KD_DEVICE int64_t quotient(int64_t a, int64_t b) {
+  return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
+// A request's row tiles and their weights w(j) = min(base + step j, cap) + own, in units of a key tile / group: the key
+// tiles that row tile j sees, about, up to the window's width.
 struct Shape {
   int q0, lq, lk, tiles;
-  int64_t base, step, cap, own;
+  int64_t base, cap, own;
+  int step;  // 0 or 2: 128 rows reach 128 / group keys further
   KD_DEVICE int64_t before(int64_t j) const {  // weight of the tiles before j
-    const int64_t grow = base >= cap ? 0 : step == 0 ? j : min(j, (cap - base + step - 1) / step);
+    const int64_t grow = base >= cap ? 0 : step == 0 ? j : min(j, (cap - base + 1) >> 1);
     return grow * base + step * (grow * (grow - 1) / 2) + (j - grow) * cap + j * own;
   }
 };
@@ -81,17 +98,17 @@ KD_DEVICE Shape shape(const Args& a, int i) {
   s.lk = r.lk;
   s.tiles = (int)(((int64_t)r.lq * a.group + 127) / 128);
   const int64_t g = a.group;
-  s.cap = g * r.lk;
-  s.base = a.right < 0 ? s.cap : min(s.cap, g * max(r.lk - r.lq + (int64_t)a.right, (int64_t)0) + 128);
-  s.step = a.right < 0 ? 0 : 128;
-  if (a.left >= 0) s.cap = min(s.cap, g * ((int64_t)a.left + 1 + max(a.right, 0)) + 128);
-  s.own = g * BN * ITEM_TILES;
+  s.cap = g * r.lk / BN;
+  s.base = a.right < 0 ? s.cap : min(s.cap, (g * max(r.lk - r.lq + (int64_t)a.right, (int64_t)0) + 128) / BN);
+  s.step = a.right < 0 ? 0 : 2;
+  if (a.left >= 0) s.cap = min(s.cap, (g * ((int64_t)a.left + 1 + max(a.right, 0)) + 128) / BN);
+  s.own = g * ITEM_TILES;
   return s;
 }
 
 // The CTAs that take part of a total weight.
 KD_DEVICE int parts(int64_t total, int64_t group, int ctas) {
-  return (int)min((int64_t)ctas, max((int64_t)1, total / (group * BN * MIN_TILES)));
+  return (int)min((int64_t)ctas, max((int64_t)1, quotient(total, group * MIN_TILES)));
 }
 
 // An item's place in the list request > key/value head > row tile > value slice, and its weight interval.
@@ -107,7 +124,7 @@ KD_DEVICE void find(const Args& a, int i, int64_t start, int64_t x, Item& it) {
   it.i = i;
   it.s = shape(a, i);
   const int64_t head = it.s.before(it.s.tiles) * SLICES;
-  it.h = (int)((x - start) / head);
+  it.h = (int)quotient(x - start, head);
   const int64_t y = x - start - it.h * head;
   int lo = 0, hi = it.s.tiles - 1;
   while (lo < hi) {
@@ -119,7 +136,7 @@ KD_DEVICE void find(const Args& a, int i, int64_t start, int64_t x, Item& it) {
   }
   it.tile = lo;
   const int64_t b = it.s.before(lo), w = it.s.before(lo + 1) - b;
-  it.slice = (int)((y - b * SLICES) / w);
+  it.slice = SLICES == 1 ? 0 : (int)quotient(y - b * SLICES, w);
   it.begin = start + it.h * head + b * SLICES + it.slice * w;
   it.end = it.begin + w;
 }
@@ -161,11 +178,11 @@ KD_DEVICE Tiles visible(const Args& a, const Shape& s, int tile) {
   return t;
 }
 
-// The key tiles [t0, t1) of an item with n tiles that the weights [x0, x1) take.
-KD_DEVICE void portion(const Item& it, int64_t x0, int64_t x1, int n, int& t0, int& t1) {
-  const int64_t w = it.end - it.begin;
-  t0 = x0 <= it.begin ? 0 : (int)((x0 - it.begin) * n / w);
-  t1 = x1 >= it.end ? n : (int)((x1 - it.begin) * n / w);
+// The key tiles [t0, t1) of an item of weights [begin, end) with n tiles that the weights [x0, x1) take.
+KD_DEVICE void portion(int64_t begin, int64_t end, int64_t x0, int64_t x1, int n, int& t0, int& t1) {
+  const int64_t w = end - begin;
+  t0 = x0 <= begin ? 0 : (int)quotient((x0 - begin) * n, w);
+  t1 = x1 >= end ? n : (int)quotient((x1 - begin) * n, w);
 }
 
 // What the roles of a CTA need of its next part of an item.
@@ -178,12 +195,13 @@ struct Work {
   int pad;
 };
 
-// One tile's block and scales, looked up 32 tiles at a time by a warp's lanes.
-struct Lookup {
-  int z;  // block * heads + head, < 0: absent
-  float k_scale;
-  int v_exp;
+// An item that begins in a CTA's share and ends in a later one, for the joining launch. rows 0: none.
+struct Split {
+  int64_t begin, end, total;  // its weights, and the launch's
+  int q0, h, slice, r0, rows, tiles, last, np;  // `last`: the CTA that finishes it
 };
+
+// block * heads + head of an item's tile j, < 0: absent. Roles look up 32 tiles at a time, one a lane.
 KD_DEVICE int block_of(const Args& a, const Work& w, int j) {
   if (j >= w.n) return -1;
   const int id = a.table[(int64_t)w.i * a.ldt + w.first + j];
@@ -226,6 +244,20 @@ KD_DEVICE int swizzled(int r, int c, int chunk) {
   }
 }
 
+// D[tmem] (+)= A[tmem] * B[smem]^T, 8-bit float operands.
+KD_DEVICE void mma_f8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate));
+}
+KD_DEVICE void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+
 template <int N>
 KD_DEVICE void set_registers_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -235,26 +267,55 @@ KD_DEVICE void set_registers_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// What the softmax needs of a key tile.
+struct Info {
+  float k_scale, v_exp;
+  int live;  // 0: the block is absent
+  int pad;
+};
+
+// What a CTA's warps share beside the tiles.
+template <int HD, int DV>
+struct Shared {
+  using C = Cfg<HD, DV>;
+  uint64_t q_full, k_full[C::KST], v_full[C::VST], k_empty[C::KST], v_empty[C::VST];
+  uint64_t s_full[C::NS], p_full[C::NS], pv_done[C::NS], item_full[2], item_empty[2];
+  int64_t warp[C::THREADS / 32], start;
+  Work works[2];
+  Info info[8];           // by key tile: at most KST + NS tiles are between their load and their softmax
+  int req;
+  uint32_t tmem_slot;
+};
+
 template <int HD, int DV>
 __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM)
     row_tiles_kernel(const __grid_constant__ CUtensorMap map_k, Args a, const uint8_t* __restrict__ v_codes) {
   using C = Cfg<HD, DV>;
-  constexpr int KST = C::KST, VST = C::VST, NS = C::NS, SL = C::SLICES;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr int KST = C::KST, VST = C::VST, NS = C::NS, SL = C::SLICES, SOFT = C::SOFT;
+  // Tiles first: nothing is declared static, so the dynamic area keeps its 1,024-byte alignment without slack.
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(a.status, KD_OK, KD_DEVICE_TIMEOUT);
+    return;
+  }
   uint8_t* s_q = smem;
-  uint8_t* s_k = smem + 2 * C::Q_BYTES;
+  uint8_t* s_k = smem + C::QS_BYTES;
   uint8_t* s_v = s_k + KST * C::K_BYTES;
-  __shared__ uint64_t q_full, k_full[KST], v_full[VST], k_empty[KST], v_empty[VST], s_full[NS], p_full[NS], pv_done[NS];
-  __shared__ uint64_t item_full[2], item_empty[2];
-  __shared__ Work works[2];
-  __shared__ uint32_t tmem_slot;
-  __shared__ int64_t s_warp[C::THREADS / 32], s_lo, s_hi, s_start;
-  __shared__ int s_req;
+  uint8_t* s_stage = C::Q_TMEM ? s_v + VST * C::V_BYTES : s_q;  // the epilogue's, 128 rows of ROW bytes
+  Shared<HD, DV>& sh = *reinterpret_cast<Shared<HD, DV>*>(smem + C::TILES);
+  uint64_t &q_full = sh.q_full, *k_full = sh.k_full, *v_full = sh.v_full, *k_empty = sh.k_empty, *v_empty = sh.v_empty;
+  uint64_t *s_full = sh.s_full, *p_full = sh.p_full, *pv_done = sh.pv_done;
+  uint64_t *item_full = sh.item_full, *item_empty = sh.item_empty;
+  Work* works = sh.works;
+  Info* infos = sh.info;
+  int64_t* s_warp = sh.warp;
+  int64_t& s_start = sh.start;
+  int& s_req = sh.req;
+  uint32_t& tmem_slot = sh.tmem_slot;
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
   if (tid == 0) {
-    mbar_init(&q_full, 128);
+    mbar_init(&q_full, SOFT);
     for (int s = 0; s < KST; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
@@ -270,58 +331,52 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&item_full[b], 1);
-      mbar_init(&item_empty[b], 5 + C::CONV_WARPS);
+      mbar_init(&item_empty[b], SOFT + 1 + C::CONV_WARPS);
     }
     fence_barrier_init();
   }
-  if (warp == 5) {
+  if (warp == SOFT + 1) {
     tmem_alloc(&tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
   }
-  // ---- this CTA's share: a scan of the requests' weights, first for the total, then for the share's first request
-  int64_t total = 0;
-  int np = 1;
-  for (int pass = 0; pass < 2; ++pass) {
-    np = parts(total, a.group, gridDim.x);
-    const int64_t lo = pass ? total * blockIdx.x / np : 0;
-    int64_t carry = 0;
-    for (int i0 = 0; i0 < a.n; i0 += C::THREADS) {
-      const int i = i0 + tid;
-      int64_t w = 0;
-      if (i < a.n) {
-        const Shape s = shape(a, i);
-        w = s.before(s.tiles) * SL * a.hkv;
-      }
-      int64_t x = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t px = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += px;
-      }
-      if (lane == 31) s_warp[warp] = x;
-      __syncthreads();
-      int64_t before = carry, chunk = 0;
-#pragma unroll
-      for (int v = 0; v < C::THREADS / 32; ++v) {
-        if (v < warp) before += s_warp[v];
-        chunk += s_warp[v];
-      }
-      before += x - w;
-      if (pass && i < a.n) {
-        if (blockIdx.x == 0) a.tile_cu[i] = before;  // for the launch that joins the partials
-        if (w > 0 && lo >= before && lo < before + w) {
-          s_req = i;
-          s_start = before;
-        }
-      }
-      carry += chunk;
-      __syncthreads();
+  // ---- this CTA's share: a scan of the requests' weights for the total, then (a second scan if the requests outnumber
+  // the threads) for the share's first request
+  int64_t w_mine = 0, w_before = 0;
+  auto scan = [&](int i0, int64_t carry) -> int64_t {  // the sum past this chunk; the thread's own weight and prefix
+    const int i = i0 + tid;
+    w_mine = 0;
+    if (i < a.n) {
+      const Shape s = shape(a, i);
+      w_mine = s.before(s.tiles) * SL * a.hkv;
     }
-    total = carry;
-    if (pass && tid == 0) {
-      s_lo = lo;
-      s_hi = (int)blockIdx.x < np ? total * (blockIdx.x + 1) / np : 0;
-      if (blockIdx.x == 0) a.tile_cu[a.n] = total;
+    int64_t x = w_mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t px = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += px;
+    }
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    w_before = carry + x - w_mine;
+#pragma unroll
+    for (int v = 0; v < C::THREADS / 32; ++v) {
+      if (v < warp) w_before += s_warp[v];
+      carry += s_warp[v];
+    }
+    __syncthreads();
+    return carry;
+  };
+  int64_t total = 0;
+  for (int i0 = 0; i0 < a.n; i0 += C::THREADS) total = scan(i0, total);
+  const int np = parts(total, a.group, gridDim.x);
+  const int64_t share_lo = quotient(total * blockIdx.x, np);
+  const int64_t share_hi = (int)blockIdx.x < np ? quotient(total * (blockIdx.x + 1), np) : 0;
+  int64_t again = 0;
+  for (int i0 = 0; i0 < a.n; i0 += C::THREADS) {
+    if (a.n > C::THREADS) again = scan(i0, again);
+    if (w_mine > 0 && share_lo >= w_before && share_lo < w_before + w_mine) {
+      s_req = i0 + tid;
+      s_start = w_before;
     }
   }
   tc_fence_before();
@@ -329,15 +384,16 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp >= 4) {
+  if (warp >= SOFT) {
   if constexpr (C::SPLIT_REGISTERS) set_registers_down<88>();  // one instruction for the whole warpgroup
-  if (warp == 4) {
+  if (warp == SOFT) {
     // ------------------------------------------------------------ work fetch, keys
-    const int64_t lo = s_lo, hi = s_hi;
+    const int64_t lo = share_lo, hi = share_hi;
     Item it;
     bool more = lo < hi;
     if (more) find<SL>(a, s_req, s_start, lo, it);
     if (lane == 0) tma_prefetch_desc(&map_k);
+    Split begun = {};
     uint32_t g = 0;  // key tiles so far
     bool ok = true;
     int64_t issued[KST];  // the last use of each stage that a copy was issued for
@@ -351,8 +407,12 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         const Tiles v = visible(a, it.s, it.tile);
         const int64_t x0 = max(lo, it.begin), x1 = min(hi, it.end);
         int t0, t1;
-        portion(it, x0, x1, v.n, t0, t1);
+        portion(it.begin, it.end, x0, x1, v.n, t0, t1);
         const bool whole = x0 == it.begin && x1 == it.end;
+        if (it.end > hi) {
+          begun = Split{it.begin, it.end, total, it.s.q0, it.h, it.slice, it.tile * 128,
+                        (int)min((int64_t)128, (int64_t)it.s.lq * a.group - it.tile * 128), v.n, 0, np};
+        }
         if (whole || t0 < t1) {
           w.q0 = it.s.q0;
           w.lq = it.s.lq;
@@ -380,18 +440,24 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok || w.i < 0) break;
-      int z_next = block_of(a, w, lane), z_now = -1;
+      int z_next = block_of(a, w, lane), z_now = -1, ve_now = 0;
+      float ks_now = 0.f;
       for (int j = 0; j < w.n && ok; ++j) {
         if ((j & 31) == 0) {
           z_now = z_next;
+          ks_now = z_now >= 0 ? a.k_scale[z_now] : 0.f;
+          ve_now = z_now >= 0 ? exponent_of(a.v_scale[z_now]) : 0;
           z_next = block_of(a, w, j + 32 + lane);
         }
         const int z = __shfl_sync(0xffffffffu, z_now, j & 31);
+        const float ks = __shfl_sync(0xffffffffu, ks_now, j & 31);
+        const int ve = __shfl_sync(0xffffffffu, ve_now, j & 31);
         const uint32_t G = g + j;
         const int st = G % KST;
         if (lane == 0) {
           ok = mbar_wait(&k_empty[st], ((G / KST) & 1) ^ 1, a.status);
           if (ok) {
+            infos[G & 7] = Info{ks, (float)ve, z >= 0, 0};
             // an absent block's keys are masked: whatever the stage holds will do
             if (z >= 0) {
               issued[st] = G / KST;
@@ -407,6 +473,18 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
       }
       g += w.n;
     }
+    if (lane == 0) {
+      // the item this CTA begins and the next ones finish, for the launch that joins them; share p holds weight y when
+      // floor(p total / np) <= y
+      Split* d = reinterpret_cast<Split*>(a.splits) + blockIdx.x;
+      const bool split = lo < hi && begun.begin >= lo && begun.end > hi;
+      if (split) {
+        begun.last = (int)min((int64_t)np - 1, quotient(begun.end * np - 1, total));
+        *d = begun;
+      } else {
+        d->rows = 0;
+      }
+    }
     if (!ok && lane == 0) {
       // another role gave up: wait (bounded) for the copies in flight before the shared memory goes away
       const uint64_t start = globaltimer();
@@ -415,7 +493,7 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
                globaltimer() - start < 1000000000ull) {
         }
     }
-  } else if (warp == 5) {
+  } else if (warp == SOFT + 1) {
     // ------------------------------------------------------------ MMA issue
     if (elect_one()) {
       constexpr uint32_t idesc_s = mma_idesc(0, C::BM, BN);     // e4m3, K-major A and B
@@ -444,8 +522,12 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
 #pragma unroll
             for (int kk = 0; kk < HD / 32; ++kk) {
               const int c = kk * 32 / C::ROW, w = kk * 32 % C::ROW;
-              mma_f8_ss(d, kmajor_desc<C::ROW>(sq + half * C::Q_BYTES + c * C::Q_CHUNK + w),
-                        kmajor_desc<C::ROW>(sk + c * C::K_CHUNK + w), idesc_s, (half | kk) > 0);
+              const uint64_t key = kmajor_desc<C::ROW>(sk + c * C::K_CHUNK + w);
+              if constexpr (C::Q_TMEM)
+                mma_f8_ts(d, tmem + (half ? C::LO_COL : C::HI_COL) + kk * 8, key, idesc_s, (half | kk) > 0);
+              else
+                mma_f8_ss(d, kmajor_desc<C::ROW>(sq + half * C::Q_BYTES + c * C::Q_CHUNK + w), key, idesc_s,
+                          (half | kk) > 0);
             }
           mma_commit(&k_empty[st]);
           mma_commit(&s_full[G % NS]);
@@ -453,7 +535,7 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         };
         if (!issue_s(0)) goto done;
         for (int j = 0; j < n; ++j) {
-          if (j + 1 < n && !issue_s(j + 1)) goto done;
+          if (j + 1 < n && !issue_s(j + 1)) goto done;  // the next scores first: their softmax starts while P V runs
           const uint32_t G = g + j;
           const int st = G % VST;
           if (!mbar_wait(&p_full[G % NS], (G / NS) & 1, a.status)) goto done;
@@ -474,11 +556,14 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
   } else {
     // ------------------------------------------------------------ conversion of value tiles
     // A warp's pass covers 8 rows x 64 columns: lanes 0-3 the four 16-code pieces of one row, lanes 4-7 of the next,
-    // whose f16 pieces fall on the other banks (the swizzle flips with the row's parity).
-    constexpr int VP = 8 * C::V_CHUNKS / C::CONV_WARPS;  // passes a warp
-    constexpr int AHEAD = 6;                             // tiles between L2 prefetch and use
-    const int cw = warp - 6;
-    const int sub = lane >> 2, quarter = lane & 3;
+    // whose f16 pieces fall on the other banks (the swizzle flips with the row's parity). Every pass is a constant away
+    // from the lane's first place.
+    constexpr int CW = C::CONV_WARPS, VP = 8 * C::V_CHUNKS / CW;  // passes a warp
+    constexpr int AHEAD = 6;                                      // tiles between L2 prefetch and use
+    const int cw = warp - SOFT - 2;
+    const int row0 = cw * 8 + (lane >> 2), quarter = lane & 3;
+    const int from = row0 * HD + quarter * 16;
+    const int to = row0 * 128, piece0 = ((2 * quarter) ^ (row0 & 7)) << 4, piece1 = ((2 * quarter + 1) ^ (row0 & 7)) << 4;
     uint4 vr[VP];
     uint32_t g = 0;
     for (uint32_t k = 0;; ++k) {
@@ -495,11 +580,17 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         return j >= w.n ? -1 : (j >> 5) == batch ? x : y;
       };
       auto load_v = [&](int z, int keys) {  // keys: rows of the block that hold tokens; the rest may hold NaN codes
-        const uint8_t* p = v_codes + (int64_t)max(z, 0) * (BN * HD) + w.slice * DV;
+        const uint8_t* p = v_codes + (int64_t)max(z, 0) * (BN * HD) + w.slice * DV + from;
+        if (z >= 0 && keys >= BN) {
 #pragma unroll
-        for (int s = 0; s < VP; ++s) {
-          const int pass = s * C::CONV_WARPS + cw, row = (pass & 7) * 8 + sub, c = pass >> 3;
-          vr[s] = z >= 0 && row < keys ? load_codes(p + row * HD + c * 64 + quarter * 16) : make_uint4(0, 0, 0, 0);
+          for (int s = 0; s < VP; ++s)
+            vr[s] = load_codes(p + (s % (8 / CW)) * CW * 8 * HD + s / (8 / CW) * 64);
+        } else {
+#pragma unroll
+          for (int s = 0; s < VP; ++s)
+            vr[s] = z >= 0 && row0 + (s % (8 / CW)) * CW * 8 < keys
+                        ? load_codes(p + (s % (8 / CW)) * CW * 8 * HD + s / (8 / CW) * 64)
+                        : make_uint4(0, 0, 0, 0);
         }
       };
       const int last_key = w.lk - w.first * BN;  // keys from the item's first tile to the request's last token
@@ -518,18 +609,17 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         const uint32_t G = g + j;
         const int st = G % VST;
         if (!mbar_wait(&v_empty[st], ((G / VST) & 1) ^ 1, a.status)) goto done;
-        uint8_t* tile = s_v + st * C::V_BYTES;
+        uint8_t* tile = s_v + st * C::V_BYTES + to;
 #pragma unroll
         for (int s = 0; s < VP; ++s) {
-          const int pass = s * C::CONV_WARPS + cw, row = (pass & 7) * 8 + sub, c = pass >> 3;
-          uint8_t* dst = tile + c * C::V_CHUNK + row * 128;
+          uint8_t* dst = tile + s / (8 / CW) * C::V_CHUNK + (s % (8 / CW)) * CW * 8 * 128;
           uint4 lo, hi;
           codes_to_f16(vr[s].x, lo.x, lo.y);
           codes_to_f16(vr[s].y, lo.z, lo.w);
           codes_to_f16(vr[s].z, hi.x, hi.y);
           codes_to_f16(vr[s].w, hi.z, hi.w);
-          *reinterpret_cast<uint4*>(dst + (((2 * quarter) ^ (row & 7)) << 4)) = lo;
-          *reinterpret_cast<uint4*>(dst + (((2 * quarter + 1) ^ (row & 7)) << 4)) = hi;
+          *reinterpret_cast<uint4*>(dst + piece0) = lo;
+          *reinterpret_cast<uint4*>(dst + piece1) = hi;
         }
         load_v(z1, last_key - (j + 1) * BN);
         fence_async_smem();
@@ -541,99 +631,109 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
   }
   } else {
     if constexpr (C::SPLIT_REGISTERS) set_registers_up<168>();
-    // ------------------------------------------------------------ queries, softmax, epilogue (warps 0-3)
+    // ------------------------------------------------------------ queries, softmax, epilogue
     const int r = tid;  // the row within the tile = TMEM lane
     const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
     uint32_t g = 0;
     for (uint32_t k = 0;; ++k) {
       if (!mbar_wait(&item_full[k & 1], (k >> 1) & 1, a.status)) goto done;
-      const Work w = works[k & 1];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&item_empty[k & 1]);
+      const Work& w = works[k & 1];  // released after the epilogue: read again where it is needed
       if (w.i < 0) break;
       const int n = w.n;
       const bool live = r < w.rows, warp_live = warp * 32 < w.rows;
-      const int gr = w.r0 + (live ? r : 0);
-      const int tok = gr / a.group, head = w.h * a.group + gr - tok * a.group;
       float q_scale = 1.f;
       bool bad = false;  // an infinity or a NaN among the row's queries: NaN wherever it sees a key
       if (n > 0) {
         // The row's queries as hi + lo. The last item's products have read theirs: its last scores were waited for.
-        const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)(w.q0 + tok) * a.ldq + (int64_t)head * HD);
-        uint32_t top = 0;  // the largest magnitude as a bf16 pattern
-        if (live) {
-#pragma unroll 4
-          for (int c = 0; c < HD / 8; ++c) {
-            const uint4 x = src[c];
-            const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+        if (warp_live) {
+          const int gr = w.r0 + (live ? r : 0), tok = gr / a.group, head = w.h * a.group + gr - tok * a.group;
+          constexpr int PIECES = HD / 8;  // 8-element pieces of the row
+          constexpr int HELD = PIECES <= 16 ? PIECES : 16;
+          const uint4* src =
+              reinterpret_cast<const uint4*>(a.q + (int64_t)(w.q0 + tok) * a.ldq + (int64_t)head * HD);
+          uint4 x[HELD];
+          uint32_t top = 0;  // the largest magnitude as a bf16 pattern
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, max(v[e] & 0x7fffu, (v[e] >> 16) & 0x7fffu));
-          }
-        }
-        bad = top >= 0x7f80u;
-        // the least e with the largest magnitude within 448 = 1.75 * 2^8
-        const int e = min(max((int)(top >> 7) - 127 - 8 + ((top & 0x7fu) > 0x60u ? 1 : 0), -120), 120);
-        q_scale = pow2i(e);
-        const float inv = pow2i(-e);
-#pragma unroll 2
-        for (int c = 0; c < HD / 16; ++c) {
-          uint32_t hi[4], lo[4];
+          for (int c0 = PIECES - HELD; c0 >= 0; c0 -= HELD) {  // the first pieces last: they stay in registers
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint4 x = live ? src[2 * c + half] : make_uint4(0, 0, 0, 0);
-            const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+            for (int c = 0; c < HELD; ++c) x[c] = live ? src[c0 + c] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const float2 f = unpack_bf16x2(v[2 * y]), h = unpack_bf16x2(v[2 * y + 1]);
-              const float4 q4 = make_float4(f.x * inv, f.y * inv, h.x * inv, h.y * inv);
-              const uint32_t w0 = e4m3_pair(q4.x, q4.y), w1 = e4m3_pair(q4.z, q4.w);
-              hi[2 * half + y] = w0 | (w1 << 16);
-              uint32_t h0, h1;
-              codes_to_f16(hi[2 * half + y], h0, h1);
-              const float2 b0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-              const float2 b1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-              lo[2 * half + y] = e4m3_pair(q4.x - b0.x, q4.y - b0.y) | (e4m3_pair(q4.z - b1.x, q4.w - b1.y) << 16);
+            for (int c = 0; c < HELD; ++c) {
+              const uint32_t v[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) top = max(top, max(v[e] & 0x7fffu, (v[e] >> 16) & 0x7fffu));
             }
           }
-          const int at = swizzled<C::ROW>(r, c, C::Q_CHUNK);
-          *reinterpret_cast<uint4*>(s_q + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(s_q + C::Q_BYTES + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          bad = top >= 0x7f80u;
+          // the least e with the largest magnitude within 448 = 1.75 * 2^8
+          const int e = min(max((int)(top >> 7) - 127 - 8 + ((top & 0x7fu) > 0x60u ? 1 : 0), -120), 120);
+          q_scale = pow2i(e);
+          const float inv = pow2i(-e);
+#pragma unroll
+          for (int c0 = 0; c0 < PIECES; c0 += HELD) {
+            if (c0 > 0) {
+#pragma unroll
+              for (int c = 0; c < HELD; ++c) x[c] = live ? src[c0 + c] : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int c = 0; c < HELD; c += 2) {
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const uint4 xv = x[c + y / 2];
+                const float2 f = unpack_bf16x2(y & 1 ? xv.z : xv.x), h = unpack_bf16x2(y & 1 ? xv.w : xv.y);
+                const float4 q4 = make_float4(f.x * inv, f.y * inv, h.x * inv, h.y * inv);
+                hi[y] = e4m3_pair(q4.x, q4.y) | (e4m3_pair(q4.z, q4.w) << 16);
+                uint32_t h0, h1;
+                codes_to_f16(hi[y], h0, h1);
+                const float2 b0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+                const float2 b1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                lo[y] = e4m3_pair(q4.x - b0.x, q4.y - b0.y) | (e4m3_pair(q4.z - b1.x, q4.w - b1.y) << 16);
+              }
+              const int piece = (c0 + c) / 2, at = swizzled<C::ROW>(r, piece, C::Q_CHUNK);
+              if constexpr (C::Q_TMEM) {
+                tmem_st4(lane_base + C::HI_COL + 4 * piece, hi);
+                tmem_st4(lane_base + C::LO_COL + 4 * piece, lo);
+              } else {
+                *reinterpret_cast<uint4*>(s_q + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(s_q + C::Q_BYTES + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              }
+            }
+          }
+          if constexpr (C::Q_TMEM) {
+            tmem_st_wait();
+            tc_fence_before();
+          } else {
+            fence_async_smem();
+          }
         }
-        fence_async_smem();
-        mbar_arrive(&q_full);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full);  // rows of other warps hold anything: they are never read back
       }
-      const int off = w.lk - w.lq;
-      const int pos0 = w.r0 / a.group + off, pos1 = (w.r0 + w.rows - 1) / a.group + off;  // the tile's first, last row
-      const int pos = tok + off;
-      const int key_lo = a.left >= 0 ? pos - a.left : 0;
-      const int key_hi = a.right >= 0 ? min(w.lk - 1, pos + a.right) : w.lk - 1;
+      // The row's visible keys [key_lo, key_hi], from the item's first tile on, and the tiles [clear0, clear1) that every
+      // row of the tile sees whole.
+      int key_lo, key_hi, clear0 = 0, clear1;
+      {
+        const int off = w.lk - w.lq, first = w.first * BN;
+        const int pos0 = w.r0 / a.group + off, pos1 = (w.r0 + w.rows - 1) / a.group + off;
+        const int pos = (w.r0 + (live ? r : 0)) / a.group + off;
+        key_lo = (a.left >= 0 ? max(pos - a.left, 0) : 0) - first;
+        key_hi = (a.right >= 0 ? min(w.lk - 1, pos + a.right) : w.lk - 1) - first;
+        const int end = a.right >= 0 ? min(w.lk, pos0 + a.right + 1) : w.lk;
+        clear1 = end <= 0 ? 0 : end / BN - w.first;
+        if (a.left >= 0) clear0 = (max(pos1 - a.left, 0) + BN - 1) / BN - w.first;
+      }
+      q_scale *= a.scale_log2;
       // running maxima in log2 units, possibly stale by the threshold: of x (the row sum's base) and of x + e_v (O's)
       float m = -INFINITY, big = -INFINITY, l = 0.f;
-      Lookup now{-1, 0.f, 0}, ahead{-1, 0.f, 0};
-      auto look_up = [&](int j) {
-        Lookup x{block_of(a, w, j), 0.f, 0};
-        if (x.z >= 0) {
-          x.k_scale = a.k_scale[x.z];
-          x.v_exp = exponent_of(a.v_scale[x.z]);
-        }
-        return x;
-      };
-      if (warp_live) ahead = look_up(lane);
-      for (int j = 0; j < n; ++j) {
-        if ((j & 31) == 0 && warp_live) {
-          now = ahead;
-          ahead = look_up(j + 32 + lane);
-        }
-        const int z = __shfl_sync(0xffffffffu, now.z, j & 31);
-        const float ks = __shfl_sync(0xffffffffu, now.k_scale, j & 31);
-        const float ve = (float)__shfl_sync(0xffffffffu, now.v_exp, j & 31);
+      float ve_max = -1000.f;  // the largest value exponent so far (the same for every row)
+      // One key tile. GENERAL: some key is hidden from some row, the block is absent, or its value scale lies so far under
+      // an earlier one's that a probability that counts could vanish beside a larger scaled one, so that the row sum takes
+      // exponentials of its own. The other form has no selects and one exponential for both.
+      auto tile = [&](auto general, int j, const Info& info) -> bool {
+        constexpr bool GENERAL = decltype(general)::value;
         const uint32_t G = g + j;
-        if (!mbar_wait(&s_full[G % NS], (G / NS) & 1, a.status)) goto done;
-        if (!warp_live) {  // no row of this warp: its probabilities are never read back
-          mbar_arrive(&p_full[G % NS]);
-          continue;
-        }
-        tc_fence_after();
+        const float mul = score_factor(q_scale, info.k_scale), ve = info.v_exp;
         const uint32_t s_addr = lane_base + C::S_COL + (G % NS) * BN;
         float sv[BN];
         {
@@ -647,11 +747,8 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
             sv[32 + e] = __uint_as_float(t1[e]);
           }
         }
-        const int key0 = (w.first + j) * BN;
-        const bool edge = z < 0 || key0 + BN > w.lk || (a.right >= 0 && key0 + BN - 1 > pos0 + a.right) ||
-                          (a.left >= 0 && key0 < pos1 - a.left);
-        if (edge) {
-          const int lo = z < 0 ? BN : key_lo - key0, hi = key_hi - key0;
+        if constexpr (GENERAL) {
+          const int lo = info.live ? key_lo - j * BN : BN, hi = key_hi - j * BN;
 #pragma unroll
           for (int e = 0; e < BN; ++e) sv[e] = (e >= lo && e <= hi) ? sv[e] : -INFINITY;
         }
@@ -661,47 +758,77 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
 #pragma unroll
         for (int e = 8; e < BN; e += 2) mx[(e / 2) & 7] = max3(mx[(e / 2) & 7], sv[e], sv[e + 1]);
         const float mraw = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
-        const float mul = score_factor(q_scale, ks, a.scale_log2);
-        const float mt = mraw == -INFINITY ? -INFINITY : mraw * mul;
+        const float mt = GENERAL && mraw == -INFINITY ? -INFINITY : mraw * mul;
+        const bool need = mt + ve > big + THRESHOLD;
+        if (__any_sync(0xffffffffu, need)) {
+          const float f = need ? fast_exp2(big - (mt + ve)) : 1.f;
+          if (j > 0) {  // rows that saw nothing so far hold zeros
+            if (!mbar_wait(&pv_done[(G - 1) % NS], ((G - 1) / NS) & 1, a.status)) return false;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < DV; c += 32) {
+              uint32_t t[32];
+              tmem_ld32(lane_base + C::O_COL + c, t);
+              tmem_ld_wait_regs(t);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) t[e] = __float_as_uint(__uint_as_float(t[e]) * f);
+              tmem_st32(lane_base + C::O_COL + c, t);
+            }
+            tmem_st_wait();
+          }
+          if (need) big = mt + ve;
+        }
         if (mt > m + THRESHOLD) {
           l *= fast_exp2(m - mt);
           m = mt;
         }
-        const bool need = mt + ve > big + THRESHOLD;
-        const float f = need ? fast_exp2(big - (mt + ve)) : 1.f;
-        if (j > 0 && __any_sync(0xffffffffu, need && big != -INFINITY)) {
-          if (!mbar_wait(&pv_done[(G - 1) % NS], ((G - 1) / NS) & 1, a.status)) goto done;
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < DV; c += 32) {
-            uint32_t t[32];
-            tmem_ld32(lane_base + C::O_COL + c, t);
-            tmem_ld_wait_regs(t);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) t[e] = __float_as_uint(__uint_as_float(t[e]) * f);
-            tmem_st32(lane_base + C::O_COL + c, t);
-          }
-          tmem_st_wait();
-        }
-        if (need) big = mt + ve;
-        const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
-        const float factor = fast_exp2(fminf(base - vbase + ve, 110.f)) * P_SCALE;
+        uint32_t pk[BN / 2];
         float2 part[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
-        const float2 mul2v = make_float2(mul, mul), base2 = make_float2(-base, -base), fac2 = make_float2(factor, factor);
-        uint32_t pk[32];
+        const float2 mul2v = make_float2(mul, mul);
+        if constexpr (!GENERAL) {
+          // What goes to the tensor cores is 2^(x + e_v + 11 - M); its sum times 2^(M - e_v - 11 - m) is the row sum's part.
+          const float shift = big - ve - P_EXPONENT;
+          const float2 shift2 = make_float2(-shift, -shift);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float2 x = fma2(make_float2(sv[2 * e], sv[2 * e + 1]), mul2v, base2);
-          float2 p = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-          part[e & 3] = add2(part[e & 3], p);
-          p = mul2(p, fac2);
-          pk[e] = pack_f16x2(p.x, p.y);
+          for (int e = 0; e < BN / 2; ++e) {
+            const float2 x = fma2(make_float2(sv[2 * e], sv[2 * e + 1]), mul2v, shift2);
+            const float2 p = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            part[e & 3] = add2(part[e & 3], p);
+            pk[e] = pack_f16x2(p.x, p.y);
+          }
+          const float2 ps = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+          l += (ps.x + ps.y) * fast_exp2(shift - m);
+        } else {
+          const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
+          const float2 base2 = make_float2(-base, -base);
+          const float factor = fast_exp2(fminf(base - vbase + ve + P_EXPONENT, 126.f));
+#pragma unroll
+          for (int e = 0; e < BN / 2; ++e) {
+            const float2 x = fma2(make_float2(sv[2 * e], sv[2 * e + 1]), mul2v, base2);
+            const float2 p = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            part[e & 3] = add2(part[e & 3], p);
+            pk[e] = pack_f16x2(p.x * factor, p.y * factor);
+          }
+          const float2 ps = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+          l += ps.x + ps.y;
         }
         tmem_st32(s_addr, pk);
-        const float2 ps = add2(add2(part[0], part[1]), add2(part[2], part[3]));
-        l += ps.x + ps.y;
         tmem_st_wait();
         tc_fence_before();
+        return true;
+      };
+      for (int j = 0; j < n; ++j) {
+        const uint32_t G = g + j;
+        if (!mbar_wait(&s_full[G % NS], (G / NS) & 1, a.status)) goto done;
+        if (warp_live) {  // else no row of this warp: its probabilities are never read back
+          tc_fence_after();
+          const Info info = infos[G & 7];
+          const bool ok = j < clear0 || j >= clear1 || !info.live || ve_max - info.v_exp > 80.f
+                              ? tile(std::true_type{}, j, info)
+                              : tile(std::false_type{}, j, info);
+          if (!ok) goto done;
+          ve_max = fmaxf(ve_max, info.v_exp);
+        }
         mbar_arrive(&p_full[G % NS]);
       }
       // ---- epilogue
@@ -713,57 +840,87 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
       if (warp_live) {
         if (bad && l != 0.f) l = __int_as_float(0x7fffffff);
         const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
-        const int64_t row = w.q0 + tok, col = (int64_t)head * HD + w.slice * DV;
+        const int gr = w.r0 + (live ? r : 0), tok = gr / a.group, head = w.h * a.group + gr - tok * a.group;
+        const uint32_t o_addr = lane_base + C::O_COL;
         if (w.slot < 0) {
+          // Through the warp's staging area (its rows' first chunk of the query tile, read by now), CC columns at a time:
+          // the gate's rows in and the output's rows out as whole lines, ROW bytes of a row by ROW / 16 lanes.
+          constexpr int CC = C::ROW / 2, LPR = C::ROW / 16, RPP = 32 / LPR;
+          uint8_t* stage = s_stage + warp * 32 * C::ROW;
+          const int piece = lane % LPR, sub = lane / LPR;
+          const int64_t at = (int64_t)head * HD + w.slice * DV;
+          const int64_t orow = (int64_t)(w.q0 + tok) * a.ldo + at, grow = (int64_t)(w.q0 + tok) * a.ldg + at;
           const float fin = l == 0.f ? 0.f : fast_exp2(fminf(vbase - base, 126.f)) / (l * P_SCALE);
-          const bool gated = a.gate && l != 0.f && live;
-          const uint4* gp = reinterpret_cast<const uint4*>(a.gate + row * a.ldg + col);
-          uint4* op = reinterpret_cast<uint4*>(a.out + row * a.ldo + col);
 #pragma unroll 1
-          for (int c = 0; c < DV; c += 32) {
-            uint32_t t[32];
-            __syncwarp();
-            if (n > 0) {
-              tmem_ld32(lane_base + C::O_COL + c, t);
-              tmem_ld_wait_regs(t);
-            }
+          for (int c = 0; c < DV; c += CC) {
+            if (a.gate) {
+              uint4 gv[LPR];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float x[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = l == 0.f ? 0.f : __uint_as_float(t[8 * q + e]) * fin;
-              if (gated) {
-                const uint4 gv = gp[c / 8 + q];
-                const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float2 s = unpack_bf16x2(gw[e]);
-                  x[2 * e] = x_sigmoid(x[2 * e], s.x);
-                  x[2 * e + 1] = x_sigmoid(x[2 * e + 1], s.y);
-                }
+              for (int p = 0; p < LPR; ++p) {
+                const int rr = p * RPP + sub;
+                const int64_t from = __shfl_sync(0xffffffffu, grow, rr) + c + piece * 8;
+                gv[p] = warp * 32 + rr < w.rows ? *reinterpret_cast<const uint4*>(a.gate + from) : make_uint4(0, 0, 0, 0);
               }
-              if (live)
-                op[c / 8 + q] = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
-                                           pack_bf16x2(x[6], x[7]));
+#pragma unroll
+              for (int p = 0; p < LPR; ++p)
+                *reinterpret_cast<uint4*>(stage + swizzled<C::ROW>(p * RPP + sub, piece, 0)) = gv[p];
+              __syncwarp();
             }
+#pragma unroll
+            for (int c2 = 0; c2 < CC; c2 += 32) {
+              uint32_t t[32];
+              if (n > 0) {
+                tmem_ld32(o_addr + c + c2, t);
+                tmem_ld_wait_regs(t);
+              }
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                uint4* mine = reinterpret_cast<uint4*>(stage + swizzled<C::ROW>(lane, c2 / 8 + q, 0));
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = l == 0.f ? 0.f : __uint_as_float(t[8 * q + e]) * fin;
+                if (a.gate && l != 0.f) {
+                  const uint4 gq = *mine;
+                  const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const float2 s = unpack_bf16x2(gw[e]);
+                    x[2 * e] = x_sigmoid(x[2 * e], s.x);
+                    x[2 * e + 1] = x_sigmoid(x[2 * e + 1], s.y);
+                  }
+                }
+                *mine = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                                   pack_bf16x2(x[6], x[7]));
+              }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int p = 0; p < LPR; ++p) {
+              const int rr = p * RPP + sub;
+              const int64_t to = __shfl_sync(0xffffffffu, orow, rr) + c + piece * 8;
+              const uint4 y = *reinterpret_cast<const uint4*>(stage + swizzled<C::ROW>(rr, piece, 0));
+              if (warp * 32 + rr < w.rows) *reinterpret_cast<uint4*>(a.out + to) = y;
+            }
+            __syncwarp();
           }
         } else {
+          // [DV / 4][128 rows][4]: a warp's stores are whole lines; then m, M and l per row
           float* part = a.partials + (int64_t)w.slot * C::PARTIAL;
           if (live) {
-            part[C::BM * DV + 3 * r] = m;
-            part[C::BM * DV + 3 * r + 1] = big;
-            part[C::BM * DV + 3 * r + 2] = l;
+            part[C::BM * DV + r] = m;
+            part[C::BM * DV + 128 + r] = big;
+            part[C::BM * DV + 256 + r] = l;
           }
 #pragma unroll 1
           for (int c = 0; c < DV; c += 32) {
             uint32_t t[32];
             __syncwarp();
-            tmem_ld32(lane_base + C::O_COL + c, t);
+            tmem_ld32(o_addr + c, t);
             tmem_ld_wait_regs(t);
             if (live) {
 #pragma unroll
               for (int q = 0; q < 8; ++q)
-                *reinterpret_cast<uint4*>(part + r * DV + c + 4 * q) =
+                *reinterpret_cast<uint4*>(part + ((c / 4 + q) * 128 + r) * 4) =
                     make_uint4(t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]);
             }
           }
@@ -771,6 +928,8 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         // the next item's first product overwrites O: every row of this warp has read it
         tc_fence_before();
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[k & 1]);
       g += n;
     }
   }
@@ -778,132 +937,115 @@ done:
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) {
+  if (warp == SOFT + 1) {
     __syncwarp();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
 }
 
-// Joins the partials of an item that spans several CTAs' shares. blockIdx.x: the share whose beginning lies inside the
-// item, the first such one of the item; blockIdx.y: 32 of its 128 rows, a warp for each fourth. The lanes read the
-// partials' statistics together and weigh them; the sums then run in key order with their loads in flight.
+// Joins the partials of the item that CTA blockIdx.x began and later ones finished, 8 of its 128 rows a block. The
+// partials' statistics first, all at once, to a weight for each; then a thread sums 4 columns of a row over the partials
+// in key order, eight loads in flight.
+constexpr int JOIN_MOST = 320;  // partials of an item: at most the CTAs
 template <int HD, int DV>
-__global__ void __launch_bounds__(256) join_tiles_kernel(Args a, int ctas) {
+__global__ void __launch_bounds__(2 * DV) join_tiles_kernel(Args a, int ctas) {
   using C = Cfg<HD, DV>;
-  constexpr int V = DV / 32;  // columns a lane holds
-  const int c = blockIdx.x + 1, lane = threadIdx.x & 31;
-  const int64_t total = a.tile_cu[a.n];
-  const int np = parts(total, a.group, ctas);
-  if (c >= np || total == 0) return;
-  const int64_t x = total * c / np;  // share c begins here; share c - 1 ends
-  int lo = 0, hi = a.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (a.tile_cu[mid] <= x)
-      lo = mid;
-    else
-      hi = mid - 1;
+  constexpr int GROUPS = 2 * DV / 8;  // threads that share a row
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the partials are there after this
+  const Split it = reinterpret_cast<const Split*>(a.splits)[blockIdx.x];
+  if ((int)blockIdx.y * 8 >= it.rows) return;
+  const int first = blockIdx.x, n = it.last - first + 1;
+  const int sub = threadIdx.x & 7, c4 = threadIdx.x >> 3, r = blockIdx.y * 8 + sub;
+  const bool live = r < it.rows;
+  __shared__ float s_w[JOIN_MOST][8];
+  __shared__ float s_red[3][2 * DV / 32][8];
+  __shared__ int s_slot[JOIN_MOST];  // < 0: the share holds none of the item's tiles
+  for (int p = threadIdx.x; p < n; p += 2 * DV) {
+    const int64_t x0 = quotient(it.total * (first + p), it.np), x1 = quotient(it.total * (first + p + 1), it.np);
+    int t0, t1;
+    portion(it.begin, it.end, max(x0, it.begin), min(x1, it.end), it.tiles, t0, t1);
+    s_slot[p] = t0 < t1 ? 2 * (first + p) + (p == 0 ? 1 : 0) : -1;
   }
-  Item it;
-  find<C::SLICES>(a, lo, a.tile_cu[lo], x, it);
-  if (it.begin >= x || (c > 1 && total * (c - 1) / np > it.begin)) return;
-  const int rows = (int)min((int64_t)128, (int64_t)it.s.lq * a.group - it.tile * 128);
-  const Tiles v = visible(a, it.s, it.tile);
-  int last = c;  // the last share that meets the item
-  {
-    // share p holds weight y when floor(p total / np) <= y: the one holding the item's last weight
-    last = (int)((it.end * np - 1) / total);
-    if (last >= np) last = np - 1;
+  __syncthreads();
+  float m = -INFINITY, big = -INFINITY;
+  for (int p = c4; p < n; p += GROUPS) {
+    const int slot = s_slot[p];
+    if (slot < 0 || !live) continue;
+    const float* st = a.partials + (int64_t)slot * C::PARTIAL + C::BM * DV + r;
+    m = fmaxf(m, st[0]);
+    big = fmaxf(big, st[128]);
   }
-  const int first = c - 1, n = last - first + 1;
-  for (int r = blockIdx.y * 32 + threadIdx.x / 32; r < min(rows, (int)blockIdx.y * 32 + 32); r += 8) {
-    const int gr = it.tile * 128 + r;
-    const int tok = gr / a.group, head = it.h * a.group + gr - tok * a.group;
-    float m = -INFINITY, big = -INFINITY, l = 0.f, o[V];
+  auto across = [&](float v, int which, auto op) -> float {  // over the threads of a row
+    v = op(v, __shfl_xor_sync(0xffffffffu, v, 8));
+    v = op(v, __shfl_xor_sync(0xffffffffu, v, 16));
+    if ((threadIdx.x & 31) < 8) s_red[which][threadIdx.x / 32][sub] = v;
+    __syncthreads();
+    v = s_red[which][0][sub];
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = 0.f;
-    for (int p0 = 0; p0 < n; p0 += 32) {
-      const int p = first + p0 + lane;
-      float pm = -INFINITY, pb = -INFINITY, pl = 0.f;
-      const float* part = a.partials;
-      if (p <= last) {
-        const int64_t x0 = total * p / np, x1 = total * (p + 1) / np;
-        int t0, t1;
-        portion(it, max(x0, it.begin), min(x1, it.end), v.n, t0, t1);
-        part += (int64_t)(2 * p + (it.begin < x0 ? 0 : 1)) * C::PARTIAL;
-        if (t0 < t1) {
-          pm = part[C::BM * DV + 3 * r];
-          pb = part[C::BM * DV + 3 * r + 1];
-          pl = part[C::BM * DV + 3 * r + 2];
-        }
-      }
-      float m_new = pm, big_new = pb;
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) {
-        m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, s));
-        big_new = fmaxf(big_new, __shfl_xor_sync(0xffffffffu, big_new, s));
-      }
-      m_new = fmaxf(m_new, m);
-      big_new = fmaxf(big_new, big);
-      const float base = m_new == -INFINITY ? 0.f : m_new, vbase = big_new == -INFINITY ? 0.f : big_new;
-      float sum = pl * fast_exp2(pm - base);
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-      l = l * fast_exp2(m - base) + sum;
-      const float f0 = fast_exp2(big - vbase), f1 = pb == -INFINITY && pl == 0.f ? -1.f : fast_exp2(pb - vbase);
-#pragma unroll
-      for (int e = 0; e < V; ++e) o[e] *= f0;
-      m = m_new;
-      big = big_new;
-      const int count = min(32, n - p0);
-      const uint64_t mine = reinterpret_cast<uint64_t>(part + r * DV);
-#pragma unroll 4
-      for (int q = 0; q < count; ++q) {
-        const float f = __shfl_sync(0xffffffffu, f1, q);
-        const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, mine, q)) + lane * V;
-        if (f < 0.f) continue;  // no key of the row (the partial may hold nothing)
-        if constexpr (V >= 4) {
-#pragma unroll
-          for (int e = 0; e < V; e += 4) {
-            const float4 y = *reinterpret_cast<const float4*>(src + e);
-            o[e] += y.x * f;
-            o[e + 1] += y.y * f;
-            o[e + 2] += y.z * f;
-            o[e + 3] += y.w * f;
-          }
-        } else {
-          const float2 y = *reinterpret_cast<const float2*>(src);
-          o[0] += y.x * f;
-          o[1] += y.y * f;
-        }
-      }
+    for (int q = 1; q < 2 * DV / 32; ++q) v = op(v, s_red[which][q][sub]);
+    return v;
+  };
+  m = across(m, 0, [](float x, float y) { return fmaxf(x, y); });
+  big = across(big, 1, [](float x, float y) { return fmaxf(x, y); });
+  const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
+  float l = 0.f;
+  for (int p = c4; p < n; p += GROUPS) {
+    const int slot = s_slot[p];
+    float f = -1.f;
+    if (slot >= 0 && live) {
+      const float* st = a.partials + (int64_t)slot * C::PARTIAL + C::BM * DV + r;
+      l += st[256] * fast_exp2(st[0] - base);
+      if (st[128] != -INFINITY || st[256] != 0.f) f = fast_exp2(st[128] - vbase);
     }
-    const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
-    const float fin = l == 0.f ? 0.f : fast_exp2(fminf(vbase - base, 126.f)) / (l * P_SCALE);
-    const int64_t row = it.s.q0 + tok, col = (int64_t)head * HD + it.slice * DV + lane * V;
-    float y[V];
+    s_w[p][sub] = f;  // < 0: no key of the row (its sums may hold anything)
+  }
+  l = across(l, 2, [](float x, float y) { return x + y; });
+  if (!live) return;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < n; p0 += 8) {
+    float4 y[8];
+    float f[8];
 #pragma unroll
-    for (int e = 0; e < V; ++e) y[e] = l == 0.f ? 0.f : o[e] * fin;
-    if (a.gate && l != 0.f) {
-#pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        const float2 s = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(a.gate + row * a.ldg + col + e));
-        y[e] = x_sigmoid(y[e], s.x);
-        y[e + 1] = x_sigmoid(y[e + 1], s.y);
-      }
+    for (int q = 0; q < 8; ++q) {
+      f[q] = p0 + q < n ? s_w[p0 + q][sub] : -1.f;
+      y[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (f[q] >= 0.f || f[q] != f[q])
+        y[q] = *reinterpret_cast<const float4*>(a.partials + (int64_t)s_slot[p0 + q] * C::PARTIAL + (c4 * 128 + r) * 4);
     }
 #pragma unroll
-    for (int e = 0; e < V; e += 2)
-      *reinterpret_cast<uint32_t*>(a.out + row * a.ldo + col + e) = pack_bf16x2(y[e], y[e + 1]);
+    for (int q = 0; q < 8; ++q) {
+      const float w = f[q] < 0.f ? 0.f : f[q];
+      o.x += y[q].x * w;
+      o.y += y[q].y * w;
+      o.z += y[q].z * w;
+      o.w += y[q].w * w;
+    }
   }
+  const float fin = l == 0.f ? 0.f : fast_exp2(fminf(vbase - base, 126.f)) / (l * P_SCALE);
+  const int gr = it.r0 + r, tok = gr / a.group, head = it.h * a.group + gr - tok * a.group;
+  const int64_t row = it.q0 + tok, col = (int64_t)head * HD + it.slice * DV + 4 * c4;
+  float x[4] = {o.x * fin, o.y * fin, o.z * fin, o.w * fin};
+  if (l == 0.f) {
+    x[0] = x[1] = x[2] = x[3] = 0.f;
+  } else if (a.gate) {
+    const uint2 g = *reinterpret_cast<const uint2*>(a.gate + row * a.ldg + col);
+    const float2 s0 = unpack_bf16x2(g.x), s1 = unpack_bf16x2(g.y);
+    x[0] = x_sigmoid(x[0], s0.x);
+    x[1] = x_sigmoid(x[1], s0.y);
+    x[2] = x_sigmoid(x[2], s1.x);
+    x[3] = x_sigmoid(x[3], s1.y);
+  }
+  *reinterpret_cast<uint2*>(a.out + row * a.ldo + col) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
 }
 
-static int64_t header_bytes(int n) { return ((int64_t)(n + 1) * 8 + 15) / 16 * 16; }
+// Scratch: a Split per CTA, two partials per CTA.
+static int64_t header_bytes(int ctas) { return ((int64_t)ctas * sizeof(Split) + 15) / 16 * 16; }
 
 template <int HD, int DV>
-int64_t workspace(int n, int sms) {
+int64_t workspace(int sms) {
   using C = Cfg<HD, DV>;
-  return header_bytes(n) + (int64_t)2 * sms * C::CTAS_PER_SM * C::PARTIAL * (int64_t)sizeof(float);
+  const int64_t ctas = (int64_t)sms * C::CTAS_PER_SM;
+  return header_bytes((int)ctas) + 2 * ctas * C::PARTIAL * (int64_t)sizeof(float);
 }
 
 template <int HD, int DV>
@@ -912,11 +1054,12 @@ int launch(Args a, const void* k_codes, const uint8_t* v_codes, uint8_t* ws, int
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return set_error(KD_ERR_ARGUMENT, "attention_cache: device index");
-  const int sms = num_sms(dev), ctas = sms * C::CTAS_PER_SM;
-  if (ws_bytes < workspace<HD, DV>(a.n, sms))
+  const int sms = num_sms(dev), ctas = min(sms * C::CTAS_PER_SM, JOIN_MOST);
+  if (ws_bytes < workspace<HD, DV>(sms))
     return set_error(KD_ERR_ARGUMENT, "attention_cache: workspace smaller than kd_attention_cache_workspace");
-  a.tile_cu = reinterpret_cast<int64_t*>(ws);
-  a.partials = reinterpret_cast<float*>(ws + header_bytes(a.n));
+  a.splits = ws;
+  a.partials = reinterpret_cast<float*>(ws + header_bytes(ctas));
+  static_assert(sizeof(Shared<HD, DV>) <= C::SMEM - C::TILES, "shared memory layout");
   auto kernel = row_tiles_kernel<HD, DV>;
   static bool configured[64] = {false};
   if (!configured[dev]) {
@@ -931,20 +1074,19 @@ int launch(Args a, const void* k_codes, const uint8_t* v_codes, uint8_t* ws, int
     return rc;
   kernel<<<ctas, C::THREADS, C::SMEM, stream>>>(mk, a, v_codes);
   if (int rc = record_cuda_error(cudaGetLastError(), "attention_cache: launch")) return rc;
-  join_tiles_kernel<HD, DV><<<dim3(ctas - 1 > 0 ? ctas - 1 : 1, 4), 256, 0, stream>>>(a, ctas);
-  return record_cuda_error(cudaGetLastError(), "attention_cache: join launch");
+  return launch_after(join_tiles_kernel<HD, DV>, dim3(ctas, 16), 2 * DV, stream, a, ctas);
 }
 
 }  // namespace ct
 
 namespace ca {
 
-int64_t row_tiles_workspace(int head_dim, int n, int sms) {
+int64_t row_tiles_workspace(int head_dim, int sms) {
   switch (head_dim) {
-    case 64: return ct::workspace<64, 64>(n, sms);
-    case 128: return ct::workspace<128, 128>(n, sms);
-    case 256: return ct::workspace<256, 256>(n, sms);
-    default: return ct::workspace<512, 256>(n, sms);
+    case 64: return ct::workspace<64, 64>(sms);
+    case 128: return ct::workspace<128, 128>(sms);
+    case 256: return ct::workspace<256, 256>(sms);
+    default: return ct::workspace<512, 256>(sms);
   }
 }
 
