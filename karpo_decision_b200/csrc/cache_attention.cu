@@ -8,59 +8,80 @@
 //
 // Few query rows per key/value head (the rows of a request that share a head's keys: Lq * Hq / Hkv) are bound by the
 // reads of the codes: 2 hd bytes a token and head, once. The work is the list of key tiles (one block of 64 tokens) of
-// every (request, key/value head, 16-row tile), in that order; CTA c of P takes the tiles [c, c + 1) * total / P of
-// it, so long and short requests balance to a tile without the host knowing a length. A producer warp reads 32 tiles'
-// table entries and scales at a time and feeds a ring per key group by TMA; each key group (one warp, or a warp
-// per 128 value columns of wide heads) takes every KG-th tile with its own running maximum and sums, and leaves a
-// partial result per 16-row tile that it met; a second launch joins them.
+// every (request, key/value head, row tile), in that order; CTA c of P takes the tiles [c, c + 1) * total / P of it, so
+// long and short requests balance to a tile without the host knowing a length. A producer warp reads 32 tiles' table
+// entries and scales at a time and keeps a ring of 192 KB filled by TMA; eight warps take the tiles in turn (teams of
+// two or four for heads of 256 and 512, each warp a part of the tile's keys), each with a running maximum and sums of
+// its own, and leave a partial result per item that they met; a second launch joins them.
 //
-// The products run on mma.sync.m16n8k16 in f16 with float32 accumulation: 16 query rows against 64 keys fit its shape
-// (a 128-row tcgen05 tile would be mostly empty), and the codes turn into f16 exactly, two per conversion. Queries are
-// scaled by a power of two per row (exact; f16 holds every bf16 within 2^-24 of the row's largest magnitude).
-// Probabilities are rounded to f16 relative to the largest *scaled* probability p 2^e_v met (11 bits, exponents down
-// to 2^-39 of it), so the blocks' value scales need no product of their own; the sum of the probabilities stays in
-// float32, unrounded.
+// The products run on mma.sync.m16n8k16 in f16 with float32 sums, keys and values as the 16-row operand and the query
+// rows as the 8 columns: S^T = K Q^T, O^T = V^T P^T. Eight rows then cost half of what a 16-row query tile would, and
+// nothing is padded further (a 128-row tcgen05 tile would be mostly empty). The codes turn into f16 exactly, two per
+// instruction; ldmatrix hands a thread four neighbouring dims of a key, or two of two keys, and the dims' order within
+// the products is permuted to match, so no byte moves but one permute per four value codes. Queries are scaled by a power
+// of two per row (exact; f16 holds every bf16 within 2^-24 of the row's largest magnitude). Probabilities are rounded to
+// f16 relative to the largest *scaled* probability p 2^e_v met (11 bits, exponents down to 2^-35 of it), so the blocks'
+// value scales need no product of their own; the sum of the probabilities stays in float32, unrounded.
 #include "cache_attention.cuh"
 
 namespace kd {
 namespace ca {
 
-constexpr float P_SCALE = 32768.f;  // f16 probabilities hold p * 2^15 (at most 2^15; subnormal below 2^-29)
+constexpr float THRESHOLD = 4.0f;  // log2 units a row's maximum may grow before its sums are rescaled
+constexpr float P_EXPONENT = 11.f, P_SCALE = 2048.f;  // f16 probabilities hold p * 2^11: at most 2^15 with the threshold
 
-template <int HD>
+// HD: head dim. NT: tiles of 8 query rows a warp holds. Registers bound both (three warpgroups launched at 168, of which the
+// consumers' two take 224 and leave the producer's 56): a thread holds
+// HD NT / 4 sums of the output, and the scores of its keys, for 32 rows of 32 or 16 of them at a time.
+template <int HD, int NT>
 struct Cfg {
-  static constexpr int DV = HD < 128 ? HD : 128;  // value columns of a warp
-  static constexpr int SL = HD / DV;              // warps of a key group
-  static constexpr int KG = HD == 64 ? 8 : HD == 128 ? 4 : HD == 256 ? 2 : 1;  // key groups
-  static constexpr int WARPS = KG * SL;
-  static constexpr int THREADS = 32 * (WARPS + 1);
+  static constexpr int RT = 8 * NT;                // query rows of an item
+  static constexpr int WARPS = 8, THREADS = 32 * (WARPS + 4);  // a third warpgroup for the producer, three warps idle
+  static constexpr int KW = HD <= 128 ? 1 : HD / 128;  // warps that share a tile, each 64 / KW of its keys
+  static constexpr int TEAMS = WARPS / KW;
+  static constexpr int PARTS = NT < 4 ? 1 : HD == 128 ? 4 : 2;    // steps in which a warp takes its keys
+  static constexpr int MT = BN / KW / PARTS / 16;  // 16-key tiles of a step
   static constexpr int BOX = HD < 128 ? HD : 128;  // bytes of a TMA box row (its swizzle span)
   static constexpr int CHUNKS = HD / BOX;
   static constexpr int TILE_BYTES = BN * HD;
-  static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
-  static constexpr int STAGES = HD == 64 ? 2 : 3;
-  static constexpr int Q_BYTES = RT * HD * 2;  // per key group, in fragment order
-  static constexpr int SMEM = KG * (STAGES * STAGE_BYTES + Q_BYTES) + 1024 + 1024;
-  static constexpr int PARTIAL = RT * (HD + 3);  // floats of one group's partial: O, then (m, M, l) per row
-  static_assert(SMEM <= 227 * 1024, "shared memory budget");
+  static constexpr int SLOT_BYTES = 2 * TILE_BYTES;
+  static constexpr int SLOTS = 192 * 1024 / SLOT_BYTES;
+  static constexpr int Q_BYTES = RT * HD * 2;      // of one item's queries, in the order of the B fragments
+  static constexpr int SMEM = SLOTS * SLOT_BYTES + 2 * Q_BYTES + 1024;
+  static constexpr int PARTIAL = RT * (HD + 3);    // floats of one warp's partial: O, then (m, M, l) per row
+  static_assert(SMEM + 2048 <= 227 * 1024, "shared memory budget");
 };
 
-// A position in the list of key tiles: request > key/value head > 16-row tile > key tile. `advance(g)` moves forward to
-// the item holding tile g.
+// A request's items: tiles of RT rows of a key/value head, each with the same key tiles.
+struct Rows {
+  Request r;
+  int nrt;
+};
+template <int RT>
+KD_DEVICE Rows rows_of(const Args& a, int i) {
+  Rows x;
+  x.r = request(a, i);
+  x.nrt = (int)(((int64_t)x.r.lq * a.group + RT - 1) / RT);
+  return x;
+}
+
+// A position in the list of key tiles: request > key/value head > row tile > key tile. `seek(g)` moves forward to the item
+// holding tile g.
+template <int RT>
 struct Cursor {
   int i, h, rt;
   int64_t begin, end;  // the item's tiles
   int item;            // its number over the launch
-  Request r;
+  Rows x;
 
   KD_DEVICE void load(const Args& a) {
     while (i < a.n) {
-      r = request(a, i);
-      if (r.nrt > 0 && r.tiles > 0) break;
-      item += r.nrt * a.hkv;
+      x = rows_of<RT>(a, i);
+      if (x.nrt > 0 && x.r.tiles > 0) break;
+      item += x.nrt * a.hkv;
       ++i;
     }
-    end = begin + (i < a.n ? r.tiles : 0);
+    end = begin + (i < a.n ? x.r.tiles : 0);
   }
   KD_DEVICE void start(const Args& a, int req, int64_t before, int items_before) {
     i = req;
@@ -70,20 +91,39 @@ struct Cursor {
     load(a);
   }
   KD_DEVICE void seek(const Args& a, int64_t g) {
-    while (i < a.n && g >= end) {
+    if (i < a.n && g >= end && x.r.tiles > 0) {  // whole items of this request at once
+      const int64_t left = (int64_t)(a.hkv - h) * x.nrt - rt;  // items from this one to the request's last
+      const int64_t k = min(left - 1, quotient(g - begin, x.r.tiles));
+      const int64_t to = (int64_t)h * x.nrt + rt + k;
+      begin += k * x.r.tiles;
+      end = begin + x.r.tiles;
+      item += (int)k;
+      h = (int)quotient(to, x.nrt);
+      rt = (int)(to - (int64_t)h * x.nrt);
+    }
+    while (i < a.n && g >= end) {  // past the request
       begin = end;
       ++item;
-      if (++rt == r.nrt) {
+      if (++rt == x.nrt) {
         rt = 0;
         if (++h == a.hkv) {
           h = 0;
           ++i;
           load(a);
+          if (i < a.n && g >= end) seek_within(a, g);
           continue;
         }
       }
-      end = begin + r.tiles;
+      end = begin + x.r.tiles;
     }
+  }
+  KD_DEVICE void seek_within(const Args& a, int64_t g) {
+    const int64_t k = min((int64_t)a.hkv * x.nrt - 1, quotient(g - begin, x.r.tiles));
+    begin += k * x.r.tiles;
+    end = begin + x.r.tiles;
+    item += (int)k;
+    h = (int)quotient(k, x.nrt);
+    rt = (int)(k - (int64_t)h * x.nrt);
   }
 };
 
@@ -99,6 +139,12 @@ KD_DEVICE void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
                : "r"(addr)
                : "memory");
 }
+// The transpose of an 8 x 8 matrix of 16-bit elements held two a thread, row by row.
+KD_DEVICE uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 // d += a (16 x 16, row) * b (16 x 8, column), f16 operands, float32 sums.
 KD_DEVICE void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -108,9 +154,7 @@ KD_DEVICE void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-KD_DEVICE void group_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
+KD_DEVICE void consumers_sync(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
 
 // Shared-memory offset of 16-byte piece `c` of row `row` in a tile stored by TMA with BOX-byte rows and BOX-byte
 // swizzling, chunk by chunk of BOX bytes.
@@ -125,112 +169,109 @@ KD_DEVICE uint32_t piece(int row, int c) {
 
 // One tile's meta data beside its ring slot.
 struct TileInfo {
-  float k_scale;
-  int v_exp;
+  float k_scale, v_exp;
   int live;  // 0: the block is absent (a table entry outside the pool): its keys are not seen
   int pad;
 };
 
-template <int HD>
-__global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
+template <int HD, int NT>
+__global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
     few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Args a) {
-  using C = Cfg<HD>;
-  constexpr int KG = C::KG, SL = C::SL, ST = C::STAGES, DV = C::DV;
+  using C = Cfg<HD, NT>;
+  constexpr int SLOTS = C::SLOTS, RT = C::RT, MT = C::MT;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* s_q = smem + KG * ST * C::STAGE_BYTES;  // [KG][Q_BYTES]
-  __shared__ uint64_t full[KG * ST], empty[KG * ST];
-  __shared__ TileInfo info[KG * ST];
-  __shared__ int64_t s_warp_tiles[C::WARPS + 1];
-  __shared__ int s_warp_items[C::WARPS + 1];
-  __shared__ int64_t s_lo, s_hi, s_before;
-  __shared__ int s_req, s_items_before;
+  uint8_t* s_q = smem + SLOTS * C::SLOT_BYTES;  // [2][Q_BYTES]
+  __shared__ uint64_t full[SLOTS], empty[SLOTS];
+  __shared__ TileInfo info[SLOTS];
+  __shared__ float s_qscale[2][RT];
+  __shared__ int64_t s_warp_tiles[C::THREADS / 32], s_before;
+  __shared__ int s_warp_items[C::THREADS / 32], s_req, s_items_before;
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
   if (tid == 0) {
-    for (int s = 0; s < KG * ST; ++s) {
+    for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], SL);
+      mbar_init(&empty[s], C::KW);
     }
     fence_barrier_init();
   }
-  // ---- this CTA's share of the tiles: a scan of the requests' tiles (twice: the total first, then the start)
-  int64_t total = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    const int64_t lo = pass ? total * blockIdx.x / shares(total, gridDim.x) : 0;
-    int64_t carry = 0;
-    int carry_items = 0;
-    for (int i0 = 0; i0 < a.n; i0 += C::THREADS) {
-      const int i = i0 + tid;
-      int64_t w = 0;
-      int items = 0;
-      if (i < a.n) {
-        const Request r = request(a, i);
-        w = (int64_t)r.nrt * r.tiles;
-        items = r.nrt;
-      }
-      int64_t x = w;
-      int y = items;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t px = __shfl_up_sync(0xffffffffu, x, o);
-        const int py = __shfl_up_sync(0xffffffffu, y, o);
-        if (lane >= o) {
-          x += px;
-          y += py;
-        }
-      }
-      if (lane == 31) {
-        s_warp_tiles[warp] = x;
-        s_warp_items[warp] = y;
-      }
-      __syncthreads();
-      int64_t before = carry, chunk = 0;
-      int items_before = carry_items, chunk_items = 0;
-#pragma unroll
-      for (int v = 0; v <= C::WARPS; ++v) {
-        if (v < warp) {
-          before += s_warp_tiles[v];
-          items_before += s_warp_items[v];
-        }
-        chunk += s_warp_tiles[v];
-        chunk_items += s_warp_items[v];
-      }
-      before += x - w;
-      items_before += y - items;
-      if (pass && i < a.n) {
-        if (blockIdx.x == 0) {  // for the launch that joins the partials
-          a.tile_cu[i] = before;
-          a.item_cu[i] = items_before;
-        }
-        if (w > 0 && lo >= before * a.hkv && lo < (before + w) * a.hkv) {
-          s_req = i;
-          s_before = before * a.hkv;
-          s_items_before = items_before * a.hkv;
-        }
-      }
-      carry += chunk;
-      carry_items += chunk_items;
-      __syncthreads();
+  // ---- this CTA's share of the tiles: a scan of the requests' tiles for the total, then (a second scan if the requests
+  // outnumber the threads) for the share's first request
+  int64_t w_mine = 0, w_before = 0, tiles = 0;
+  int items_mine = 0, items_before = 0, items = 0;
+  auto scan = [&](int i0, int64_t carry, int carry_items) {
+    const int i = i0 + tid;
+    w_mine = 0;
+    items_mine = 0;
+    if (i < a.n) {
+      const Rows r = rows_of<RT>(a, i);
+      w_mine = (int64_t)r.nrt * r.r.tiles;
+      items_mine = r.nrt;
     }
-    total = carry * a.hkv;
-    if (pass && tid == 0) {
-      s_lo = lo;
-      s_hi = blockIdx.x < shares(total, gridDim.x) ? total * (blockIdx.x + 1) / shares(total, gridDim.x) : 0;
-      if (blockIdx.x == 0) {
-        a.tile_cu[a.n] = carry;
-        a.item_cu[a.n] = carry_items;
+    int64_t x = w_mine;
+    int y = items_mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t px = __shfl_up_sync(0xffffffffu, x, o);
+      const int py = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) {
+        x += px;
+        y += py;
       }
+    }
+    if (lane == 31) {
+      s_warp_tiles[warp] = x;
+      s_warp_items[warp] = y;
+    }
+    __syncthreads();
+    w_before = carry + x - w_mine;
+    items_before = carry_items + y - items_mine;
+#pragma unroll
+    for (int v = 0; v < C::THREADS / 32; ++v) {
+      if (v < warp) {
+        w_before += s_warp_tiles[v];
+        items_before += s_warp_items[v];
+      }
+      carry += s_warp_tiles[v];
+      carry_items += s_warp_items[v];
+    }
+    __syncthreads();
+    tiles = carry;
+    items = carry_items;
+  };
+  for (int i0 = 0; i0 < a.n; i0 += C::THREADS) scan(i0, tiles, items);
+  const int64_t total = tiles * a.hkv;
+  const int np = (int)shares(total, gridDim.x);
+  const int64_t lo = quotient(total * blockIdx.x, np);
+  const int64_t hi = (int)blockIdx.x < np ? quotient(total * (blockIdx.x + 1), np) : 0;
+  if (a.n > C::THREADS) tiles = items = 0;
+  for (int i0 = 0; i0 < a.n; i0 += C::THREADS) {
+    if (a.n > C::THREADS) scan(i0, tiles, items);
+    const int i = i0 + tid;
+    if (i < a.n && blockIdx.x == 0) {  // for the launch that joins the partials
+      a.tile_cu[i] = w_before;
+      a.item_cu[i] = items_before;
+    }
+    if (w_mine > 0 && lo >= w_before * a.hkv && lo < (w_before + w_mine) * a.hkv) {
+      s_req = i;
+      s_before = w_before * a.hkv;
+      s_items_before = items_before * a.hkv;
     }
   }
+  if (tid == 0 && blockIdx.x == 0) {
+    a.tile_cu[a.n] = tiles;
+    a.item_cu[a.n] = items;
+  }
   __syncthreads();
-  const int64_t lo = s_lo, hi = s_hi;
   if (lo >= hi) return;
 
-  if (warp == C::WARPS) {
-    // ------------------------------------------------------------ producer
-    Cursor c;
+  Cursor<RT> c;
+  if (warp >= C::WARPS) {
+    set_registers_down<56>();
+    if (warp > C::WARPS) return;
     c.start(a, s_req, s_before, s_items_before);
+    // ------------------------------------------------------------ producer
     if (lane == 0) {
       tma_prefetch_desc(&map_k);
       tma_prefetch_desc(&map_v);
@@ -245,7 +286,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
       e = 0;
       if (g < hi) {
         c.seek(a, g);
-        const int id = a.table[(int64_t)c.i * a.ldt + c.r.first + (int)(g - c.begin)];
+        const int id = a.table[(int64_t)c.i * a.ldt + c.x.r.first + (int)(g - c.begin)];
         if (id >= 0 && id < a.blocks) {
           zz = id * a.hkv + c.h;
           s = a.k_scale[zz];
@@ -261,27 +302,24 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
       look_up(g0 + 32 + lane, next_z, next_ks, next_ve);
       const int m = (int)min((int64_t)32, hi - g0);
       for (int j = 0; j < m; ++j) {
-        const int64_t at = g0 + j - lo;
+        const uint32_t at = (uint32_t)(g0 - lo) + j, slot = at % SLOTS;
         const int zz = __shfl_sync(0xffffffffu, z, j);
         const float s = __shfl_sync(0xffffffffu, ks, j);
         const int e = __shfl_sync(0xffffffffu, ve, j);
-        const int kg = (int)(at % KG);
-        const int64_t use = at / KG;  // the group's tiles before this one
-        const int st = kg * ST + (int)(use % ST);
         bool ok = true;
         if (lane == 0) {
-          ok = mbar_wait(&empty[st], (uint32_t)((use / ST) & 1) ^ 1, a.status);
+          ok = mbar_wait(&empty[slot], ((at / SLOTS) & 1) ^ 1, a.status);
           if (ok) {
-            info[st] = TileInfo{s, e, zz >= 0, 0};
+            info[slot] = TileInfo{s, (float)e, zz >= 0, 0};
             if (zz >= 0) {
-              mbar_arrive_expect_tx(&full[st], C::STAGE_BYTES);
-              uint8_t* dst = smem + st * C::STAGE_BYTES;
+              mbar_arrive_expect_tx(&full[slot], C::SLOT_BYTES);
+              uint8_t* dst = smem + slot * C::SLOT_BYTES;
               for (int x = 0; x < C::CHUNKS; ++x) {
-                tma_load_3d(&map_k, &full[st], dst + x * BN * C::BOX, x * C::BOX, 0, zz);
-                tma_load_3d(&map_v, &full[st], dst + C::TILE_BYTES + x * BN * C::BOX, x * C::BOX, 0, zz);
+                tma_load_3d(&map_k, &full[slot], dst + x * BN * C::BOX, x * C::BOX, 0, zz);
+                tma_load_3d(&map_v, &full[slot], dst + C::TILE_BYTES + x * BN * C::BOX, x * C::BOX, 0, zz);
               }
             } else {
-              mbar_arrive(&full[st]);
+              mbar_arrive(&full[slot]);
             }
           }
         }
@@ -294,14 +332,13 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
     return;
   drain:
     // A consumer gave up: wait (bounded) for the copies in flight before the shared memory goes away. Tiles before
-    // `failed` were issued; slot (kg, st) last took its group's tile u.
+    // `failed` were issued; slot s last took tile u.
     if (lane == 0) {
       const uint64_t start = globaltimer();
-      for (int s = 0; s < KG * ST; ++s) {
-        const int64_t issued = (failed - s / ST + KG - 1) / KG;
-        const int64_t u = issued - 1 - ((issued - 1 - s % ST) % ST + ST) % ST;
+      for (int s = 0; s < SLOTS; ++s) {
+        const int64_t u = failed - 1 - ((failed - 1 - s) % SLOTS + SLOTS) % SLOTS;
         if (u < 0) continue;
-        while (!mbar_try_wait(smem_u32(&full[s]), (uint32_t)((u / ST) & 1)) && globaltimer() - start < 1000000000ull) {
+        while (!mbar_try_wait(smem_u32(&full[s]), (uint32_t)((u / SLOTS) & 1)) && globaltimer() - start < 1000000000ull) {
         }
       }
     }
@@ -309,365 +346,450 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
   }
 
   // ------------------------------------------------------------ consumers
-  const int kg = warp / SL, slice = warp % SL;
-  const int row_a = lane >> 2, t4 = lane & 3;  // this thread's rows are row_a and row_a + 8 of the 16-row tile
-  uint4* qf = reinterpret_cast<uint4*>(s_q + kg * C::Q_BYTES);
-  const uint32_t ring = smem_u32(smem) + kg * ST * C::STAGE_BYTES;
-  Cursor c;
+  set_registers_up<224>();
   c.start(a, s_req, s_before, s_items_before);
+  const int team = warp / C::KW, part_of = warp % C::KW;
+  const int row_g = lane >> 2, t4 = lane & 3;  // fragments: row_g a key or dim (and key + 8), 2 t4 and 2 t4 + 1 query rows
+  const uint32_t ring = smem_u32(smem);
   c.seek(a, lo);
-  int64_t use = 0;    // the group's tiles so far
-  bool dead = false;  // a wait gave up: walk on to the end without computing, so that no warp waits at a barrier alone
-  for (int64_t g = lo; g < hi;) {
+  uint32_t at = team;  // the team's next tile, counted from the CTA's first
+  bool dead = false;   // a wait gave up: walk on to the end without computing, so that no warp waits at a barrier alone
+  int buf = 0;
+  for (int64_t g = lo; g < hi; buf ^= 1) {
     const int64_t stop = min(c.end, hi);  // the fragment of this item: tiles [g, stop)
-    const int rows = min(RT, c.r.lq * a.group - c.rt * RT);
-    // ---- queries: f16, scaled to the row's largest magnitude, in the order of the A fragments
-    float q_scale[2];
-    const __nv_bfloat16* qp[2];
+    const int lq = c.x.r.lq, lk = c.x.r.lk;
+    const int rows = min(RT, lq * a.group - c.rt * RT);
+    // ---- queries: f16, scaled to the row's largest magnitude, in the order of the B fragments; a warp a row
+    uint2* qf = reinterpret_cast<uint2*>(s_q + buf * C::Q_BYTES);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int r = c.rt * RT + row_a + 8 * u;
-      const bool live = row_a + 8 * u < rows;
-      const int tok = live ? r / a.group : 0;
-      qp[u] = live ? a.q + (int64_t)(c.r.q0 + tok) * a.ldq + (c.h * a.group + r - tok * a.group) * HD + 4 * t4 : nullptr;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int rr = nt * 8 + warp, r = c.rt * RT + rr;
+      const int tok = r / a.group;
+      const bool live = rr < rows;
+      const __nv_bfloat16* src = a.q + (int64_t)(c.x.r.q0 + (live ? tok : 0)) * a.ldq +
+                                 (int64_t)(c.h * a.group + (live ? r - tok * a.group : 0)) * HD;
+      constexpr int UNITS = (HD + 127) / 128;  // 4 dims each
+      uint2 w[UNITS];
+      uint32_t top = 0;  // the largest finite magnitude as a bf16 pattern
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int d = (u * 32 + lane) * 4;
+        w[u] = live && d < HD ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
+        const uint32_t v[4] = {w[u].x & 0x7fffu, (w[u].x >> 16) & 0x7fffu, w[u].y & 0x7fffu, (w[u].y >> 16) & 0x7fffu};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, v[e] < 0x7f80u ? v[e] : 0u);
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      const int e = max((int)(top >> 7) - 127, -120);
+      const float inv = pow2i(-e);
+      if (lane == 0) s_qscale[buf][rr] = pow2i(e) * a.scale_log2;
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int d4 = u * 32 + lane;  // dims 4 d4 ..: step d4 / 4, thread d4 % 4 of the fragment
+        if (d4 * 4 < HD) {
+          const float2 p = unpack_bf16x2(w[u].x), q = unpack_bf16x2(w[u].y);
+          qf[((d4 >> 2) * NT + nt) * 32 + warp * 4 + (d4 & 3)] =
+              make_uint2(pack_f16x2(p.x * inv, p.y * inv), pack_f16x2(q.x * inv, q.y * inv));
+        }
+      }
     }
-    if (SL > 1) group_sync(1 + kg, SL * 32);  // the previous item's queries have been read
-    else __syncwarp();
-    {
-      uint32_t big[2] = {0, 0};  // the largest finite magnitude as a bf16 pattern
-#pragma unroll 4
+    consumers_sync(32 * C::WARPS);  // and every warp has left the item before the last, whose buffer this was
+    // the item's rows from the first to the last: which key tiles need a mask
+    const int pos0 = c.rt * RT / a.group + lk - lq;
+    const int pos1 = (c.rt * RT + rows - 1) / a.group + lk - lq;
+
+    float m[NT][2], big[NT][2], l[NT][2];  // running maxima (log2 units, possibly stale) of x and of x + e_v; row sums
+    float o[HD / 16][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = big[nt][0] = big[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
       for (int x = 0; x < HD / 16; ++x)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint2 w = qp[u] ? *reinterpret_cast<const uint2*>(qp[u] + 16 * x) : make_uint2(0, 0);
-          const uint32_t v[4] = {w.x & 0x7fffu, (w.x >> 16) & 0x7fffu, w.y & 0x7fffu, (w.y >> 16) & 0x7fffu};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) big[u] = max(big[u], v[e] < 0x7f80u ? v[e] : 0u);
-        }
-      float inv[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        big[u] = max(big[u], __shfl_xor_sync(0xffffffffu, big[u], 1));
-        big[u] = max(big[u], __shfl_xor_sync(0xffffffffu, big[u], 2));
-        const int e = max((int)(big[u] >> 7) - 127, -120);
-        q_scale[u] = pow2i(e);
-        inv[u] = pow2i(-e);
-      }
-#pragma unroll 4
-      for (int x = slice; x < HD / 16; x += SL) {
-        uint4 f;
-        const uint2 w0 = qp[0] ? *reinterpret_cast<const uint2*>(qp[0] + 16 * x) : make_uint2(0, 0);
-        const uint2 w1 = qp[1] ? *reinterpret_cast<const uint2*>(qp[1] + 16 * x) : make_uint2(0, 0);
-        float2 p = unpack_bf16x2(w0.x), r = unpack_bf16x2(w0.y);
-        f.x = pack_f16x2(p.x * inv[0], p.y * inv[0]);
-        f.z = pack_f16x2(r.x * inv[0], r.y * inv[0]);
-        p = unpack_bf16x2(w1.x);
-        r = unpack_bf16x2(w1.y);
-        f.y = pack_f16x2(p.x * inv[1], p.y * inv[1]);
-        f.w = pack_f16x2(r.x * inv[1], r.y * inv[1]);
-        qf[x * 32 + lane] = f;
-      }
+        for (int e = 0; e < 4; ++e) o[x][nt][e] = 0.f;
     }
-    if (SL > 1) group_sync(1 + kg, SL * 32);
-    else __syncwarp();
-    // the rows' visible keys
-    int key_lo[2], key_hi[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int r = c.rt * RT + row_a + 8 * u;
-      const int pos = r / a.group + c.r.lk - c.r.lq;
-      key_lo[u] = a.left >= 0 ? pos - a.left : 0;
-      key_hi[u] = a.right >= 0 ? min(c.r.lk - 1, pos + a.right) : c.r.lk - 1;
-    }
-    // the tile's rows from the first to the last: which key tiles need a mask
-    const int pos0 = c.rt * RT / a.group + c.r.lk - c.r.lq;
-    const int pos1 = (c.rt * RT + rows - 1) / a.group + c.r.lk - c.r.lq;
-
-    float m[2] = {-INFINITY, -INFINITY};  // running maximum of x (log2 units)
-    float big[2] = {-INFINITY, -INFINITY};  // running maximum of x + e_v
-    float l[2] = {0.f, 0.f};
-    float o[DV / 8][4];
-#pragma unroll
-    for (int d = 0; d < DV / 8; ++d)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
-
-    for (int64_t t = g + ((kg - (g - lo)) % KG + KG) % KG; t < stop; t += KG, ++use) {
-      const int st = (int)(use % ST);
-      dead = dead || !mbar_wait(&full[kg * ST + st], (uint32_t)((use / ST) & 1), a.status);
+    bool met = false;
+    for (; (int64_t)at + lo < stop; at += C::TEAMS) {
+      const uint32_t slot = at % SLOTS;
+      // A team may be a lap ahead of the team that takes the slot's tile before this one, and a parity cannot tell the
+      // phase before from the one after: that tile's release first, then this one's arrival.
+      const uint32_t lap = at / SLOTS;
+      dead = dead || (lap > 0 && !mbar_wait(&empty[slot], (lap - 1) & 1, a.status)) ||
+             !mbar_wait(&full[slot], lap & 1, a.status);
       if (__any_sync(0xffffffffu, dead)) {
         dead = true;
         continue;
       }
-      const TileInfo ti = info[kg * ST + st];
-      const uint32_t sk = ring + st * C::STAGE_BYTES, sv = sk + C::TILE_BYTES;
-      if (ti.live) {
-        // ---- S = Q K^T: 8 n-tiles of 8 keys; thread (row_a, t4) holds keys 8 j + 2 t4, + 1 of its two rows
-        float s[8][4];
+      const TileInfo ti = info[slot];
+      const uint32_t sk = ring + slot * C::SLOT_BYTES, sv = sk + C::TILE_BYTES;
+      const int tile0 = (c.x.r.first + (int)((int64_t)at + lo - c.begin)) * BN;
+#pragma unroll 1
+      for (int part = 0; part < C::PARTS; ++part) {
+        const int key_off = part_of * (BN / C::KW) + part * (16 * MT);  // the step's first key within the tile
+        const int key0 = tile0 + key_off;
+        if (!ti.live || key0 >= lk) break;
+        met = true;
+        // ---- S^T = K Q^T: 16 keys a tile; a thread holds keys row_g and row_g + 8 of its rows 2 t4 and 2 t4 + 1
+        float s[MT][NT][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
+        auto keys = [&](int mt, uint32_t w0, uint32_t w1, const uint2 (&q2)[NT]) {
+          uint32_t af[4];
+          codes_to_f16(w0, af[0], af[2]);
+          codes_to_f16(w1, af[1], af[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(s[mt][nt], af, q2[nt].x, q2[nt].y);
+        };
+        if constexpr (MT >= 2) {
 #pragma unroll 8
-        for (int x = 0; x < HD / 16; ++x) {
-          const uint4 f = qf[x * 32 + lane];
-          const uint32_t af[4] = {f.x, f.y, f.z, f.w};
+          for (int x = 0; x < HD / 16; ++x) {
+            uint2 q2[NT];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+            for (int nt = 0; nt < NT; ++nt) q2[nt] = qf[(x * NT + nt) * 32 + lane];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt += 2) {
+              uint32_t w[4];
+              ldmatrix4(sk + piece<HD>(key_off + mt * 16 + lane, x), w);
+              keys(mt, w[0], w[1], q2);
+              keys(mt + 1, w[2], w[3], q2);
+            }
+          }
+        } else {
+#pragma unroll 8
+          for (int x = 0; x < HD / 16; x += 2) {
             uint32_t w[4];
-            ldmatrix4(sk + piece<HD>(half * 32 + lane, x), w);
+            ldmatrix4(sk + piece<HD>(key_off + (lane & 15), x + (lane >> 4)), w);
+            uint2 q2[NT];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              uint32_t b0, b1;
-              codes_to_f16(w[y], b0, b1);
-              mma_f16(s[half * 4 + y], af, b0, b1);
+            for (int nt = 0; nt < NT; ++nt) q2[nt] = qf[(x * NT + nt) * 32 + lane];
+            keys(0, w[0], w[1], q2);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) q2[nt] = qf[((x + 1) * NT + nt) * 32 + lane];
+            keys(0, w[2], w[3], q2);
+          }
+        }
+        const bool tail = key0 + 16 * MT > lk;  // places past the request's tokens hold anything
+        const bool edge = tail || (a.right >= 0 && key0 + 16 * MT - 1 > pos0 + a.right) ||
+                          (a.left >= 0 && key0 < pos1 - a.left);
+        // ---- softmax
+        float mt_new[NT][2];
+        bool need = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int rr = nt * 8 + 2 * t4 + u;
+            const float mul = score_factor(s_qscale[buf][rr], ti.k_scale);
+            int key_lo = 0, key_hi = 0;
+            if (edge) {
+              const int pos = (c.rt * RT + rr) / a.group + lk - lq;
+              key_lo = a.left >= 0 ? pos - a.left : 0;
+              key_hi = a.right >= 0 ? min(lk - 1, pos + a.right) : lk - 1;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float x = s[mt][nt][2 * e + u] * mul;
+                if (edge) {
+                  const int key = key0 + mt * 16 + 8 * e + row_g;
+                  x = key >= key_lo && key <= key_hi ? x : -INFINITY;
+                }
+                s[mt][nt][2 * e + u] = x;
+                mx = fmaxf(mx, x);
+              }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mt_new[nt][u] = mx;
+            need |= mx + ti.v_exp > big[nt][u] + THRESHOLD || mx > m[nt][u] + THRESHOLD;
+          }
+        if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float alpha[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const float mx = mt_new[nt][u], mv = mx + ti.v_exp;
+              if (mx > m[nt][u] + THRESHOLD) {
+                l[nt][u] *= fast_exp2(m[nt][u] - mx);
+                m[nt][u] = mx;
+              }
+              alpha[u] = 1.f;
+              if (mv > big[nt][u] + THRESHOLD) {
+                alpha[u] = fast_exp2(big[nt][u] - mv);
+                big[nt][u] = mv;
+              }
+            }
+#pragma unroll
+            for (int x = 0; x < HD / 16; ++x) {
+              o[x][nt][0] *= alpha[0];
+              o[x][nt][1] *= alpha[1];
+              o[x][nt][2] *= alpha[0];
+              o[x][nt][3] *= alpha[1];
             }
           }
         }
-        const int key0 = (c.r.first + (int)(t - c.begin)) * BN;
-        const bool tail = key0 + BN > c.r.lk;  // rows past the request's tokens hold anything
-        const bool edge = tail || (a.right >= 0 && key0 + BN - 1 > pos0 + a.right) || (a.left >= 0 && key0 < pos1 - a.left);
-        // ---- softmax: two rows, 16 keys each, over the quad's four threads
-        float factor[2], alpha_o[2];
+        uint32_t pb[MT][NT][2];  // P^T as B fragments
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float mul = score_factor(q_scale[u] * a.scale_log2, ti.k_scale);
-          float mx = -INFINITY;
+        for (int nt = 0; nt < NT; ++nt) {
+          float base[2], factor[2];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int u = 0; u < 2; ++u) {
+            base[u] = m[nt][u] == -INFINITY ? 0.f : m[nt][u];
+            const float vbase = big[nt][u] == -INFINITY ? 0.f : big[nt][u];
+            factor[u] = fast_exp2(fminf(base[u] - vbase + ti.v_exp + P_EXPONENT, 126.f));
+          }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float x = s[j][2 * u + e] * mul;
-              if (edge) {
-                const int key = key0 + 8 * j + 2 * t4 + e;
-                x = key >= key_lo[u] && key <= key_hi[u] ? x : -INFINITY;
-              }
-              s[j][2 * u + e] = x;
-              mx = fmaxf(mx, x);
+          for (int mt = 0; mt < MT; ++mt) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              p[e] = fast_exp2(s[mt][nt][e] - base[e & 1]);
+              l[nt][e & 1] += p[e];
+              p[e] *= factor[e & 1];
             }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float m_new = fmaxf(m[u], mx), big_new = fmaxf(big[u], mx + (float)ti.v_exp);
-          const float base = m_new == -INFINITY ? 0.f : m_new, vbase = big_new == -INFINITY ? 0.f : big_new;
-          const float alpha = fast_exp2(m[u] - base);  // 0 while nothing was seen
-          alpha_o[u] = fast_exp2(big[u] - vbase);
-          factor[u] = fast_exp2(fminf(base - vbase + (float)ti.v_exp, 110.f)) * P_SCALE;
-          m[u] = m_new;
-          big[u] = big_new;
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float p = fast_exp2(s[j][2 * u + e] - base);
-              sum += p;
-              s[j][2 * u + e] = p * factor[u];
-            }
-          l[u] = l[u] * alpha + sum;
+            pb[mt][nt][0] = transpose8(pack_f16x2(p[0], p[1]));
+            pb[mt][nt][1] = transpose8(pack_f16x2(p[2], p[3]));
+          }
         }
+        // ---- O^T += V^T P^T: 16 keys a step; a 16-dim piece gives the even dims (rows 0-7) and the odd ones (8-15)
 #pragma unroll
-        for (int d = 0; d < DV / 8; ++d) {
-          o[d][0] *= alpha_o[0];
-          o[d][1] *= alpha_o[0];
-          o[d][2] *= alpha_o[1];
-          o[d][3] *= alpha_o[1];
-        }
-        // ---- O += P V: 16 keys per step; two n-tiles per 16 value columns, the even and the odd ones
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const uint32_t pf[4] = {pack_f16x2(s[2 * kk][0], s[2 * kk][1]), pack_f16x2(s[2 * kk][2], s[2 * kk][3]),
-                                  pack_f16x2(s[2 * kk + 1][0], s[2 * kk + 1][1]),
-                                  pack_f16x2(s[2 * kk + 1][2], s[2 * kk + 1][3])};
-          // codes of keys past the request's last token are cleared: a probability of 0 times a NaN code is NaN
+        for (int mt = 0; mt < MT; ++mt) {
+          // codes of places past the request's last token are cleared: a probability of 0 times a NaN code is NaN
           uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
           if (tail) {
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              const int left_keys = c.r.lk - (key0 + kk * 16 + y * 8 + 2 * t4);
+              const int left_keys = lk - (key0 + mt * 16 + y * 8 + 2 * t4);
               keep[y] = left_keys >= 2 ? 0xffffffffu : left_keys == 1 ? 0x0000ffffu : 0u;
             }
           }
 #pragma unroll
-          for (int x = 0; x < DV / 32; ++x) {
-            uint32_t w[4];  // (keys 0-7, keys 8-15) of 16-column piece 2 x, then of 2 x + 1
-            ldmatrix4_trans(sv + piece<HD>(kk * 16 + (lane & 15), slice * (DV / 16) + 2 * x + (lane >> 4)), w);
+          for (int x = 0; x < HD / 16; x += 2) {
+            uint32_t w[4];  // (keys 0-7, keys 8-15) of piece x, then of x + 1
+            ldmatrix4_trans(sv + piece<HD>(key_off + mt * 16 + (lane & 15), x + (lane >> 4)), w);
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              uint32_t a0, a1, b0, b1;  // (even, odd columns) of keys 0-7 and of keys 8-15
-              codes_to_f16(__byte_perm(w[2 * y] & keep[0], 0, 0x3120), a0, a1);
-              codes_to_f16(__byte_perm(w[2 * y + 1] & keep[1], 0, 0x3120), b0, b1);
-              mma_f16(o[(2 * x + y) * 2], pf, a0, b0);
-              mma_f16(o[(2 * x + y) * 2 + 1], pf, a1, b1);
+              uint32_t af[4];
+              codes_to_f16(__byte_perm(w[2 * y] & keep[0], 0, 0x3120), af[0], af[1]);
+              codes_to_f16(__byte_perm(w[2 * y + 1] & keep[1], 0, 0x3120), af[2], af[3]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_f16(o[x + y][nt], af, pb[mt][nt][0], pb[mt][nt][1]);
             }
           }
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[kg * ST + st]);
+      if (lane == 0) mbar_arrive(&empty[slot]);
     }
-    // ---- the group's partial of this fragment: item + CTA number its place (both only grow along the list)
+    // ---- the warp's partial of this fragment: item + CTA number its place (both only grow along the list)
+    float* part = a.partials + ((int64_t)(c.item + (int)blockIdx.x) * C::WARPS + warp) * C::PARTIAL;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-    }
-    float* part = a.partials + ((int64_t)(c.item + (int)blockIdx.x) * KG + kg) * C::PARTIAL;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int r = row_a + 8 * u;
-      if (r < rows) {
-        if (slice == 0 && t4 == 0) {
-          float* st3 = part + RT * HD + 3 * r;
-          st3[0] = m[u];
-          st3[1] = big[u];
-          st3[2] = l[u];
-        }
-        if (big[u] != -INFINITY || l[u] != 0.f) {
+      for (int u = 0; u < 2; ++u) {
+        const int rr = nt * 8 + 2 * t4 + u;
+        float sum = l[nt][u];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (rr < rows) {
+          if (row_g == 0) {
+            float* st = part + RT * HD + 3 * rr;
+            st[0] = m[nt][u];
+            st[1] = big[nt][u];
+            st[2] = sum;
+          }
+          if (met) {
 #pragma unroll
-          for (int x = 0; x < DV / 16; ++x)
-            *reinterpret_cast<float4*>(part + r * HD + slice * DV + 16 * x + 4 * t4) =
-                make_float4(o[2 * x][2 * u], o[2 * x + 1][2 * u], o[2 * x][2 * u + 1], o[2 * x + 1][2 * u + 1]);
+            for (int x = 0; x < HD / 16; ++x)
+              *reinterpret_cast<float2*>(part + rr * HD + 16 * x + 2 * row_g) = make_float2(o[x][nt][u], o[x][nt][2 + u]);
+          }
         }
       }
-    }
     g = stop;
     c.seek(a, g);
   }
 }
 
-// Joins the partials of one row of one item: blockIdx.x the item, blockIdx.y its row. Every partial's (m, M, l) is
-// read twice and its O once; partials lie in the order of the keys, and so do the sums.
-template <int HD>
-__global__ void __launch_bounds__(128) join_kernel(Args a, int ctas) {
-  using C = Cfg<HD>;
-  constexpr int V = HD / 64 < 4 ? HD / 64 : 4;  // columns a thread holds at once
-  constexpr int LANES = HD / V < 128 ? HD / V : 128;
-  constexpr int GROUPS = 128 / LANES;           // partials taken at once
-  constexpr int PASSES = HD / (V * LANES);
-  const int item = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+// Joins the partials of one row of one item: blockIdx.x the item, blockIdx.y its row. Warp w takes what the CTAs' warps w
+// left, in key order, its lanes the partials' statistics all at once and then HD / 32 columns each; the eight sums are
+// added in order.
+template <int HD, int NT>
+__global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
+  using C = Cfg<HD, NT>;
+  constexpr int RT = C::RT, V = HD / 32;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the partials are there after this
+  const int item = blockIdx.x, row = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   if (item >= a.item_cu[a.n] * a.hkv) return;
-  int lo = 0, hi = a.n - 1;  // the request holding the item
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if ((int64_t)a.item_cu[mid] * a.hkv <= item)
-      lo = mid;
-    else
-      hi = mid - 1;
+  int lo = 0, count = a.n;  // the request holding the item: the last with item_cu * hkv <= item, 32 probes at a time
+  while (count > 1) {
+    const int step = (count + 31) / 32;
+    const bool at_most = (int64_t)a.item_cu[lo + min(lane * step, count - 1)] * a.hkv <= item;
+    const int hits = __popc(__ballot_sync(0xffffffffu, at_most));
+    const int next = min(max(hits - 1, 0) * step, count - 1);
+    count = min(step, count - next);
+    lo += next;
   }
-  const Request r = request(a, lo);
+  const Rows x = rows_of<RT>(a, lo);
   const int local = item - a.item_cu[lo] * a.hkv;
-  const int h = local / r.nrt, rt = local - h * r.nrt;
+  const int h = local / x.nrt, rt = local - h * x.nrt;
   const int gr = rt * RT + row;
-  if (gr >= r.lq * a.group) return;
-  const int tok = gr / a.group;
-  const int head = h * a.group + gr - tok * a.group;
+  if (gr >= x.r.lq * a.group) return;
   const int64_t total = a.tile_cu[a.n] * a.hkv;
-  const int64_t begin = a.tile_cu[lo] * a.hkv + (int64_t)local * r.tiles, end = begin + r.tiles;
+  const int64_t begin = a.tile_cu[lo] * a.hkv + (int64_t)local * x.r.tiles, end = begin + x.r.tiles;
   // CTA c holds tiles [c total / P, (c + 1) total / P): the one holding tile g is ((g + 1) P - 1) / total
   const int64_t p = shares(total, ctas);
-  const int c0 = r.tiles ? (int)(((begin + 1) * p - 1) / total) : 0;
-  const int c1 = r.tiles ? (int)((end * p - 1) / total) : -1;
-  const int n = (c1 - c0 + 1) * C::KG;
-  const float* part = a.partials + (int64_t)(item + c0) * C::KG * C::PARTIAL;
-  __shared__ float s_red[3][4];
+  const int c0 = x.r.tiles ? (int)quotient((begin + 1) * p - 1, total) : 0;
+  const int n = x.r.tiles ? (int)quotient(end * p - 1, total) - c0 + 1 : 0;
+  const float* part = a.partials + ((int64_t)(item + c0) * C::WARPS + warp) * C::PARTIAL;
+  constexpr int64_t STEP = (int64_t)C::WARPS * C::PARTIAL;
+  __shared__ float s_red[2][8], s_l[8];
+  __shared__ __align__(16) float s_o[8][HD];
   float m = -INFINITY, big = -INFINITY;
-  for (int p = tid; p < n; p += 128) {
-    const float* st3 = part + (int64_t)p * C::PARTIAL + RT * HD + 3 * row;
-    m = fmaxf(m, st3[0]);
-    big = fmaxf(big, st3[1]);
+  for (int q = lane; q < n; q += 32) {
+    const float* st = part + q * STEP + RT * HD + 3 * row;
+    m = fmaxf(m, st[0]);
+    big = fmaxf(big, st[1]);
   }
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) {
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+  for (int o = 16; o > 0; o >>= 1) {
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
   }
-  if ((tid & 31) == 0) {
-    s_red[0][tid / 32] = m;
-    s_red[1][tid / 32] = big;
+  if (lane == 0) {
+    s_red[0][warp] = m;
+    s_red[1][warp] = big;
   }
   __syncthreads();
-  m = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
-  big = fmaxf(fmaxf(s_red[1][0], s_red[1][1]), fmaxf(s_red[1][2], s_red[1][3]));
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    m = fmaxf(m, s_red[0][w]);
+    big = fmaxf(big, s_red[1][w]);
+  }
   const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
-  float l = 0.f;
-  for (int p = tid; p < n; p += 128) {
-    const float* st3 = part + (int64_t)p * C::PARTIAL + RT * HD + 3 * row;
-    l += st3[2] * fast_exp2(st3[0] - base);
+  float l = 0.f, acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+  for (int q0 = 0; q0 < n; q0 += 32) {
+    float f = -1.f;  // < 0: the warp met no key there (its sums may hold anything)
+    if (q0 + lane < n) {
+      const float* st = part + (q0 + lane) * STEP + RT * HD + 3 * row;
+      l += st[2] * fast_exp2(st[0] - base);
+      if (st[1] != -INFINITY || st[2] != 0.f) f = fast_exp2(st[1] - vbase);
+    }
+    const int some = min(32, n - q0);
+    constexpr int BATCH = V <= 4 ? 8 : 4;
+    for (int q1 = 0; q1 < some; q1 += BATCH) {
+      float y[BATCH][V], w[BATCH];
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q) {
+        w[q] = __shfl_sync(0xffffffffu, f, (q1 + q) & 31);
+        if (q1 + q >= some) w[q] = -1.f;
+        const float* src = part + (q0 + q1 + q) * STEP + row * HD;
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[q][e] = 0.f;
+        if (!(w[q] < 0.f)) {
+          if constexpr (V == 2) {
+            const float2 t = *reinterpret_cast<const float2*>(src + lane * 2);
+            y[q][0] = t.x;
+            y[q][1] = t.y;
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+              const float4 t = *reinterpret_cast<const float4*>(src + e * 32 + lane * 4);
+              y[q][e] = t.x;
+              y[q][e + 1] = t.y;
+              y[q][e + 2] = t.z;
+              y[q][e + 3] = t.w;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += y[q][e] * (w[q] < 0.f ? 0.f : w[q]);
+    }
   }
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-  if ((tid & 31) == 0) s_red[2][tid / 32] = l;
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if (lane == 0) s_l[warp] = l;
+  if constexpr (V == 2) {
+    *reinterpret_cast<float2*>(&s_o[warp][lane * 2]) = make_float2(acc[0], acc[1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; e += 4)
+      *reinterpret_cast<float4*>(&s_o[warp][e * 32 + lane * 4]) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+  }
   __syncthreads();
-  l = (s_red[2][0] + s_red[2][1]) + (s_red[2][2] + s_red[2][3]);
-  // o = O 2^(M - m) / (2^15 l); without a visible key 0
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) l += s_l[w];
+  // o = O 2^(M - m) / (2^11 l); without a visible key 0
   const float fin = l == 0.f ? 0.f : fast_exp2(fminf(vbase - base, 126.f)) / (l * P_SCALE);
-  __shared__ float s_o[GROUPS > 1 ? 128 * V : 1];
-  const int grp = tid / LANES, col = (tid % LANES) * V;
-  const int64_t orow = (int64_t)(r.q0 + tok) * a.ldo + (int64_t)head * HD;
-  const int64_t grow = (int64_t)(r.q0 + tok) * a.ldg + (int64_t)head * HD;
+  const int tok = gr / a.group, head = h * a.group + gr - tok * a.group;
+  const int64_t orow = (int64_t)(x.r.q0 + tok) * a.ldo + (int64_t)head * HD;
+  const int64_t grow = (int64_t)(x.r.q0 + tok) * a.ldg + (int64_t)head * HD;
+  for (int d = threadIdx.x; d < HD / 2; d += 256) {
+    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int pass = 0; pass < PASSES; ++pass) {
-    const int cc = col + pass * V * LANES;
-    float acc[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = 0.f;
-    for (int p = grp; p < n; p += GROUPS) {
-      const float* pp = part + (int64_t)p * C::PARTIAL;
-      const float st_big = pp[RT * HD + 3 * row + 1];
-      if (st_big == -INFINITY && pp[RT * HD + 3 * row + 2] == 0.f) continue;  // this group met no key of the row
-      const float w = fast_exp2(st_big - vbase);
-#pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] += w * pp[row * HD + cc + e];
+    for (int w = 0; w < 8; ++w) {
+      const float2 y = *reinterpret_cast<const float2*>(&s_o[w][2 * d]);
+      sum.x += y.x;
+      sum.y += y.y;
     }
-    if constexpr (GROUPS > 1) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) s_o[tid * V + e] = acc[e];
-      __syncthreads();
-      if (grp == 0) {
-#pragma unroll
-        for (int gq = 1; gq < GROUPS; ++gq)
-#pragma unroll
-          for (int e = 0; e < V; ++e) acc[e] += s_o[(gq * LANES + tid) * V + e];
-      }
+    float2 y = l == 0.f ? make_float2(0.f, 0.f) : make_float2(sum.x * fin, sum.y * fin);
+    if (a.gate && l != 0.f) {
+      const float2 s = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(a.gate + grow + 2 * d));
+      y.x = x_sigmoid(y.x, s.x);
+      y.y = x_sigmoid(y.y, s.y);
     }
-    if (grp == 0) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float x = l == 0.f ? 0.f : acc[e] * fin;
-        if (a.gate && l != 0.f) x *= sigmoid(__bfloat162float(a.gate[grow + cc + e]));
-        a.out[orow + cc + e] = __float2bfloat16_rn(x);
-      }
-    }
+    *reinterpret_cast<uint32_t*>(a.out + orow + 2 * d) = pack_bf16x2(y.x, y.y);
   }
 }
 
-// Whether the requests' rows per key/value head fit one 16-row tile: the kernel of this file. Both kernels are right for
-// any rows.
-static bool few_rows(int max_q, int group) { return (int64_t)max_q * group <= RT; }
-
-// Bytes of scratch: the two request arrays, then one partial per (item + CTA, key group).
-template <int HD>
-int64_t few_rows_items(int n, int64_t total_q, int hkv, int group) {
-  return ((total_q * group + RT - 1) / RT + n) * hkv;
+// Whether the requests' rows per key/value head fit the row tile of this file's kernel. Both kernels are right for any
+// rows.
+static int row_tiles_of_8(int max_q, int group, int head_dim) {
+  const int64_t rows = (int64_t)max_q * group;
+  if (rows <= 8) return 1;
+  if (rows <= 16 && head_dim <= 256) return 2;
+  if (rows <= 32 && head_dim <= 128) return 4;
+  return 0;
 }
-int64_t header_bytes(int n) { return ((int64_t)(n + 1) * 12 + 15) / 16 * 16 + 16; }
 
-template <int HD>
+// Bytes of scratch: the two request arrays, then the warps' partials per (item + CTA).
+static int64_t header_bytes(int n) { return ((int64_t)(n + 1) * 12 + 15) / 16 * 16; }
+
+template <int HD, int NT>
+int64_t items_bound(int n, int64_t total_q, int hkv, int group) {
+  return (total_q * group / Cfg<HD, NT>::RT + n) * hkv;
+}
+template <int HD, int NT>
 int64_t workspace_bytes(int n, int64_t total_q, int hkv, int group, int ctas) {
+  using C = Cfg<HD, NT>;
   return header_bytes(n) +
-         (few_rows_items<HD>(n, total_q, hkv, group) + ctas) * Cfg<HD>::KG * Cfg<HD>::PARTIAL * (int64_t)sizeof(float);
+         (items_bound<HD, NT>(n, total_q, hkv, group) + ctas) * C::WARPS * C::PARTIAL * (int64_t)sizeof(float);
 }
 
-template <int HD>
+template <int HD, int NT>
 int launch(Args a, const void* k_codes, const void* v_codes, uint8_t* ws, int64_t ws_bytes, cudaStream_t stream) {
-  using C = Cfg<HD>;
+  using C = Cfg<HD, NT>;
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return set_error(KD_ERR_ARGUMENT, "attention_cache: device index");
   const int ctas = num_sms(dev);
-  const int64_t items = few_rows_items<HD>(a.n, a.total_q, a.hkv, a.group);
+  const int64_t items = items_bound<HD, NT>(a.n, a.total_q, a.hkv, a.group);
   if (items > 0x7fffffff - 4096) return set_error(KD_ERR_ARGUMENT, "attention_cache: too many row tiles");
-  if (ws_bytes < workspace_bytes<HD>(a.n, a.total_q, a.hkv, a.group, ctas))
+  if (ws_bytes < workspace_bytes<HD, NT>(a.n, a.total_q, a.hkv, a.group, ctas))
     return set_error(KD_ERR_ARGUMENT, "attention_cache: workspace smaller than kd_attention_cache_workspace");
   a.tile_cu = reinterpret_cast<int64_t*>(ws);
   a.item_cu = reinterpret_cast<int32_t*>(ws + 8 * (int64_t)(a.n + 1));
@@ -680,7 +802,7 @@ int launch(Args a, const void* k_codes, const void* v_codes, uint8_t* ws, int64_
   if (!rc)
     rc = make_tma_3d(&mv, v_codes, dt, 1, HD, BN, (uint64_t)a.blocks * a.hkv, HD, (uint64_t)BN * HD, C::BOX, BN, 1, sw);
   if (rc) return rc;
-  auto kernel = few_rows_kernel<HD>;
+  auto kernel = few_rows_kernel<HD, NT>;
   static bool configured[64] = {false};
   if (!configured[dev]) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
@@ -690,8 +812,27 @@ int launch(Args a, const void* k_codes, const void* v_codes, uint8_t* ws, int64_
   kernel<<<ctas, C::THREADS, C::SMEM, stream>>>(mk, mv, a);
   rc = record_cuda_error(cudaGetLastError(), "attention_cache: launch");
   if (rc) return rc;
-  join_kernel<HD><<<dim3((unsigned)items, RT), 128, 0, stream>>>(a, ctas);
-  return record_cuda_error(cudaGetLastError(), "attention_cache: join launch");
+  return launch_after(join_kernel<HD, NT>, dim3((unsigned)items, C::RT), 256, stream, a, ctas);
+}
+
+// Calls f.template operator()<HD, NT>() for the kernel of a head dim and a number of 8-row tiles.
+template <typename F>
+auto with_kernel(int head_dim, int nt, F f) {
+  switch (head_dim) {
+    case 64:
+      return nt == 1 ? f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{})
+             : nt == 2 ? f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{})
+                       : f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+    case 128:
+      return nt == 1 ? f(std::integral_constant<int, 128>{}, std::integral_constant<int, 1>{})
+             : nt == 2 ? f(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{})
+                       : f(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{});
+    case 256:
+      return nt == 1 ? f(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{})
+                     : f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    default:
+      return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 1>{});
+  }
 }
 
 }  // namespace ca
@@ -709,16 +850,11 @@ extern "C" int kd_attention_cache_workspace(int num_requests, int max_q, int64_t
   int dev = 0;
   if (int rc = record_cuda_error(cudaGetDevice(&dev), "attention_cache_workspace: device")) return rc;
   const int sms = num_sms(dev), group = num_heads_q / num_heads_kv;
-  if (!ca::few_rows(max_q, group)) {
-    *bytes = ca::row_tiles_workspace(head_dim, sms);
-    return KD_OK;
-  }
-  switch (head_dim) {
-    case 64: *bytes = ca::workspace_bytes<64>(num_requests, total_q, num_heads_kv, group, sms); break;
-    case 128: *bytes = ca::workspace_bytes<128>(num_requests, total_q, num_heads_kv, group, sms); break;
-    case 256: *bytes = ca::workspace_bytes<256>(num_requests, total_q, num_heads_kv, group, sms); break;
-    default: *bytes = ca::workspace_bytes<512>(num_requests, total_q, num_heads_kv, group, sms); break;
-  }
+  const int nt = ca::row_tiles_of_8(max_q, group, head_dim);
+  *bytes = nt == 0 ? ca::row_tiles_workspace(head_dim, sms)
+                   : ca::with_kernel(head_dim, nt, [&](auto hd, auto t) {
+                       return ca::workspace_bytes<hd(), t()>(num_requests, total_q, num_heads_kv, group, sms);
+                     });
   return KD_OK;
 }
 
@@ -780,11 +916,9 @@ extern "C" int kd_attention_cache(const void* q, int64_t ldq, const void* k_code
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512)
     return set_error(KD_ERR_ARGUMENT, "attention_cache: head_dim must be 64, 128, 256 or 512");
-  if (!ca::few_rows(max_q, a.group)) return ca::row_tiles(head_dim, a, k_codes, v_codes, ws, workspace_bytes, stream);
-  switch (head_dim) {
-    case 64: return ca::launch<64>(a, k_codes, v_codes, ws, workspace_bytes, stream);
-    case 128: return ca::launch<128>(a, k_codes, v_codes, ws, workspace_bytes, stream);
-    case 256: return ca::launch<256>(a, k_codes, v_codes, ws, workspace_bytes, stream);
-    default: return ca::launch<512>(a, k_codes, v_codes, ws, workspace_bytes, stream);
-  }
+  const int nt = ca::row_tiles_of_8(max_q, a.group, head_dim);
+  if (nt == 0) return ca::row_tiles(head_dim, a, k_codes, v_codes, ws, workspace_bytes, stream);
+  return ca::with_kernel(head_dim, nt, [&](auto hd, auto t) {
+    return ca::launch<hd(), t()>(a, k_codes, v_codes, ws, workspace_bytes, stream);
+  });
 }

@@ -4,6 +4,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kd_internal.h"
 
@@ -11,7 +13,6 @@ namespace kd {
 namespace ca {
 
 constexpr int BN = KD_KV_BLOCK;  // keys per tile: one block
-constexpr int RT = 16;           // query rows per tile of the kernel for few rows
 
 struct Args {
   const __nv_bfloat16* q;
@@ -31,8 +32,8 @@ struct Args {
   int hq, hkv, group;
   float scale_log2;
   int left, right;
-  int64_t* tile_cu;   // [n + 1] few rows: key tiles of the requests before (of one key/value head); many: their weights
-  int32_t* item_cu;   // [n + 1] few rows: 16-row tiles of the requests before
+  int64_t* tile_cu;   // [n + 1] few rows: key tiles of the requests before (of one key/value head)
+  int32_t* item_cu;   // [n + 1] few rows: row tiles of the requests before
   void* splits;       // many rows: an item begun by a CTA and finished by later ones, per CTA
   float* partials;
   int* status;
@@ -40,8 +41,7 @@ struct Args {
 
 struct Request {
   int q0, lq, lk;
-  int nrt;          // 16-row tiles
-  int first, tiles; // key tiles that any row may see
+  int first, tiles;  // key tiles that any row may see
 };
 
 KD_DEVICE Request request(const Args& a, int i) {
@@ -50,11 +50,16 @@ KD_DEVICE Request request(const Args& a, int i) {
   const int end = a.cu[i + 1];
   r.lq = r.q0 < 0 || end > a.total_q ? 0 : max(end - r.q0, 0);
   r.lk = (int)min((int64_t)max(a.kv_len[i], 0), (int64_t)a.width * BN);
-  r.nrt = (int)(((int64_t)r.lq * a.group + RT - 1) / RT);
   const int kmin = a.left >= 0 ? max(0, r.lk - r.lq - a.left) : 0;
   r.first = kmin / BN;
   r.tiles = r.lq > 0 && r.lk > kmin ? (r.lk - 1) / BN - r.first + 1 : 0;
   return r;
+}
+
+// Quotients of non-negative numbers: in 32 bits where both fit (a 64-bit division costs some 600 cycles here, and the
+// first key tile waits for several).
+KD_DEVICE int64_t quotient(int64_t a, int64_t b) {
+  return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
 // CTAs that take part: every one of them has a tile, so no partial of an item is missing.
@@ -95,6 +100,16 @@ KD_DEVICE float score_factor(float row, float k_scale) {
 KD_DEVICE uint32_t pack_f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// A warpgroup's share of the block's registers (executed by all of it, one instruction).
+template <int N>
+KD_DEVICE void set_registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+KD_DEVICE void set_registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // Launches the joining kernel so that its blocks are in place when the kernel before it in the stream ends (it waits for

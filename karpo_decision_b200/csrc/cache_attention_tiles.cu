@@ -21,8 +21,6 @@
 //
 // Warps: 0-3 softmax and epilogue, a thread a row (they also split the item's query rows), 4 work fetch and the keys' TMA
 // loads, 5 MMA issue, 6.. conversion of values.
-#include <type_traits>
-
 #include "cache_attention.cuh"
 
 namespace kd {
@@ -71,12 +69,6 @@ constexpr float THRESHOLD = 4.0f;   // log2 units a row's maximum may grow befor
 constexpr float P_EXPONENT = 11.f, P_SCALE = 2048.f;  // f16 probabilities hold p * 2^11: at most 2^15 with the threshold
 constexpr int ITEM_TILES = 4;       // an item's own cost (queries, epilogue) in key tiles
 constexpr int MIN_TILES = 6;        // the least share of a CTA in key tiles: less costs more to join than it saves
-
-// Quotients of non-negative numbers: in 32 bits where both fit (a 64-bit division costs some 600 cycles here, and the
-// first key tile waits for several).
-KD_DEVICE int64_t quotient(int64_t a, int64_t b) {
-  return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
-}
 
 // A request's row tiles and their weights w(j) = min(base + step j, cap) + own, in units of a key tile / group: the key
 // tiles that row tile j sees, about, up to the window's width.
@@ -256,15 +248,6 @@ KD_DEVICE void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
                "r"(r[2]), "r"(r[3])
                : "memory");
-}
-
-template <int N>
-KD_DEVICE void set_registers_up() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-KD_DEVICE void set_registers_down() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // What the softmax needs of a key tile.

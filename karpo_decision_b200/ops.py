@@ -6,7 +6,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -410,14 +409,25 @@ def gated_norm(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, heads: in
 # ------------------------------------------------------------------------------------------------ cache of states
 
 
-class KVBlocks(NamedTuple):
-    """One layer's pool of cached keys and values: e4m3 codes (blocks, Hkv, 64, hd) and float32 power-of-two scales
-    (blocks, Hkv); value = code * scale."""
+class KVBlocks:
+    """One layer's pool of cached keys and values: e4m3 codes ``k``, ``v`` (blocks, Hkv, 64, hd) and float32 power-of-two
+    scales ``k_scale``, ``v_scale`` (blocks, Hkv); value = code * scale. Checked here, once, for every call that takes
+    it."""
 
-    k: torch.Tensor
-    v: torch.Tensor
-    k_scale: torch.Tensor
-    v_scale: torch.Tensor
+    __slots__ = ("k", "v", "k_scale", "v_scale", "blocks", "heads", "head_dim", "index")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
+        _require(k.dim() == 4 and k.shape[2] == KV_BLOCK and k.shape == v.shape,
+                 "cache codes: (blocks, Hkv, 64, head_dim)")
+        _require(k.dtype == v.dtype == torch.float8_e4m3fn and k.is_contiguous() and v.is_contiguous(),
+                 "cache codes: contiguous e4m3")
+        _require(k_scale.shape == v_scale.shape == k.shape[:2] and k_scale.dtype == v_scale.dtype == torch.float32
+                 and k_scale.is_contiguous() and v_scale.is_contiguous(),
+                 "cache scales: contiguous float32 (blocks, Hkv)")
+        _require(k.device == v.device == k_scale.device == v_scale.device, "cache: on one device")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.blocks, self.heads, self.head_dim = k.shape[0], k.shape[1], k.shape[3]
+        self.index = k.get_device()  # -1: not on a GPU
 
 
 def kv_blocks(blocks: int, kv_heads: int, head_dim: int, device: torch.device) -> KVBlocks:
@@ -431,29 +441,36 @@ def kv_blocks(blocks: int, kv_heads: int, head_dim: int, device: torch.device) -
     return KVBlocks(codes(), codes(), scales(), scales())
 
 
-def _pool(cache: KVBlocks) -> tuple[int, int, int]:
-    """(blocks, Hkv, hd) of a well-formed pool."""
-    k, v, ks, vs = cache
-    _require(k.dim() == 4 and k.shape[2] == KV_BLOCK and k.shape == v.shape, "cache codes: (blocks, Hkv, 64, head_dim)")
-    _require(k.dtype == v.dtype == torch.float8_e4m3fn and k.is_contiguous() and v.is_contiguous(),
-             "cache codes: contiguous e4m3")
-    _require(ks.shape == vs.shape == k.shape[:2] and ks.dtype == vs.dtype == torch.float32 and ks.is_contiguous()
-             and vs.is_contiguous(), "cache scales: contiguous float32 (blocks, Hkv)")
-    _require(k.is_cuda and k.device == v.device == ks.device == vs.device, "cache: on one CUDA device")
-    return k.shape[0], k.shape[1], k.shape[3]
+def _call_on(index: int, name: str, *args) -> None:
+    """``call`` with the device current (the launch goes to it) and its current stream as the last argument."""
+    if torch._C._cuda_getDevice() == index:
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _int32s(t: torch.Tensor, n: int, name: str, device: torch.device) -> None:
-    _require(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n, f"{name}: {n} contiguous int32")
-    _require(t.device == device, f"{name}: on {device}")
+def _int32s(t: torch.Tensor, n: int, name: str, index: int) -> None:
+    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}: {n} contiguous int32")
+    if t.get_device() != index:
+        raise ValueError(f"{name}: on the same CUDA device as the others")
 
 
-def _block_table(table: torch.Tensor, n: int, device: torch.device) -> None:
-    _require(table.dim() == 2 and table.dtype == torch.int32 and (table.stride(1) == 1 or table.shape[1] <= 1),
-             "table: int32 (requests, width) with contiguous rows")
-    _require(table.shape[0] == n and (n <= 1 or table.stride(0) >= table.shape[1]),
-             f"table: {n} rows that do not overlap")
-    _require(table.device == device, f"table: on {device}")
+def _block_table(table: torch.Tensor, n: int, index: int) -> tuple[int, int]:
+    """(row stride, width) of int32 rows that do not overlap."""
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != n:
+        raise ValueError(f"table: int32 ({n}, width)")
+    ld, step = table.stride()
+    width = table.shape[1]
+    if (step != 1 and width > 1) or (ld < width and n > 1) or table.get_device() != index:
+        raise ValueError("table: contiguous rows that do not overlap, on the same CUDA device as the others")
+    return max(ld, width), width
+
+
+def _int64s(t: torch.Tensor, n: int, name: str, index: int) -> None:
+    if t.dtype != torch.int64 or t.numel() != n or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{name}: {n} contiguous int64 on the same CUDA device as the others")
 
 
 def kv_assign(lens: torch.Tensor, cu: torch.Tensor, table: torch.Tensor, free: torch.Tensor, count: torch.Tensor,
@@ -463,25 +480,25 @@ def kv_assign(lens: torch.Tensor, cu: torch.Tensor, table: torch.Tensor, free: t
     (n,), seqpos int64 (rows,), slots int64 (rows,)), or writes them to ``out`` (whose kv_len may be ``lens``). When
     blocks are missing nothing is taken, every slot is -1 and ``count[1]`` says how many (or KV_TABLE_FULL /
     KV_MALFORMED)."""
-    n, dev = lens.numel(), lens.device
-    _require(lens.is_cuda, "lens must be on a CUDA device")
-    _int32s(lens, n, "lens", dev)
-    _int32s(cu, n + 1, "cu", dev)
-    _block_table(table, n, dev)
-    _int32s(free, free.numel(), "free", dev)
-    _int32s(count, 2, "count", dev)
+    n, index = lens.numel(), lens.get_device()
+    _require(index >= 0, "lens must be on a CUDA device")
+    _int32s(lens, n, "lens", index)
+    _int32s(cu, n + 1, "cu", index)
+    ld, width = _block_table(table, n, index)
+    capacity = free.numel()
+    _int32s(free, capacity, "free", index)
+    _int32s(count, 2, "count", index)
     if out is None:
-        out = (torch.empty(n, dtype=torch.int32, device=dev), torch.empty(rows, dtype=torch.int64, device=dev),
-               torch.empty(rows, dtype=torch.int64, device=dev))
-    kv_len, seqpos, slots = out
-    _int32s(kv_len, n, "kv_len", dev)
-    _require(seqpos.dtype == slots.dtype == torch.int64 and seqpos.is_contiguous() and slots.is_contiguous()
-             and seqpos.numel() == slots.numel() == rows, "seqpos, slots: contiguous int64, one per row")
-    _require(seqpos.device == dev and slots.device == dev, f"seqpos, slots: on {dev}")
-    with torch.cuda.device(dev):
-        call("kd_kv_assign", lens.data_ptr(), cu.data_ptr(), n, rows, table.data_ptr(),
-             max(table.stride(0), table.shape[1]), table.shape[1], free.data_ptr(), free.numel(), count.data_ptr(),
-             kv_len.data_ptr(), seqpos.data_ptr(), slots.data_ptr(), _stream(lens))
+        both = lens.new_empty((2, rows), dtype=torch.int64)
+        out = (torch.empty_like(lens), both[0], both[1])
+        kv_len, seqpos, slots = out
+    else:
+        kv_len, seqpos, slots = out
+        _int32s(kv_len, n, "kv_len", index)
+        _int64s(seqpos, rows, "seqpos", index)
+        _int64s(slots, rows, "slots", index)
+    _call_on(index, "kd_kv_assign", lens.data_ptr(), cu.data_ptr(), n, rows, table.data_ptr(), ld, width,
+             free.data_ptr(), capacity, count.data_ptr(), kv_len.data_ptr(), seqpos.data_ptr(), slots.data_ptr())
     return out
 
 
@@ -489,50 +506,62 @@ def kv_release(table: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor, free
                ) -> None:
     """Gives the blocks past each request's first ``keep`` tokens (of ``lens``) back to the stack, undoing a
     ``kv_assign`` exactly; ``lens`` is not written. No two requests may share a block given back."""
-    n, dev = lens.numel(), lens.device
-    _require(lens.is_cuda, "lens must be on a CUDA device")
-    _int32s(lens, n, "lens", dev)
-    _int32s(keep, n, "keep", dev)
-    _block_table(table, n, dev)
-    _int32s(free, free.numel(), "free", dev)
-    _int32s(count, 2, "count", dev)
-    with torch.cuda.device(dev):
-        call("kd_kv_release", table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1], lens.data_ptr(),
-             keep.data_ptr(), n, free.data_ptr(), free.numel(), count.data_ptr(), _stream(lens))
+    n, index = lens.numel(), lens.get_device()
+    _require(index >= 0, "lens must be on a CUDA device")
+    _int32s(lens, n, "lens", index)
+    _int32s(keep, n, "keep", index)
+    ld, width = _block_table(table, n, index)
+    capacity = free.numel()
+    _int32s(free, capacity, "free", index)
+    _int32s(count, 2, "count", index)
+    _call_on(index, "kd_kv_release", table.data_ptr(), ld, width, lens.data_ptr(), keep.data_ptr(), n,
+             free.data_ptr(), capacity, count.data_ptr())
 
 
-def _head_rows(t: torch.Tensor, name: str, heads: int, head_dim: int) -> int:
+def _head_rows(t: torch.Tensor, name: str, heads: int, head_dim: int, index: int) -> int:
     """Row stride of (rows, heads, head_dim) bf16 with the heads packed within a row."""
-    _require(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == head_dim and t.dtype == torch.bfloat16,
-             f"{name}: bf16 (rows, {heads}, {head_dim})")
-    _require(t.stride(2) == 1 and (heads == 1 or t.stride(1) == head_dim), f"{name}: heads must be packed within a row")
-    return t.stride(0) if t.shape[0] > 1 else heads * head_dim
+    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
+        raise ValueError(f"{name}: bf16 (rows, {heads}, {head_dim})")
+    ld, head, step = t.stride()
+    if step != 1 or (head != head_dim and heads > 1):
+        raise ValueError(f"{name}: heads must be packed within a row")
+    if t.get_device() != index:
+        raise ValueError(f"{name}: on the cache's CUDA device")
+    return ld if t.shape[0] > 1 else heads * head_dim
 
 
 def kv_store_e4m3(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, slots: torch.Tensor, cache: KVBlocks) -> None:
     """Writes the rows' keys and values (T, Hkv, hd) into the blocks ``slots`` (from ``kv_assign``) names, quantized to
     e4m3 with a power-of-two scale per (block, head); a half-filled block's scale grows as its new rows need."""
-    blocks, heads, hd = _pool(cache)
-    dev = cache.k.device
-    ldk, ldv = _head_rows(k, "k", heads, hd), _head_rows(v, "v", heads, hd)
-    rows = k.shape[0]
-    _require(v.shape[0] == rows and k.device == dev and v.device == dev, "k, v: the same rows, on the cache's device")
-    _int32s(cu, cu.numel(), "cu", dev)
-    _require(cu.numel() >= 1, "cu: at least one bound")
-    _require(slots.dtype == torch.int64 and slots.is_contiguous() and slots.numel() == rows and slots.device == dev,
-             "slots: contiguous int64, one per row")
-    with torch.cuda.device(dev):
-        call("kd_kv_store_e4m3", k.data_ptr(), ldk, v.data_ptr(), ldv, rows, cu.data_ptr(), cu.numel() - 1,
+    index, heads, hd = cache.index, cache.heads, cache.head_dim
+    _require(index >= 0, "the cache must be on a CUDA device")
+    ldk, ldv = _head_rows(k, "k", heads, hd, index), _head_rows(v, "v", heads, hd, index)
+    rows, bounds = k.shape[0], cu.numel()
+    _require(v.shape[0] == rows, "k, v: the same rows")
+    _require(bounds >= 1, "cu: at least one bound")
+    _int32s(cu, bounds, "cu", index)
+    _int64s(slots, rows, "slots", index)
+    _call_on(index, "kd_kv_store_e4m3", k.data_ptr(), ldk, v.data_ptr(), ldv, rows, cu.data_ptr(), bounds - 1,
              slots.data_ptr(), heads, hd, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-             cache.v_scale.data_ptr(), blocks, _stream(k))
+             cache.v_scale.data_ptr(), cache.blocks)
 
 
 @functools.lru_cache(maxsize=4096)
-def _cache_workspace(device: int, n: int, max_q: int, rows: int, heads: int, kv_heads: int, head_dim: int) -> int:
-    """Bytes of scratch of an ``attention_cache`` launch (on the current device, ``device``)."""
+def _cache_workspace(index: int, n: int, max_q: int, rows: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of scratch of an ``attention_cache`` launch of these sizes on device ``index``."""
     size = ctypes.c_int64()
-    call("kd_attention_cache_workspace", n, max_q, rows, heads, kv_heads, head_dim, ctypes.addressof(size))
+    with torch.cuda.device(index):
+        call("kd_attention_cache_workspace", n, max_q, rows, heads, kv_heads, head_dim, ctypes.addressof(size))
     return size.value
+
+
+def _wide_rows(t: torch.Tensor, name: str, rows: int, width: int, index: int) -> int:
+    """Row stride of bf16 (rows, width)."""
+    if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width or t.stride(1) != 1:
+        raise ValueError(f"{name}: bf16 ({rows}, {width}) with contiguous rows")
+    if t.get_device() != index:
+        raise ValueError(f"{name}: on the cache's CUDA device")
+    return t.stride(0) if rows > 1 else width
 
 
 def attention_cache(q: torch.Tensor, cache: KVBlocks, table: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
@@ -541,33 +570,31 @@ def attention_cache(q: torch.Tensor, cache: KVBlocks, table: torch.Tensor, cu_q:
     """Attention of the new rows ``q`` (Tq, Hq, hd) over their requests' cached tokens (``kv_len`` of them, the new ones
     included, in the blocks ``table`` names), with ``attention_varlen``'s end-aligned window; returns (Tq, Hq * hd),
     gated by sigmoid(gate) when given. Rows of ``out`` outside every request are left as they were."""
-    blocks, hkv, hd = _pool(cache)
-    dev = cache.k.device
+    index, hkv, hd = cache.index, cache.heads, cache.head_dim
+    _require(index >= 0, "the cache must be on a CUDA device")
     _require(q.dim() == 3, "q: bf16 (rows, heads, head_dim)")
     tq, hq = q.shape[0], q.shape[1]
-    ldq = _head_rows(q, "q", hq, hd)
-    n = kv_len.numel()
-    _int32s(kv_len, n, "kv_len", dev)
-    _int32s(cu_q, n + 1, "cu_q", dev)
-    _block_table(table, n, dev)
-    _require(q.device == dev, f"q: on {dev}")
+    ldq = _head_rows(q, "q", hq, hd, index)
+    n, wide = kv_len.numel(), hq * hd
+    _int32s(kv_len, n, "kv_len", index)
+    _int32s(cu_q, n + 1, "cu_q", index)
+    ld, width = _block_table(table, n, index)
     if out is None:
-        out = torch.empty(tq, hq * hd, dtype=torch.bfloat16, device=dev)
-    _require(out.shape == (tq, hq * hd) and out.dtype == torch.bfloat16 and out.stride(1) == 1 and out.device == dev,
-             f"out: bf16 ({tq}, {hq * hd}) with contiguous rows")
-    if gate is not None:
-        _require(gate.shape == (tq, hq * hd) and gate.dtype == torch.bfloat16 and gate.stride(1) == 1
-                 and gate.device == dev, f"gate: bf16 ({tq}, {hq * hd}) with contiguous rows")
+        out, ldo = q.new_empty((tq, wide)), wide
+    else:
+        ldo = _wide_rows(out, "out", tq, wide, index)
+    ldg = 0 if gate is None else _wide_rows(gate, "gate", tq, wide, index)
     if n == 0 or tq == 0:
         return out
     _require(hkv > 0 and hq % hkv == 0, "query heads must be a multiple of key/value heads")
-    with torch.cuda.device(dev):
-        size = _cache_workspace(dev.index, n, int(max_q), tq, hq, hkv, hd)
-        scratch = torch.empty(size, dtype=torch.uint8, device=dev)
-        call("kd_attention_cache", q.data_ptr(), ldq, cache.k.data_ptr(), cache.v.data_ptr(),
-             cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), blocks, table.data_ptr(),
-             max(table.stride(0), table.shape[1]), table.shape[1], cu_q.data_ptr(), kv_len.data_ptr(), n, int(max_q),
-             tq, out.data_ptr(), out.stride(0) if tq > 1 else hq * hd, _ptr(gate),
-             0 if gate is None else gate.stride(0) if tq > 1 else hq * hd, hq, hkv, hd, float(scale), int(window[0]),
-             int(window[1]), scratch.data_ptr(), size, status_word(dev).data_ptr(), _stream(q))
+    size = _cache_workspace(index, n, int(max_q), tq, hq, hkv, hd)
+    scratch = q.new_empty(size, dtype=torch.uint8)
+    status = _STATUS.get(index)
+    if status is None:
+        status = status_word(q.device)
+    _call_on(index, "kd_attention_cache", q.data_ptr(), ldq, cache.k.data_ptr(), cache.v.data_ptr(),
+             cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cache.blocks, table.data_ptr(), ld, width,
+             cu_q.data_ptr(), kv_len.data_ptr(), n, max_q, tq, out.data_ptr(), ldo,
+             None if gate is None else gate.data_ptr(), ldg, hq, hkv, hd, scale, window[0], window[1],
+             scratch.data_ptr(), size, status.data_ptr())
     return out

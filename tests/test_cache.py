@@ -75,9 +75,11 @@ def test_the_wrappers_check_types_shapes_and_devices():
     with pytest.raises(ValueError, match="CUDA"):
         ops.attention_cache(rows, cache, torch.zeros(2, 2, dtype=torch.int32), i32, i32[:2], 1, 0.1, (-1, 0))
     with pytest.raises(ValueError, match="scales"):
-        ops.kv_store_e4m3(rows, rows, i32, i32, cache._replace(k_scale=torch.ones(4, 3)))
+        ops.KVBlocks(cache.k, cache.v, torch.ones(4, 3), cache.v_scale)
     with pytest.raises(ValueError, match="e4m3"):
-        ops.kv_store_e4m3(rows, rows, i32, i32, cache._replace(k=torch.zeros(4, 2, 64, 64), v=torch.zeros(4, 2, 64, 64)))
+        ops.KVBlocks(cache.k.float(), cache.v.float(), cache.k_scale, cache.v_scale)
+    with pytest.raises(ValueError, match="codes"):
+        ops.KVBlocks(cache.k[:, :, :32], cache.v[:, :, :32], cache.k_scale, cache.v_scale)
 
 
 def test_the_restatement_rounds_as_torch_does():

@@ -151,7 +151,7 @@ def placed(lens, new, seed=0, spare=3):
 
 
 def check_store(k, v, cu, slots, cache, rows):
-    before = [x.clone() for x in cache]
+    before = [x.clone() for x in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
     ops.kv_store_e4m3(k, v, ints(cu), torch.tensor(slots, dtype=torch.int64, device=DEV), cache)
     kd, vd = k.double().cpu(), v.double().cpu()
     for got, scale, was, was_scale, x, other, is_key in (
