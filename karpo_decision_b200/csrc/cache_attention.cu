@@ -30,24 +30,30 @@ namespace ca {
 constexpr float THRESHOLD = 4.0f;  // log2 units a row's maximum may grow before its sums are rescaled
 constexpr float P_EXPONENT = 11.f, P_SCALE = 2048.f;  // f16 probabilities hold p * 2^11: at most 2^15 with the threshold
 
-// HD: head dim. NT: tiles of 8 query rows a warp holds. Registers bound both (three warpgroups launched at 168, of which the
-// consumers' two take 224 and leave the producer's 56): a thread holds
-// HD NT / 4 sums of the output, and the scores of its keys, for 32 rows of 32 or 16 of them at a time.
+// HD: head dim. NT: tiles of 8 query rows a warp holds. Registers bound both: a thread holds HD NT / 4 sums of the output
+// and the scores of its keys, for 32 rows of half of them at a time.
 template <int HD, int NT>
 struct Cfg {
   static constexpr int RT = 8 * NT;                // query rows of an item
-  static constexpr int WARPS = 8, THREADS = 32 * (WARPS + 4);  // a third warpgroup for the producer, three warps idle
-  static constexpr int KW = HD <= 128 ? 1 : HD / 128;  // warps that share a tile, each 64 / KW of its keys
+  static constexpr int WARPS = 8, THREADS = 32 * (WARPS + 4);  // two warpgroups of consumers, one of producers
+  static constexpr int KW = HD <= 64 ? 1 : HD == 128 ? (NT == 1 ? 2 : 1) : HD / 128;  // warps that share a tile by keys
   static constexpr int TEAMS = WARPS / KW;
-  static constexpr int PARTS = NT < 4 ? 1 : HD == 128 ? 4 : 2;    // steps in which a warp takes its keys
+  static constexpr int PARTS = NT < 4 ? 1 : 2;    // steps in which a warp takes its keys
   static constexpr int MT = BN / KW / PARTS / 16;  // 16-key tiles of a step
   static constexpr int BOX = HD < 128 ? HD : 128;  // bytes of a TMA box row (its swizzle span)
   static constexpr int CHUNKS = HD / BOX;
   static constexpr int TILE_BYTES = BN * HD;
   static constexpr int SLOT_BYTES = 2 * TILE_BYTES;
   static constexpr int SLOTS = 192 * 1024 / SLOT_BYTES;
+  // A producer takes some 650 cycles a tile, as long as a tile of 16 KB takes to arrive: up to four share the ring. Every
+  // slot belongs to one producer, which so sees its uses in order (a parity does not tell laps apart).
+  static constexpr int PRODUCERS = HD <= 128 ? 4 : HD == 256 ? 2 : 1;
+  static_assert(SLOTS % PRODUCERS == 0, "a slot's uses belong to one producer");
+  static_assert(2 * SLOTS % TEAMS == 0, "a team takes every second use of a slot, or every one");
+  // Registers: three warpgroups launched at 168; 256 x CONSUMER + 128 x PRODUCER = 384 x 168.
+  static constexpr int CONSUMER_REGS = NT * HD >= 512 ? 224 : 208, PRODUCER_REGS = NT * HD >= 512 ? 56 : 88;
   static constexpr int Q_BYTES = RT * HD * 2;      // of one item's queries, in the order of the B fragments
-  static constexpr int SMEM = SLOTS * SLOT_BYTES + 2 * Q_BYTES + 1024;
+  static constexpr int SMEM = SLOTS * SLOT_BYTES + TEAMS * Q_BYTES + 1024;
   static constexpr int PARTIAL = RT * (HD + 3);    // floats of one warp's partial: O, then (m, M, l) per row
   static_assert(SMEM + 2048 <= 227 * 1024, "shared memory budget");
 };
@@ -154,7 +160,14 @@ KD_DEVICE void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-KD_DEVICE void consumers_sync(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
+// The warps of one team.
+template <int KW>
+KD_DEVICE void team_sync(int team) {
+  if constexpr (KW == 1)
+    __syncwarp();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * KW) : "memory");
+}
 
 // Shared-memory offset of 16-byte piece `c` of row `row` in a tile stored by TMA with BOX-byte rows and BOX-byte
 // swizzling, chunk by chunk of BOX bytes.
@@ -181,10 +194,10 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
   constexpr int SLOTS = C::SLOTS, RT = C::RT, MT = C::MT;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* s_q = smem + SLOTS * C::SLOT_BYTES;  // [2][Q_BYTES]
+  uint8_t* s_q = smem + SLOTS * C::SLOT_BYTES;  // [TEAMS][Q_BYTES]
   __shared__ uint64_t full[SLOTS], empty[SLOTS];
   __shared__ TileInfo info[SLOTS];
-  __shared__ float s_qscale[2][RT];
+  __shared__ float s_qscale[C::TEAMS][RT];
   __shared__ int64_t s_warp_tiles[C::THREADS / 32], s_before;
   __shared__ int s_warp_items[C::THREADS / 32], s_req, s_items_before;
 
@@ -268,41 +281,44 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
 
   Cursor<RT> c;
   if (warp >= C::WARPS) {
-    set_registers_down<56>();
-    if (warp > C::WARPS) return;
+    set_registers_down<C::PRODUCER_REGS>();
+    const int me = warp - C::WARPS;
+    if (me >= C::PRODUCERS) return;
     c.start(a, s_req, s_before, s_items_before);
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       tma_prefetch_desc(&map_k);
       tma_prefetch_desc(&map_v);
     }
-    // 32 tiles ahead: each lane looks up its tile's block and scales
-    int64_t failed = 0;
+    // This producer's k-th tile is lo + k PRODUCERS + me; each lane looks up one tile's block and scales, 32 ahead.
+    const uint32_t mine = hi - lo > me ? (uint32_t)((hi - lo - me + C::PRODUCERS - 1) / C::PRODUCERS) : 0;
+    uint32_t failed = 0;
     int z = -1, next_z = -1, ve = 0, next_ve = 0;
     float ks = 0.f, next_ks = 0.f;
-    auto look_up = [&](int64_t g, int& zz, float& s, int& e) {
-      zz = -1;
-      s = 0.f;
-      e = 0;
-      if (g < hi) {
+    auto look_up = [&](uint32_t k) {
+      next_z = -1;
+      next_ks = 0.f;
+      next_ve = 0;
+      if (k < mine) {
+        const int64_t g = lo + (int64_t)k * C::PRODUCERS + me;
         c.seek(a, g);
         const int id = a.table[(int64_t)c.i * a.ldt + c.x.r.first + (int)(g - c.begin)];
         if (id >= 0 && id < a.blocks) {
-          zz = id * a.hkv + c.h;
-          s = a.k_scale[zz];
-          e = exponent_of(a.v_scale[zz]);
+          next_z = id * a.hkv + c.h;
+          next_ks = a.k_scale[next_z];
+          next_ve = exponent_of(a.v_scale[next_z]);
         }
       }
     };
-    look_up(lo + lane, next_z, next_ks, next_ve);
-    for (int64_t g0 = lo; g0 < hi; g0 += 32) {
+    look_up(lane);
+    for (uint32_t k0 = 0; k0 < mine; k0 += 32) {
       z = next_z;
       ks = next_ks;
       ve = next_ve;
-      look_up(g0 + 32 + lane, next_z, next_ks, next_ve);
-      const int m = (int)min((int64_t)32, hi - g0);
-      for (int j = 0; j < m; ++j) {
-        const uint32_t at = (uint32_t)(g0 - lo) + j, slot = at % SLOTS;
+      look_up(k0 + 32 + lane);
+      const uint32_t some = min(32u, mine - k0);
+      for (uint32_t j = 0; j < some; ++j) {
+        const uint32_t at = (k0 + j) * C::PRODUCERS + me, slot = at % SLOTS;
         const int zz = __shfl_sync(0xffffffffu, z, j);
         const float s = __shfl_sync(0xffffffffu, ks, j);
         const int e = __shfl_sync(0xffffffffu, ve, j);
@@ -324,21 +340,20 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
           }
         }
         if (!__shfl_sync(0xffffffffu, ok, 0)) {
-          failed = at;
+          failed = k0 + j;
           goto drain;
         }
       }
     }
     return;
   drain:
-    // A consumer gave up: wait (bounded) for the copies in flight before the shared memory goes away. Tiles before
-    // `failed` were issued; slot s last took tile u.
+    // A consumer gave up: wait (bounded) for this producer's copies in flight before the shared memory goes away: the last
+    // tile of each of its slots, of the `failed` that it issued.
     if (lane == 0) {
       const uint64_t start = globaltimer();
-      for (int s = 0; s < SLOTS; ++s) {
-        const int64_t u = failed - 1 - ((failed - 1 - s) % SLOTS + SLOTS) % SLOTS;
-        if (u < 0) continue;
-        while (!mbar_try_wait(smem_u32(&full[s]), (uint32_t)((u / SLOTS) & 1)) && globaltimer() - start < 1000000000ull) {
+      for (uint32_t k = failed > SLOTS / C::PRODUCERS ? failed - SLOTS / C::PRODUCERS : 0; k < failed; ++k) {
+        const uint32_t at = k * C::PRODUCERS + me;
+        while (!mbar_try_wait(smem_u32(&full[at % SLOTS]), (at / SLOTS) & 1) && globaltimer() - start < 1000000000ull) {
         }
       }
     }
@@ -346,7 +361,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
   }
 
   // ------------------------------------------------------------ consumers
-  set_registers_up<224>();
+  set_registers_up<C::CONSUMER_REGS>();
   c.start(a, s_req, s_before, s_items_before);
   const int team = warp / C::KW, part_of = warp % C::KW;
   const int row_g = lane >> 2, t4 = lane & 3;  // fragments: row_g a key or dim (and key + 8), 2 t4 and 2 t4 + 1 query rows
@@ -354,46 +369,58 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
   c.seek(a, lo);
   uint32_t at = team;  // the team's next tile, counted from the CTA's first
   bool dead = false;   // a wait gave up: walk on to the end without computing, so that no warp waits at a barrier alone
-  int buf = 0;
-  for (int64_t g = lo; g < hi; buf ^= 1) {
+  uint2* qf = reinterpret_cast<uint2*>(s_q + team * C::Q_BYTES);
+  // Teams walk the items on their own: one that is done with an item goes on to the next while others finish.
+  for (int64_t g = lo; g < hi;) {
     const int64_t stop = min(c.end, hi);  // the fragment of this item: tiles [g, stop)
     const int lq = c.x.r.lq, lk = c.x.r.lk;
     const int rows = min(RT, lq * a.group - c.rt * RT);
-    // ---- queries: f16, scaled to the row's largest magnitude, in the order of the B fragments; a warp a row
-    uint2* qf = reinterpret_cast<uint2*>(s_q + buf * C::Q_BYTES);
+    if ((int64_t)at + lo < stop) {
+      // ---- queries: f16, scaled to the row's largest magnitude, in the order of the B fragments; RT / KW rows a warp
+      constexpr int MINE = RT / C::KW, UNITS = (HD + 127) / 128, BATCH = MINE * UNITS <= 16 ? MINE : 16 / UNITS;
+      team_sync<C::KW>(team);  // the team has left its last item, whose queries these replace
+#pragma unroll 1
+      for (int i0 = 0; i0 < MINE; i0 += BATCH) {
+        uint2 w[BATCH][UNITS];  // 4 dims a lane and unit
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int rr = nt * 8 + warp, r = c.rt * RT + rr;
-      const int tok = r / a.group;
-      const bool live = rr < rows;
-      const __nv_bfloat16* src = a.q + (int64_t)(c.x.r.q0 + (live ? tok : 0)) * a.ldq +
-                                 (int64_t)(c.h * a.group + (live ? r - tok * a.group : 0)) * HD;
-      constexpr int UNITS = (HD + 127) / 128;  // 4 dims each
-      uint2 w[UNITS];
-      uint32_t top = 0;  // the largest finite magnitude as a bf16 pattern
+        for (int i = 0; i < BATCH; ++i) {
+          const int rr = part_of * MINE + i0 + i, r = c.rt * RT + rr;
+          const int tok = r / a.group;
+          const __nv_bfloat16* src = a.q + (int64_t)(c.x.r.q0 + tok) * a.ldq + (int64_t)(c.h * a.group + r - tok * a.group) * HD;
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        const int d = (u * 32 + lane) * 4;
-        w[u] = live && d < HD ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
-        const uint32_t v[4] = {w[u].x & 0x7fffu, (w[u].x >> 16) & 0x7fffu, w[u].y & 0x7fffu, (w[u].y >> 16) & 0x7fffu};
+          for (int u = 0; u < UNITS; ++u) {
+            const int d = (u * 32 + lane) * 4;
+            w[i][u] = rr < rows && d < HD ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
+          }
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, v[e] < 0x7f80u ? v[e] : 0u);
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      const int e = max((int)(top >> 7) - 127, -120);
-      const float inv = pow2i(-e);
-      if (lane == 0) s_qscale[buf][rr] = pow2i(e) * a.scale_log2;
+        for (int i = 0; i < BATCH; ++i) {
+          const int rr = part_of * MINE + i0 + i;
+          uint32_t top = 0;  // the largest finite magnitude as a bf16 pattern
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        const int d4 = u * 32 + lane;  // dims 4 d4 ..: step d4 / 4, thread d4 % 4 of the fragment
-        if (d4 * 4 < HD) {
-          const float2 p = unpack_bf16x2(w[u].x), q = unpack_bf16x2(w[u].y);
-          qf[((d4 >> 2) * NT + nt) * 32 + warp * 4 + (d4 & 3)] =
-              make_uint2(pack_f16x2(p.x * inv, p.y * inv), pack_f16x2(q.x * inv, q.y * inv));
+          for (int u = 0; u < UNITS; ++u) {
+            const uint2 x = w[i][u];
+            const uint32_t v[4] = {x.x & 0x7fffu, (x.x >> 16) & 0x7fffu, x.y & 0x7fffu, (x.y >> 16) & 0x7fffu};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = max(top, v[e] < 0x7f80u ? v[e] : 0u);
+          }
+          top = __reduce_max_sync(0xffffffffu, top);
+          const int e = max((int)(top >> 7) - 127, -120);
+          const float inv = pow2i(-e);
+          if (lane == 0) s_qscale[team][rr] = pow2i(e) * a.scale_log2;
+#pragma unroll
+          for (int u = 0; u < UNITS; ++u) {
+            const int d4 = u * 32 + lane;  // dims 4 d4 ..: step d4 / 4, thread d4 % 4 of the fragment
+            if (d4 * 4 < HD) {
+              const float2 p = unpack_bf16x2(w[i][u].x), q = unpack_bf16x2(w[i][u].y);
+              qf[((d4 >> 2) * NT + (rr >> 3)) * 32 + (rr & 7) * 4 + (d4 & 3)] =
+                  make_uint2(pack_f16x2(p.x * inv, p.y * inv), pack_f16x2(q.x * inv, q.y * inv));
+            }
+          }
         }
       }
+      team_sync<C::KW>(team);
     }
-    consumers_sync(32 * C::WARPS);  // and every warp has left the item before the last, whose buffer this was
     // the item's rows from the first to the last: which key tiles need a mask
     const int pos0 = c.rt * RT / a.group + lk - lq;
     const int pos1 = (c.rt * RT + rows - 1) / a.group + lk - lq;
@@ -484,7 +511,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int rr = nt * 8 + 2 * t4 + u;
-            const float mul = score_factor(s_qscale[buf][rr], ti.k_scale);
+            const float mul = score_factor(s_qscale[team][rr], ti.k_scale);
             int key_lo = 0, key_hi = 0;
             if (edge) {
               const int pos = (c.rt * RT + rr) / a.group + lk - lq;
@@ -619,140 +646,141 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
   }
 }
 
-// Joins the partials of one row of one item: blockIdx.x the item, blockIdx.y its row. Warp w takes what the CTAs' warps w
-// left, in key order, its lanes the partials' statistics all at once and then HD / 32 columns each; the eight sums are
-// added in order.
+// Joins an item's partials, a block an item, a warp or (few rows) several a row. The lanes read all the partials' statistics
+// of the row together, then HD / 32 columns each of the partials, in key order, eight loads in flight; where several
+// warps share a row, each takes every WPR-th partial and their sums are added in order.
 template <int HD, int NT>
 __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
   using C = Cfg<HD, NT>;
   constexpr int RT = C::RT, V = HD / 32;
+  const int item = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the partials are there after this
-  const int item = blockIdx.x, row = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   if (item >= a.item_cu[a.n] * a.hkv) return;
-  int lo = 0, count = a.n;  // the request holding the item: the last with item_cu * hkv <= item, 32 probes at a time
+  int req = 0, count = a.n;  // the last request with item_cu * hkv <= item, 32 probes at a time
   while (count > 1) {
     const int step = (count + 31) / 32;
-    const bool at_most = (int64_t)a.item_cu[lo + min(lane * step, count - 1)] * a.hkv <= item;
+    const bool at_most = (int64_t)a.item_cu[req + min(lane * step, count - 1)] * a.hkv <= item;
     const int hits = __popc(__ballot_sync(0xffffffffu, at_most));
     const int next = min(max(hits - 1, 0) * step, count - 1);
     count = min(step, count - next);
-    lo += next;
+    req += next;
   }
-  const Rows x = rows_of<RT>(a, lo);
-  const int local = item - a.item_cu[lo] * a.hkv;
+  const Rows x = rows_of<RT>(a, req);
+  const int local = item - a.item_cu[req] * a.hkv;
   const int h = local / x.nrt, rt = local - h * x.nrt;
-  const int gr = rt * RT + row;
-  if (gr >= x.r.lq * a.group) return;
+  const int rows = min(RT, x.r.lq * a.group - rt * RT);
   const int64_t total = a.tile_cu[a.n] * a.hkv;
-  const int64_t begin = a.tile_cu[lo] * a.hkv + (int64_t)local * x.r.tiles, end = begin + x.r.tiles;
+  const int64_t begin = a.tile_cu[req] * a.hkv + (int64_t)local * x.r.tiles, end = begin + x.r.tiles;
   // CTA c holds tiles [c total / P, (c + 1) total / P): the one holding tile g is ((g + 1) P - 1) / total
   const int64_t p = shares(total, ctas);
   const int c0 = x.r.tiles ? (int)quotient((begin + 1) * p - 1, total) : 0;
-  const int n = x.r.tiles ? (int)quotient(end * p - 1, total) - c0 + 1 : 0;
-  const float* part = a.partials + ((int64_t)(item + c0) * C::WARPS + warp) * C::PARTIAL;
-  constexpr int64_t STEP = (int64_t)C::WARPS * C::PARTIAL;
-  __shared__ float s_red[2][8], s_l[8];
+  const int n = x.r.tiles ? ((int)quotient(end * p - 1, total) - c0 + 1) * C::WARPS : 0;  // partials, one behind another
+  const float* part = a.partials + (int64_t)(item + c0) * C::WARPS * C::PARTIAL;
+  const int wpr = rows == 1 ? 8 : rows == 2 ? 4 : rows <= 4 ? 2 : 1;
+  const int sub = warp % wpr;
   __shared__ __align__(16) float s_o[8][HD];
-  float m = -INFINITY, big = -INFINITY;
-  for (int q = lane; q < n; q += 32) {
-    const float* st = part + q * STEP + RT * HD + 3 * row;
-    m = fmaxf(m, st[0]);
-    big = fmaxf(big, st[1]);
-  }
+  for (int r0 = 0; r0 < rows; r0 += 8 / wpr) {
+    const int row = r0 + warp / wpr;
+    const bool live = row < rows;
+    float acc[V], l = 0.f, m = -INFINITY, big = -INFINITY;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-  }
-  if (lane == 0) {
-    s_red[0][warp] = m;
-    s_red[1][warp] = big;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    m = fmaxf(m, s_red[0][w]);
-    big = fmaxf(big, s_red[1][w]);
-  }
-  const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
-  float l = 0.f, acc[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) acc[e] = 0.f;
-  for (int q0 = 0; q0 < n; q0 += 32) {
-    float f = -1.f;  // < 0: the warp met no key there (its sums may hold anything)
-    if (q0 + lane < n) {
-      const float* st = part + (q0 + lane) * STEP + RT * HD + 3 * row;
-      l += st[2] * fast_exp2(st[0] - base);
-      if (st[1] != -INFINITY || st[2] != 0.f) f = fast_exp2(st[1] - vbase);
-    }
-    const int some = min(32, n - q0);
-    constexpr int BATCH = V <= 4 ? 8 : 4;
-    for (int q1 = 0; q1 < some; q1 += BATCH) {
-      float y[BATCH][V], w[BATCH];
-#pragma unroll
-      for (int q = 0; q < BATCH; ++q) {
-        w[q] = __shfl_sync(0xffffffffu, f, (q1 + q) & 31);
-        if (q1 + q >= some) w[q] = -1.f;
-        const float* src = part + (q0 + q1 + q) * STEP + row * HD;
-#pragma unroll
-        for (int e = 0; e < V; ++e) y[q][e] = 0.f;
-        if (!(w[q] < 0.f)) {
-          if constexpr (V == 2) {
-            const float2 t = *reinterpret_cast<const float2*>(src + lane * 2);
-            y[q][0] = t.x;
-            y[q][1] = t.y;
-          } else {
-#pragma unroll
-            for (int e = 0; e < V; e += 4) {
-              const float4 t = *reinterpret_cast<const float4*>(src + e * 32 + lane * 4);
-              y[q][e] = t.x;
-              y[q][e + 1] = t.y;
-              y[q][e + 2] = t.z;
-              y[q][e + 3] = t.w;
-            }
-          }
-        }
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+    if (live) {
+      const float* stats = part + RT * HD + 3 * row;
+      for (int q = lane; q < n; q += 32) {
+        m = fmaxf(m, stats[(int64_t)q * C::PARTIAL]);
+        big = fmaxf(big, stats[(int64_t)q * C::PARTIAL + 1]);
       }
 #pragma unroll
-      for (int q = 0; q < BATCH; ++q)
+      for (int o = 16; o > 0; o >>= 1) {
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+      }
+      const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
+      for (int q = lane; q < n; q += 32)
+        l += stats[(int64_t)q * C::PARTIAL + 2] * fast_exp2(stats[(int64_t)q * C::PARTIAL] - base);
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] += y[q][e] * (w[q] < 0.f ? 0.f : w[q]);
+      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      const int mine = n > sub ? (n - sub + wpr - 1) / wpr : 0;  // this warp's partials: sub, sub + wpr, ..
+      for (int k0 = 0; k0 < mine; k0 += 32) {
+        float f = -1.f;  // < 0: the warp met no key of the row there (its sums may hold anything)
+        if (k0 + lane < mine) {
+          const float* st = stats + (int64_t)(sub + (k0 + lane) * wpr) * C::PARTIAL;
+          if (st[1] != -INFINITY || st[2] != 0.f) f = fast_exp2(st[1] - vbase);
+        }
+        const int some = min(32, mine - k0);
+        constexpr int BATCH = V <= 4 ? 8 : 4;
+        for (int k1 = 0; k1 < some; k1 += BATCH) {
+          float y[BATCH][V], w[BATCH];
+#pragma unroll
+          for (int q = 0; q < BATCH; ++q) {
+            w[q] = __shfl_sync(0xffffffffu, f, (k1 + q) & 31);
+            if (k1 + q >= some) w[q] = -1.f;
+            const float* src = part + (int64_t)(sub + (k0 + k1 + q) * wpr) * C::PARTIAL + row * HD;
+#pragma unroll
+            for (int e = 0; e < V; ++e) y[q][e] = 0.f;
+            if (!(w[q] < 0.f)) {
+              if constexpr (V == 2) {
+                const float2 t = *reinterpret_cast<const float2*>(src + lane * 2);
+                y[q][0] = t.x;
+                y[q][1] = t.y;
+              } else {
+#pragma unroll
+                for (int e = 0; e < V; e += 4) {
+                  const float4 t = *reinterpret_cast<const float4*>(src + e * 32 + lane * 4);
+                  y[q][e] = t.x;
+                  y[q][e + 1] = t.y;
+                  y[q][e + 2] = t.z;
+                  y[q][e + 3] = t.w;
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < BATCH; ++q)
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] += y[q][e] * (w[q] < 0.f ? 0.f : w[q]);
+        }
+      }
     }
-  }
+    if (wpr > 1) {  // one pass of the loop: rows <= 8 / wpr
+      if (sub > 0) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  if (lane == 0) s_l[warp] = l;
-  if constexpr (V == 2) {
-    *reinterpret_cast<float2*>(&s_o[warp][lane * 2]) = make_float2(acc[0], acc[1]);
-  } else {
+        for (int e = 0; e < V; ++e) s_o[warp][e * 32 + lane] = acc[e];
+      }
+      __syncthreads();
+      if (sub > 0) continue;
+      for (int w = 1; w < wpr; ++w)
 #pragma unroll
-    for (int e = 0; e < V; e += 4)
-      *reinterpret_cast<float4*>(&s_o[warp][e * 32 + lane * 4]) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
-  }
-  __syncthreads();
-  l = 0.f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) l += s_l[w];
-  // o = O 2^(M - m) / (2^11 l); without a visible key 0
-  const float fin = l == 0.f ? 0.f : fast_exp2(fminf(vbase - base, 126.f)) / (l * P_SCALE);
-  const int tok = gr / a.group, head = h * a.group + gr - tok * a.group;
-  const int64_t orow = (int64_t)(x.r.q0 + tok) * a.ldo + (int64_t)head * HD;
-  const int64_t grow = (int64_t)(x.r.q0 + tok) * a.ldg + (int64_t)head * HD;
-  for (int d = threadIdx.x; d < HD / 2; d += 256) {
-    float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      const float2 y = *reinterpret_cast<const float2*>(&s_o[w][2 * d]);
-      sum.x += y.x;
-      sum.y += y.y;
+        for (int e = 0; e < V; ++e) acc[e] += s_o[warp + w][e * 32 + lane];
     }
-    float2 y = l == 0.f ? make_float2(0.f, 0.f) : make_float2(sum.x * fin, sum.y * fin);
-    if (a.gate && l != 0.f) {
-      const float2 s = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(a.gate + grow + 2 * d));
-      y.x = x_sigmoid(y.x, s.x);
-      y.y = x_sigmoid(y.y, s.y);
+    if (!live) continue;
+    // o = O 2^(M - m) / (2^11 l); without a visible key 0
+    const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
+    const float fin = l == 0.f ? 0.f : fast_exp2(fminf(vbase - base, 126.f)) / (l * P_SCALE);
+    const int gr = rt * RT + row, tok = gr / a.group, head = h * a.group + gr - tok * a.group;
+    const int64_t orow = (int64_t)(x.r.q0 + tok) * a.ldo + (int64_t)head * HD;
+    const int64_t grow = (int64_t)(x.r.q0 + tok) * a.ldg + (int64_t)head * HD;
+    constexpr int W = V == 2 ? 2 : 4;  // neighbouring columns of a lane
+#pragma unroll
+    for (int e = 0; e < V; e += W) {
+      const int d = e * 32 + lane * W;
+      uint32_t out[W / 2];
+#pragma unroll
+      for (int y = 0; y < W / 2; ++y) {
+        float2 v = l == 0.f ? make_float2(0.f, 0.f) : make_float2(acc[e + 2 * y] * fin, acc[e + 2 * y + 1] * fin);
+        if (a.gate && l != 0.f) {
+          const float2 s = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(a.gate + grow + d + 2 * y));
+          v.x = x_sigmoid(v.x, s.x);
+          v.y = x_sigmoid(v.y, s.y);
+        }
+        out[y] = pack_bf16x2(v.x, v.y);
+      }
+      if constexpr (W == 2)
+        *reinterpret_cast<uint32_t*>(a.out + orow + d) = out[0];
+      else
+        *reinterpret_cast<uint2*>(a.out + orow + d) = make_uint2(out[0], out[1]);
     }
-    *reinterpret_cast<uint32_t*>(a.out + orow + 2 * d) = pack_bf16x2(y.x, y.y);
   }
 }
 
@@ -762,7 +790,7 @@ static int row_tiles_of_8(int max_q, int group, int head_dim) {
   const int64_t rows = (int64_t)max_q * group;
   if (rows <= 8) return 1;
   if (rows <= 16 && head_dim <= 256) return 2;
-  if (rows <= 32 && head_dim <= 128) return 4;
+  if (rows <= 32 && head_dim == 64) return 4;
   return 0;
 }
 
@@ -812,7 +840,7 @@ int launch(Args a, const void* k_codes, const void* v_codes, uint8_t* ws, int64_
   kernel<<<ctas, C::THREADS, C::SMEM, stream>>>(mk, mv, a);
   rc = record_cuda_error(cudaGetLastError(), "attention_cache: launch");
   if (rc) return rc;
-  return launch_after(join_kernel<HD, NT>, dim3((unsigned)items, C::RT), 256, stream, a, ctas);
+  return launch_after(join_kernel<HD, NT>, dim3((unsigned)items), 256, stream, a, ctas);
 }
 
 // Calls f.template operator()<HD, NT>() for the kernel of a head dim and a number of 8-row tiles.
@@ -825,8 +853,7 @@ auto with_kernel(int head_dim, int nt, F f) {
                        : f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
     case 128:
       return nt == 1 ? f(std::integral_constant<int, 128>{}, std::integral_constant<int, 1>{})
-             : nt == 2 ? f(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{})
-                       : f(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{});
+                     : f(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{});
     case 256:
       return nt == 1 ? f(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{})
                      : f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
