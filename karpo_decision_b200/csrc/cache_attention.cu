@@ -9,7 +9,8 @@
 // Few query rows per key/value head (the rows of a request that share a head's keys: Lq * Hq / Hkv) are bound by the
 // reads of the codes: 2 hd bytes a token and head, once. The work is the list of key tiles (one block of 64 tokens) of
 // every (request, key/value head, row tile), in that order; CTA c of P takes the tiles [c, c + 1) * total / P of it, so
-// long and short requests balance to a tile without the host knowing a length. A producer warp reads 32 tiles' table
+// long and short requests balance without the host knowing a length (an item counts ITEM_TILES further tiles, before its
+// own, for what it costs beside them). A producer warp reads 32 tiles' table
 // entries and scales at a time and keeps a ring of 192 KB filled by TMA; eight warps take the tiles in turn (teams of
 // two or four for heads of 256 and 512, each warp a part of the tile's keys), each with a running maximum and sums of
 // its own, and leave a partial result per item that they met; a second launch joins them.
@@ -29,6 +30,8 @@ namespace ca {
 
 constexpr float THRESHOLD = 4.0f;  // log2 units a row's maximum may grow before its sums are rescaled
 constexpr float P_EXPONENT = 11.f, P_SCALE = 2048.f;  // f16 probabilities hold p * 2^11: at most 2^15 with the threshold
+
+constexpr int ITEM_TILES = 8;  // an item's own cost (queries, its partial, the teams' drain) in key tiles: some 6,000 cycles
 
 // HD: head dim. NT: tiles of 8 query rows a warp holds. Registers bound both: a thread holds HD NT / 4 sums of the output
 // and the scores of its keys, for 32 rows of half of them at a time.
@@ -97,7 +100,7 @@ struct Cursor {
     load(a);
   }
   KD_DEVICE void seek(const Args& a, int64_t g) {
-    if (i < a.n && g >= end && x.r.tiles > 0) {  // whole items of this request at once
+    if (i < a.n && g >= end && g - end >= x.r.tiles) {  // whole items of this request at once
       const int64_t left = (int64_t)(a.hkv - h) * x.nrt - rt;  // items from this one to the request's last
       const int64_t k = min(left - 1, quotient(g - begin, x.r.tiles));
       const int64_t to = (int64_t)h * x.nrt + rt + k;
@@ -180,6 +183,12 @@ KD_DEVICE uint32_t piece(int row, int c) {
   }
 }
 
+// An item, for the launch that joins its partials.
+struct Desc {
+  int q0, h, r0, rows;  // the request's first query row, the key/value head, the item's first packed row and their number
+  int first, n;         // its partials, one behind another
+};
+
 // One tile's meta data beside its ring slot.
 struct TileInfo {
   float k_scale, v_exp;
@@ -198,10 +207,11 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
   __shared__ uint64_t full[SLOTS], empty[SLOTS];
   __shared__ TileInfo info[SLOTS];
   __shared__ float s_qscale[C::TEAMS][RT];
-  __shared__ int64_t s_warp_tiles[C::THREADS / 32], s_before;
+  __shared__ int64_t s_warp_tiles[C::THREADS / 32], s_before, s_ends[2];
   __shared__ int s_warp_items[C::THREADS / 32], s_req, s_items_before;
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+  Desc* descs = reinterpret_cast<Desc*>(a.descs);
   if (tid == 0) {
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&full[s], 1);
@@ -209,8 +219,9 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
     }
     fence_barrier_init();
   }
-  // ---- this CTA's share of the tiles: a scan of the requests' tiles for the total, then (a second scan if the requests
-  // outnumber the threads) for the share's first request
+  // ---- this CTA's share of the tiles: a scan of the requests' tiles and items for the total, then (a second scan if the
+  // requests outnumber the threads) for the share's first request and the tiles at its ends. w counts key tiles of one
+  // key/value head; with ITEM_TILES for each item before it, that is the weight that the shares divide.
   int64_t w_mine = 0, w_before = 0, tiles = 0;
   int items_mine = 0, items_before = 0, items = 0;
   auto scan = [&](int i0, int64_t carry, int carry_items) {
@@ -254,29 +265,45 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
     items = carry_items;
   };
   for (int i0 = 0; i0 < a.n; i0 += C::THREADS) scan(i0, tiles, items);
-  const int64_t total = tiles * a.hkv;
+  const int64_t total = (tiles + (int64_t)ITEM_TILES * items) * a.hkv;
   const int np = (int)shares(total, gridDim.x);
-  const int64_t lo = quotient(total * blockIdx.x, np);
-  const int64_t hi = (int)blockIdx.x < np ? quotient(total * (blockIdx.x + 1), np) : 0;
+  const int64_t v_lo = quotient(total * blockIdx.x, np);
+  const int64_t v_hi = (int)blockIdx.x < np ? quotient(total * (blockIdx.x + 1), np) : v_lo;
+  if (tid == 0) s_ends[0] = s_ends[1] = tiles * a.hkv;  // a bound past the last request
+  __syncthreads();
   if (a.n > C::THREADS) tiles = items = 0;
   for (int i0 = 0; i0 < a.n; i0 += C::THREADS) {
     if (a.n > C::THREADS) scan(i0, tiles, items);
     const int i = i0 + tid;
-    if (i < a.n && blockIdx.x == 0) {  // for the launch that joins the partials
-      a.tile_cu[i] = w_before;
-      a.item_cu[i] = items_before;
-    }
-    if (w_mine > 0 && lo >= w_before * a.hkv && lo < (w_before + w_mine) * a.hkv) {
-      s_req = i;
-      s_before = w_before * a.hkv;
-      s_items_before = items_before * a.hkv;
+    if (items_mine > 0) {
+      if (w_mine == 0 && blockIdx.x == 0) {  // rows that see no key: for the launch that joins the partials
+        const Rows x = rows_of<RT>(a, i);
+        for (int k = 0; k < items_mine * a.hkv; ++k) {
+          const int h = k / items_mine, r0 = (k - h * items_mine) * RT;
+          descs[items_before * a.hkv + k] = Desc{x.r.q0, h, r0, min(RT, x.r.lq * a.group - r0), 0, 0};
+        }
+      }
+      const int64_t v = (w_before + (int64_t)ITEM_TILES * items_before) * a.hkv;  // the request's weights
+      const int64_t own = w_mine + (int64_t)ITEM_TILES * items_mine;
+      const int64_t per = own / items_mine, mine = w_mine / items_mine;            // an item's weight, its tiles
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int64_t x = (e ? v_hi : v_lo) - v;
+        if (x >= 0 && x < own * a.hkv) {
+          const int64_t k = quotient(x, per);
+          s_ends[e] = w_before * a.hkv + k * mine + max((int64_t)0, x - k * per - ITEM_TILES);
+          if (e == 0) {
+            s_req = i;
+            s_before = w_before * a.hkv;
+            s_items_before = items_before * a.hkv;
+          }
+        }
+      }
     }
   }
-  if (tid == 0 && blockIdx.x == 0) {
-    a.tile_cu[a.n] = tiles;
-    a.item_cu[a.n] = items;
-  }
+  if (tid == 0 && blockIdx.x == 0) *a.items = items * a.hkv;
   __syncthreads();
+  const int64_t lo = s_ends[0], hi = s_ends[1];
   if (lo >= hi) return;
 
   Cursor<RT> c;
@@ -375,48 +402,52 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
     const int64_t stop = min(c.end, hi);  // the fragment of this item: tiles [g, stop)
     const int lq = c.x.r.lq, lk = c.x.r.lk;
     const int rows = min(RT, lq * a.group - c.rt * RT);
+    if (g == c.begin && tid == 0) {
+      // the weight at the item's first tile is c.begin + ITEM_TILES * (its number + 1); the last tile's CTA as in the shares
+      const int64_t v = c.begin + (int64_t)ITEM_TILES * (c.item + 1) + c.x.r.tiles;
+      const int last = (int)quotient(v * np - 1, total);
+      descs[c.item] = Desc{c.x.r.q0, c.h, c.rt * RT, rows, (c.item + (int)blockIdx.x) * C::WARPS,
+                           (last - (int)blockIdx.x + 1) * C::WARPS};
+    }
     if ((int64_t)at + lo < stop) {
-      // ---- queries: f16, scaled to the row's largest magnitude, in the order of the B fragments; RT / KW rows a warp
-      constexpr int MINE = RT / C::KW, UNITS = (HD + 127) / 128, BATCH = MINE * UNITS <= 16 ? MINE : 16 / UNITS;
+      // ---- queries: f16, scaled to the row's largest magnitude, in the order of the B fragments; RT / KW rows a warp, LPR
+      // lanes a row, each every LPR-th piece of 8 dims
+      constexpr int MINE = RT / C::KW, LPR = MINE >= 32 ? 1 : 32 / MINE, PIECES = HD / 8 / LPR > 0 ? HD / 8 / LPR : 1;
+      static_assert(MINE <= 32, "a lane has one row");
       team_sync<C::KW>(team);  // the team has left its last item, whose queries these replace
-#pragma unroll 1
-      for (int i0 = 0; i0 < MINE; i0 += BATCH) {
-        uint2 w[BATCH][UNITS];  // 4 dims a lane and unit
+      const int rr = part_of * MINE + lane / LPR, first = lane % LPR, r = c.rt * RT + rr;
+      const int tok = r / a.group;
+      const __nv_bfloat16* src = a.q + (int64_t)(c.x.r.q0 + tok) * a.ldq + (int64_t)(c.h * a.group + r - tok * a.group) * HD;
+      uint4 w[PIECES];
+      uint32_t top = 0;  // the largest finite magnitude as a bf16 pattern
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          const int rr = part_of * MINE + i0 + i, r = c.rt * RT + rr;
-          const int tok = r / a.group;
-          const __nv_bfloat16* src = a.q + (int64_t)(c.x.r.q0 + tok) * a.ldq + (int64_t)(c.h * a.group + r - tok * a.group) * HD;
+      for (int u = 0; u < PIECES; ++u) {
+        const int d8 = u * LPR + first;
+        w[u] = rr < rows && d8 < HD / 8 ? reinterpret_cast<const uint4*>(src)[d8] : make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
-          for (int u = 0; u < UNITS; ++u) {
-            const int d = (u * 32 + lane) * 4;
-            w[i][u] = rr < rows && d < HD ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
-          }
+      for (int u = 0; u < PIECES; ++u) {
+        const uint32_t x[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t v0 = x[e] & 0x7fffu, v1 = (x[e] >> 16) & 0x7fffu;
+          top = max(top, max(v0 < 0x7f80u ? v0 : 0u, v1 < 0x7f80u ? v1 : 0u));
         }
+      }
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          const int rr = part_of * MINE + i0 + i;
-          uint32_t top = 0;  // the largest finite magnitude as a bf16 pattern
+      for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const int e = max((int)(top >> 7) - 127, -120);
+      const float inv = pow2i(-e);
+      if (first == 0) s_qscale[team][rr] = pow2i(e) * a.scale_log2;
 #pragma unroll
-          for (int u = 0; u < UNITS; ++u) {
-            const uint2 x = w[i][u];
-            const uint32_t v[4] = {x.x & 0x7fffu, (x.x >> 16) & 0x7fffu, x.y & 0x7fffu, (x.y >> 16) & 0x7fffu};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, v[e] < 0x7f80u ? v[e] : 0u);
-          }
-          top = __reduce_max_sync(0xffffffffu, top);
-          const int e = max((int)(top >> 7) - 127, -120);
-          const float inv = pow2i(-e);
-          if (lane == 0) s_qscale[team][rr] = pow2i(e) * a.scale_log2;
-#pragma unroll
-          for (int u = 0; u < UNITS; ++u) {
-            const int d4 = u * 32 + lane;  // dims 4 d4 ..: step d4 / 4, thread d4 % 4 of the fragment
-            if (d4 * 4 < HD) {
-              const float2 p = unpack_bf16x2(w[i][u].x), q = unpack_bf16x2(w[i][u].y);
-              qf[((d4 >> 2) * NT + (rr >> 3)) * 32 + (rr & 7) * 4 + (d4 & 3)] =
-                  make_uint2(pack_f16x2(p.x * inv, p.y * inv), pack_f16x2(q.x * inv, q.y * inv));
-            }
-          }
+      for (int u = 0; u < PIECES; ++u) {
+        const int d8 = u * LPR + first;  // dims 8 d8 ..: step d8 / 2, threads 2 (d8 % 2) and the next of the fragment
+        if (d8 < HD / 8) {
+          const float2 p0 = unpack_bf16x2(w[u].x), p1 = unpack_bf16x2(w[u].y), p2 = unpack_bf16x2(w[u].z),
+                       p3 = unpack_bf16x2(w[u].w);
+          *reinterpret_cast<uint4*>(qf + ((d8 >> 1) * NT + (rr >> 3)) * 32 + (rr & 7) * 4 + (d8 & 1) * 2) =
+              make_uint4(pack_f16x2(p0.x * inv, p0.y * inv), pack_f16x2(p1.x * inv, p1.y * inv),
+                         pack_f16x2(p2.x * inv, p2.y * inv), pack_f16x2(p3.x * inv, p3.y * inv));
         }
       }
       team_sync<C::KW>(team);
@@ -646,142 +677,143 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
   }
 }
 
-// Joins an item's partials, a block an item, a warp or (few rows) several a row. The lanes read all the partials' statistics
-// of the row together, then HD / 32 columns each of the partials, in key order, eight loads in flight; where several
-// warps share a row, each takes every WPR-th partial and their sums are added in order.
+// Joins an item's partials. A warp has 128 columns (64 for heads of 64) of a row, so a block RB rows; where the item has
+// fewer, several warps share a row and each takes every WPR-th partial. The lanes read all the partials' statistics of the
+// row together, then four columns each of the partials, in key order, eight loads in flight.
 template <int HD, int NT>
 __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
   using C = Cfg<HD, NT>;
-  constexpr int RT = C::RT, V = HD / 32;
-  const int item = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  constexpr int RT = C::RT, CW = HD <= 128 ? 1 : HD / 128, RB = 8 / CW, V = HD == 64 ? 2 : 4;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the partials are there after this
-  if (item >= a.item_cu[a.n] * a.hkv) return;
-  int req = 0, count = a.n;  // the last request with item_cu * hkv <= item, 32 probes at a time
-  while (count > 1) {
-    const int step = (count + 31) / 32;
-    const bool at_most = (int64_t)a.item_cu[req + min(lane * step, count - 1)] * a.hkv <= item;
-    const int hits = __popc(__ballot_sync(0xffffffffu, at_most));
-    const int next = min(max(hits - 1, 0) * step, count - 1);
-    count = min(step, count - next);
-    req += next;
+  const int items = *a.items;
+  const Desc d = reinterpret_cast<const Desc*>(a.descs)[blockIdx.x];
+  const int r0 = blockIdx.y * RB;
+  if ((int)blockIdx.x >= items || r0 >= d.rows) return;
+  const int n = d.n;
+  const float* part = a.partials + (int64_t)d.first * C::PARTIAL;
+  const int here = min(RB, d.rows - r0);
+  const int wpr = here * 2 > RB ? 1 : here * 4 > RB ? 2 : here * 8 > RB ? 4 : 8;  // warps of a row's columns
+  const int unit = warp / CW, col = (warp % CW) * 128 + lane * V;
+  const int sub = unit % wpr, row = r0 + unit / wpr;
+  const bool live = row < d.rows;
+  const int gr = d.r0 + (live ? row : 0), tok = gr / a.group, head = d.h * a.group + gr - tok * a.group;
+  uint2 gate = make_uint2(0, 0);
+  if (a.gate && live) {
+    const __nv_bfloat16* src = a.gate + (int64_t)(d.q0 + tok) * a.ldg + (int64_t)head * HD + col;
+    if constexpr (V == 4)
+      gate = *reinterpret_cast<const uint2*>(src);
+    else
+      gate.x = *reinterpret_cast<const uint32_t*>(src);
   }
-  const Rows x = rows_of<RT>(a, req);
-  const int local = item - a.item_cu[req] * a.hkv;
-  const int h = local / x.nrt, rt = local - h * x.nrt;
-  const int rows = min(RT, x.r.lq * a.group - rt * RT);
-  const int64_t total = a.tile_cu[a.n] * a.hkv;
-  const int64_t begin = a.tile_cu[req] * a.hkv + (int64_t)local * x.r.tiles, end = begin + x.r.tiles;
-  // CTA c holds tiles [c total / P, (c + 1) total / P): the one holding tile g is ((g + 1) P - 1) / total
-  const int64_t p = shares(total, ctas);
-  const int c0 = x.r.tiles ? (int)quotient((begin + 1) * p - 1, total) : 0;
-  const int n = x.r.tiles ? ((int)quotient(end * p - 1, total) - c0 + 1) * C::WARPS : 0;  // partials, one behind another
-  const float* part = a.partials + (int64_t)(item + c0) * C::WARPS * C::PARTIAL;
-  const int wpr = rows == 1 ? 8 : rows == 2 ? 4 : rows <= 4 ? 2 : 1;
-  const int sub = warp % wpr;
-  __shared__ __align__(16) float s_o[8][HD];
-  for (int r0 = 0; r0 < rows; r0 += 8 / wpr) {
-    const int row = r0 + warp / wpr;
-    const bool live = row < rows;
-    float acc[V], l = 0.f, m = -INFINITY, big = -INFINITY;
+  float acc[V], l = 0.f, m = -INFINITY, big = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = 0.f;
-    if (live) {
-      const float* stats = part + RT * HD + 3 * row;
-      for (int q = lane; q < n; q += 32) {
-        m = fmaxf(m, stats[(int64_t)q * C::PARTIAL]);
-        big = fmaxf(big, stats[(int64_t)q * C::PARTIAL + 1]);
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+  if (live) {
+    const float* stats = part + RT * HD + 3 * row;
+    for (int q0 = lane; q0 < n; q0 += 128) {  // four loads in flight
+      float x[4], y[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float* st = stats + (int64_t)(q0 + 32 * u) * C::PARTIAL;
+        x[u] = q0 + 32 * u < n ? st[0] : -INFINITY;
+        y[u] = q0 + 32 * u < n ? st[1] : -INFINITY;
       }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+      for (int u = 0; u < 4; ++u) {
+        m = fmaxf(m, x[u]);
+        big = fmaxf(big, y[u]);
       }
-      const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
-      for (int q = lane; q < n; q += 32)
-        l += stats[(int64_t)q * C::PARTIAL + 2] * fast_exp2(stats[(int64_t)q * C::PARTIAL] - base);
+    }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      const int mine = n > sub ? (n - sub + wpr - 1) / wpr : 0;  // this warp's partials: sub, sub + wpr, ..
-      for (int k0 = 0; k0 < mine; k0 += 32) {
-        float f = -1.f;  // < 0: the warp met no key of the row there (its sums may hold anything)
-        if (k0 + lane < mine) {
-          const float* st = stats + (int64_t)(sub + (k0 + lane) * wpr) * C::PARTIAL;
-          if (st[1] != -INFINITY || st[2] != 0.f) f = fast_exp2(st[1] - vbase);
-        }
-        const int some = min(32, mine - k0);
-        constexpr int BATCH = V <= 4 ? 8 : 4;
-        for (int k1 = 0; k1 < some; k1 += BATCH) {
-          float y[BATCH][V], w[BATCH];
+    for (int o = 16; o > 0; o >>= 1) {
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+    }
+    const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
+    for (int q0 = lane; q0 < n; q0 += 128) {
+      float x[4], y[4];
 #pragma unroll
-          for (int q = 0; q < BATCH; ++q) {
-            w[q] = __shfl_sync(0xffffffffu, f, (k1 + q) & 31);
-            if (k1 + q >= some) w[q] = -1.f;
-            const float* src = part + (int64_t)(sub + (k0 + k1 + q) * wpr) * C::PARTIAL + row * HD;
+      for (int u = 0; u < 4; ++u) {
+        const float* st = stats + (int64_t)(q0 + 32 * u) * C::PARTIAL;
+        x[u] = q0 + 32 * u < n ? st[0] : -INFINITY;
+        y[u] = q0 + 32 * u < n ? st[2] : 0.f;
+      }
 #pragma unroll
-            for (int e = 0; e < V; ++e) y[q][e] = 0.f;
-            if (!(w[q] < 0.f)) {
-              if constexpr (V == 2) {
-                const float2 t = *reinterpret_cast<const float2*>(src + lane * 2);
-                y[q][0] = t.x;
-                y[q][1] = t.y;
-              } else {
+      for (int u = 0; u < 4; ++u) l += y[u] * fast_exp2(x[u] - base);
+    }
 #pragma unroll
-                for (int e = 0; e < V; e += 4) {
-                  const float4 t = *reinterpret_cast<const float4*>(src + e * 32 + lane * 4);
-                  y[q][e] = t.x;
-                  y[q][e + 1] = t.y;
-                  y[q][e + 2] = t.z;
-                  y[q][e + 3] = t.w;
-                }
-              }
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const int mine = n > sub ? (n - sub + wpr - 1) / wpr : 0;  // this warp's partials: sub, sub + wpr, ..
+    for (int k0 = 0; k0 < mine; k0 += 32) {
+      float f = -1.f;  // < 0: the warp that left it met no key of the row (its sums may hold anything)
+      if (k0 + lane < mine) {
+        const float* st = stats + (int64_t)(sub + (k0 + lane) * wpr) * C::PARTIAL;
+        if (st[1] != -INFINITY || st[2] != 0.f) f = fast_exp2(st[1] - vbase);
+      }
+      const int some = min(32, mine - k0);
+      for (int k1 = 0; k1 < some; k1 += 8) {
+        float4 y[8];
+        float w[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          w[q] = __shfl_sync(0xffffffffu, f, (k1 + q) & 31);
+          if (k1 + q >= some) w[q] = -1.f;
+          y[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (!(w[q] < 0.f)) {
+            const float* src = part + (int64_t)(sub + (k0 + k1 + q) * wpr) * C::PARTIAL + row * HD + col;
+            if constexpr (V == 4) {
+              y[q] = *reinterpret_cast<const float4*>(src);
+            } else {
+              const float2 t = *reinterpret_cast<const float2*>(src);
+              y[q].x = t.x;
+              y[q].y = t.y;
             }
           }
+        }
 #pragma unroll
-          for (int q = 0; q < BATCH; ++q)
-#pragma unroll
-            for (int e = 0; e < V; ++e) acc[e] += y[q][e] * (w[q] < 0.f ? 0.f : w[q]);
+        for (int q = 0; q < 8; ++q) {
+          const float x = w[q] < 0.f ? 0.f : w[q];
+          acc[0] += y[q].x * x;
+          acc[1] += y[q].y * x;
+          if constexpr (V == 4) {
+            acc[2] += y[q].z * x;
+            acc[3] += y[q].w * x;
+          }
         }
       }
-    }
-    if (wpr > 1) {  // one pass of the loop: rows <= 8 / wpr
-      if (sub > 0) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) s_o[warp][e * 32 + lane] = acc[e];
-      }
-      __syncthreads();
-      if (sub > 0) continue;
-      for (int w = 1; w < wpr; ++w)
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] += s_o[warp + w][e * 32 + lane];
-    }
-    if (!live) continue;
-    // o = O 2^(M - m) / (2^11 l); without a visible key 0
-    const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
-    const float fin = l == 0.f ? 0.f : fast_exp2(fminf(vbase - base, 126.f)) / (l * P_SCALE);
-    const int gr = rt * RT + row, tok = gr / a.group, head = h * a.group + gr - tok * a.group;
-    const int64_t orow = (int64_t)(x.r.q0 + tok) * a.ldo + (int64_t)head * HD;
-    const int64_t grow = (int64_t)(x.r.q0 + tok) * a.ldg + (int64_t)head * HD;
-    constexpr int W = V == 2 ? 2 : 4;  // neighbouring columns of a lane
-#pragma unroll
-    for (int e = 0; e < V; e += W) {
-      const int d = e * 32 + lane * W;
-      uint32_t out[W / 2];
-#pragma unroll
-      for (int y = 0; y < W / 2; ++y) {
-        float2 v = l == 0.f ? make_float2(0.f, 0.f) : make_float2(acc[e + 2 * y] * fin, acc[e + 2 * y + 1] * fin);
-        if (a.gate && l != 0.f) {
-          const float2 s = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(a.gate + grow + d + 2 * y));
-          v.x = x_sigmoid(v.x, s.x);
-          v.y = x_sigmoid(v.y, s.y);
-        }
-        out[y] = pack_bf16x2(v.x, v.y);
-      }
-      if constexpr (W == 2)
-        *reinterpret_cast<uint32_t*>(a.out + orow + d) = out[0];
-      else
-        *reinterpret_cast<uint2*>(a.out + orow + d) = make_uint2(out[0], out[1]);
     }
   }
+  if (wpr > 1) {
+    __shared__ float s_o[8][V][32];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s_o[warp][e][lane] = acc[e];
+    __syncthreads();
+    if (sub > 0) return;
+    for (int w = 1; w < wpr; ++w)
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += s_o[warp + w * CW][e][lane];
+  }
+  if (!live) return;
+  // o = O 2^(M - m) / (2^11 l); without a visible key 0
+  const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
+  const float fin = l == 0.f ? 0.f : fast_exp2(fminf(vbase - base, 126.f)) / (l * P_SCALE);
+  uint32_t out[V / 2];
+#pragma unroll
+  for (int y = 0; y < V / 2; ++y) {
+    float2 v = l == 0.f ? make_float2(0.f, 0.f) : make_float2(acc[2 * y] * fin, acc[2 * y + 1] * fin);
+    if (a.gate && l != 0.f) {
+      const float2 s = unpack_bf16x2(y ? gate.y : gate.x);
+      v.x = x_sigmoid(v.x, s.x);
+      v.y = x_sigmoid(v.y, s.y);
+    }
+    out[y] = pack_bf16x2(v.x, v.y);
+  }
+  __nv_bfloat16* dst = a.out + (int64_t)(d.q0 + tok) * a.ldo + (int64_t)head * HD + col;
+  if constexpr (V == 4)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(out[0], out[1]);
+  else
+    *reinterpret_cast<uint32_t*>(dst) = out[0];
 }
 
 // Whether the requests' rows per key/value head fit the row tile of this file's kernel. Both kernels are right for any
@@ -794,8 +826,8 @@ static int row_tiles_of_8(int max_q, int group, int head_dim) {
   return 0;
 }
 
-// Bytes of scratch: the two request arrays, then the warps' partials per (item + CTA).
-static int64_t header_bytes(int n) { return ((int64_t)(n + 1) * 12 + 15) / 16 * 16; }
+// Bytes of scratch: the number of items, their descriptions, the warps' partials per (item + CTA).
+static int64_t header_bytes(int64_t items) { return 16 + (items * (int64_t)sizeof(Desc) + 15) / 16 * 16; }
 
 template <int HD, int NT>
 int64_t items_bound(int n, int64_t total_q, int hkv, int group) {
@@ -804,8 +836,8 @@ int64_t items_bound(int n, int64_t total_q, int hkv, int group) {
 template <int HD, int NT>
 int64_t workspace_bytes(int n, int64_t total_q, int hkv, int group, int ctas) {
   using C = Cfg<HD, NT>;
-  return header_bytes(n) +
-         (items_bound<HD, NT>(n, total_q, hkv, group) + ctas) * C::WARPS * C::PARTIAL * (int64_t)sizeof(float);
+  const int64_t items = items_bound<HD, NT>(n, total_q, hkv, group);
+  return header_bytes(items) + (items + ctas) * C::WARPS * C::PARTIAL * (int64_t)sizeof(float);
 }
 
 template <int HD, int NT>
@@ -816,12 +848,12 @@ int launch(Args a, const void* k_codes, const void* v_codes, uint8_t* ws, int64_
   if (dev < 0 || dev >= 64) return set_error(KD_ERR_ARGUMENT, "attention_cache: device index");
   const int ctas = num_sms(dev);
   const int64_t items = items_bound<HD, NT>(a.n, a.total_q, a.hkv, a.group);
-  if (items > 0x7fffffff - 4096) return set_error(KD_ERR_ARGUMENT, "attention_cache: too many row tiles");
+  if ((items + ctas) * C::WARPS > 0x7fffffff) return set_error(KD_ERR_ARGUMENT, "attention_cache: too many row tiles");
   if (ws_bytes < workspace_bytes<HD, NT>(a.n, a.total_q, a.hkv, a.group, ctas))
     return set_error(KD_ERR_ARGUMENT, "attention_cache: workspace smaller than kd_attention_cache_workspace");
-  a.tile_cu = reinterpret_cast<int64_t*>(ws);
-  a.item_cu = reinterpret_cast<int32_t*>(ws + 8 * (int64_t)(a.n + 1));
-  a.partials = reinterpret_cast<float*>(ws + header_bytes(a.n));
+  a.items = reinterpret_cast<int*>(ws);
+  a.descs = ws + 16;
+  a.partials = reinterpret_cast<float*>(ws + header_bytes(items));
   CUtensorMap mk, mv;
   const auto dt = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   const auto sw = HD == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
@@ -840,7 +872,7 @@ int launch(Args a, const void* k_codes, const void* v_codes, uint8_t* ws, int64_
   kernel<<<ctas, C::THREADS, C::SMEM, stream>>>(mk, mv, a);
   rc = record_cuda_error(cudaGetLastError(), "attention_cache: launch");
   if (rc) return rc;
-  return launch_after(join_kernel<HD, NT>, dim3((unsigned)items), 256, stream, a, ctas);
+  return launch_after(join_kernel<HD, NT>, dim3((unsigned)items, C::RT * HD / (HD <= 128 ? 8 * HD : 1024)), 256, stream, a, ctas);
 }
 
 // Calls f.template operator()<HD, NT>() for the kernel of a head dim and a number of 8-row tiles.
@@ -937,8 +969,8 @@ extern "C" int kd_attention_cache(const void* q, int64_t ldq, const void* k_code
   a.left = window_left > far ? far : window_left;
   a.right = window_right > far ? far : window_right;
   a.status = status;
-  a.tile_cu = nullptr;
-  a.item_cu = nullptr;
+  a.items = nullptr;
+  a.descs = nullptr;
   a.partials = nullptr;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512)

@@ -32,9 +32,8 @@ struct Args {
   int hq, hkv, group;
   float scale_log2;
   int left, right;
-  int64_t* tile_cu;   // [n + 1] few rows: key tiles of the requests before (of one key/value head)
-  int32_t* item_cu;   // [n + 1] few rows: row tiles of the requests before
-  void* splits;       // many rows: an item begun by a CTA and finished by later ones, per CTA
+  int* items;   // scratch of the kernel for few rows: the number of items
+  void* descs;  // what the joining launch needs of an item (few rows), or of one that several CTAs share (many)
   float* partials;
   int* status;
 };

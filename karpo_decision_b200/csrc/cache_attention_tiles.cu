@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
     if (lane == 0) {
       // the item this CTA begins and the next ones finish, for the launch that joins them; share p holds weight y when
       // floor(p total / np) <= y
-      Split* d = reinterpret_cast<Split*>(a.splits) + blockIdx.x;
+      Split* d = reinterpret_cast<Split*>(a.descs) + blockIdx.x;
       const bool split = lo < hi && begun.begin >= lo && begun.end > hi;
       if (split) {
         begun.last = (int)min((int64_t)np - 1, quotient(begun.end * np - 1, total));
@@ -935,7 +935,7 @@ __global__ void __launch_bounds__(2 * DV) join_tiles_kernel(Args a, int ctas) {
   using C = Cfg<HD, DV>;
   constexpr int GROUPS = 2 * DV / 8;  // threads that share a row
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the partials are there after this
-  const Split it = reinterpret_cast<const Split*>(a.splits)[blockIdx.x];
+  const Split it = reinterpret_cast<const Split*>(a.descs)[blockIdx.x];
   if ((int)blockIdx.y * 8 >= it.rows) return;
   const int first = blockIdx.x, n = it.last - first + 1;
   const int sub = threadIdx.x & 7, c4 = threadIdx.x >> 3, r = blockIdx.y * 8 + sub;
@@ -1040,7 +1040,7 @@ int launch(Args a, const void* k_codes, const uint8_t* v_codes, uint8_t* ws, int
   const int sms = num_sms(dev), ctas = min(sms * C::CTAS_PER_SM, JOIN_MOST);
   if (ws_bytes < workspace<HD, DV>(sms))
     return set_error(KD_ERR_ARGUMENT, "attention_cache: workspace smaller than kd_attention_cache_workspace");
-  a.splits = ws;
+  a.descs = ws;
   a.partials = reinterpret_cast<float*>(ws + header_bytes(ctas));
   static_assert(sizeof(Shared<HD, DV>) <= C::SMEM - C::TILES, "shared memory layout");
   auto kernel = row_tiles_kernel<HD, DV>;
