@@ -13,7 +13,8 @@
 // own, for what it costs beside them). A producer warp reads 32 tiles' table
 // entries and scales at a time and keeps a ring of 192 KB filled by TMA; eight warps take the tiles in turn (teams of
 // two or four for heads of 256 and 512, each warp a part of the tile's keys), each with a running maximum and sums of
-// its own, and leave a partial result per item that they met; a second launch joins them.
+// its own. Each warp leaves a partial result of an item that the CTA goes on from; of the CTA's last item the warps' sums
+// become one partial first. A second launch joins them.
 //
 // The products run on mma.sync.m16n8k16 in f16 with float32 sums, keys and values as the 16-row operand and the query
 // rows as the 8 columns: S^T = K Q^T, O^T = V^T P^T. Eight rows then cost half of what a 16-row query tile would, and
@@ -34,15 +35,14 @@ constexpr float P_EXPONENT = 11.f, P_SCALE = 2048.f;  // f16 probabilities hold 
 constexpr int ITEM_TILES = 8;  // an item's own cost (queries, its partial, the teams' drain) in key tiles: some 6,000 cycles
 
 // HD: head dim. NT: tiles of 8 query rows a warp holds. Registers bound both: a thread holds HD NT / 4 sums of the output
-// and the scores of its keys, for 32 rows of half of them at a time.
+// and the scores of its keys.
 template <int HD, int NT>
 struct Cfg {
   static constexpr int RT = 8 * NT;                // query rows of an item
   static constexpr int WARPS = 8, THREADS = 32 * (WARPS + 4);  // two warpgroups of consumers, one of producers
   static constexpr int KW = HD <= 64 ? 1 : HD == 128 ? (NT == 1 ? 2 : 1) : HD / 128;  // warps that share a tile by keys
   static constexpr int TEAMS = WARPS / KW;
-  static constexpr int PARTS = NT < 4 ? 1 : 2;    // steps in which a warp takes its keys
-  static constexpr int MT = BN / KW / PARTS / 16;  // 16-key tiles of a step
+  static constexpr int MT = BN / KW / 16;          // 16-key tiles of a warp
   static constexpr int BOX = HD < 128 ? HD : 128;  // bytes of a TMA box row (its swizzle span)
   static constexpr int CHUNKS = HD / BOX;
   static constexpr int TILE_BYTES = BN * HD;
@@ -163,6 +163,8 @@ KD_DEVICE void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// All consumers.
+KD_DEVICE void all_sync(int threads) { asm volatile("bar.sync 9, %0;" ::"r"(threads) : "memory"); }
 // The warps of one team.
 template <int KW>
 KD_DEVICE void team_sync(int team) {
@@ -186,7 +188,7 @@ KD_DEVICE uint32_t piece(int row, int c) {
 // An item, for the launch that joins its partials.
 struct Desc {
   int q0, h, r0, rows;  // the request's first query row, the key/value head, the item's first packed row and their number
-  int first, n;         // its partials, one behind another
+  int first, ctas;      // the first CTA's place among the partials, and the CTAs that met the item (0: it has no key tile)
 };
 
 // One tile's meta data beside its ring slot.
@@ -406,8 +408,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
       // the weight at the item's first tile is c.begin + ITEM_TILES * (its number + 1); the last tile's CTA as in the shares
       const int64_t v = c.begin + (int64_t)ITEM_TILES * (c.item + 1) + c.x.r.tiles;
       const int last = (int)quotient(v * np - 1, total);
-      descs[c.item] = Desc{c.x.r.q0, c.h, c.rt * RT, rows, (c.item + (int)blockIdx.x) * C::WARPS,
-                           (last - (int)blockIdx.x + 1) * C::WARPS};
+      descs[c.item] = Desc{c.x.r.q0, c.h, c.rt * RT, rows, c.item + (int)blockIdx.x, last - (int)blockIdx.x + 1};
     }
     if ((int64_t)at + lo < stop) {
       // ---- queries: f16, scaled to the row's largest magnitude, in the order of the B fragments; RT / KW rows a warp, LPR
@@ -482,11 +483,8 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
       const TileInfo ti = info[slot];
       const uint32_t sk = ring + slot * C::SLOT_BYTES, sv = sk + C::TILE_BYTES;
       const int tile0 = (c.x.r.first + (int)((int64_t)at + lo - c.begin)) * BN;
-#pragma unroll 1
-      for (int part = 0; part < C::PARTS; ++part) {
-        const int key_off = part_of * (BN / C::KW) + part * (16 * MT);  // the step's first key within the tile
-        const int key0 = tile0 + key_off;
-        if (!ti.live || key0 >= lk) break;
+      const int key_off = part_of * (16 * MT), key0 = tile0 + key_off;  // the warp's first key in the tile, in the request
+      if (ti.live && key0 < lk) {
         met = true;
         // ---- S^T = K Q^T: 16 keys a tile; a thread holds keys row_g and row_g + 8 of its rows 2 t4 and 2 t4 + 1
         float s[MT][NT][4];
@@ -647,31 +645,94 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[slot]);
     }
-    // ---- the warp's partial of this fragment: item + CTA number its place (both only grow along the list)
-    float* part = a.partials + ((int64_t)(c.item + (int)blockIdx.x) * C::WARPS + warp) * C::PARTIAL;
+    // ---- the partials of this fragment: item + CTA number their place (both only grow along the list)
+    float* place = a.partials + (int64_t)(c.item + (int)blockIdx.x) * C::WARPS * C::PARTIAL;
+    float sum[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int rr = nt * 8 + 2 * t4 + u;
-        float sum = l[nt][u];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        if (rr < rows) {
-          if (row_g == 0) {
-            float* st = part + RT * HD + 3 * rr;
-            st[0] = m[nt][u];
-            st[1] = big[nt][u];
-            st[2] = sum;
-          }
-          if (met) {
+        float x = l[nt][u];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        sum[nt][u] = x + __shfl_xor_sync(0xffffffffu, x, 16);
+      }
+    if (stop < hi) {
+      // more items follow: each warp leaves its own and goes on
+      float* part = place + warp * C::PARTIAL;
 #pragma unroll
-            for (int x = 0; x < HD / 16; ++x)
-              *reinterpret_cast<float2*>(part + rr * HD + 16 * x + 2 * row_g) = make_float2(o[x][nt][u], o[x][nt][2 + u]);
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int rr = nt * 8 + 2 * t4 + u;
+          if (rr < rows) {
+            if (row_g == 0) {
+              float* st = part + RT * HD + 3 * rr;
+              st[0] = m[nt][u];
+              st[1] = big[nt][u];
+              st[2] = sum[nt][u];
+            }
+            if (met) {
+#pragma unroll
+              for (int x = 0; x < HD / 16; ++x)
+                *reinterpret_cast<float2*>(part + rr * HD + 16 * x + 2 * row_g) = make_float2(o[x][nt][u], o[x][nt][2 + u]);
+            }
           }
         }
+    } else {
+      // the CTA's last: the warps' sums become one partial, in the ring, which every tile has left
+      constexpr int LD = HD + 8;  // floats between rows
+      static_assert(C::WARPS * RT * (LD + 3) * 4 <= SLOTS * C::SLOT_BYTES, "the ring holds the warps' sums");
+      float* all = reinterpret_cast<float*>(smem);
+      float* stats = all + C::WARPS * RT * LD;  // [3][WARPS][RT]
+      all_sync(32 * C::WARPS);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int rr = nt * 8 + 2 * t4 + u;
+          if (row_g == 0) {
+            stats[warp * RT + rr] = m[nt][u];
+            stats[(C::WARPS + warp) * RT + rr] = big[nt][u];
+            stats[(2 * C::WARPS + warp) * RT + rr] = sum[nt][u];
+          }
+#pragma unroll
+          for (int x = 0; x < HD / 16; ++x)
+            *reinterpret_cast<float2*>(all + (warp * RT + rr) * LD + 16 * x + 2 * row_g) =
+                make_float2(o[x][nt][u], o[x][nt][2 + u]);
+        }
+      all_sync(32 * C::WARPS);
+      for (int i = tid; i < rows * (HD / 4); i += 32 * C::WARPS) {
+        const int rr = i / (HD / 4), d = (i - rr * (HD / 4)) * 4;
+        float mm = -INFINITY, bb = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < C::WARPS; ++w) {
+          mm = fmaxf(mm, stats[w * RT + rr]);
+          bb = fmaxf(bb, stats[(C::WARPS + w) * RT + rr]);
+        }
+        const float base = mm == -INFINITY ? 0.f : mm, vbase = bb == -INFINITY ? 0.f : bb;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float ll = 0.f;
+#pragma unroll
+        for (int w = 0; w < C::WARPS; ++w) {
+          ll += stats[(2 * C::WARPS + w) * RT + rr] * fast_exp2(stats[w * RT + rr] - base);
+          const float f = fast_exp2(stats[(C::WARPS + w) * RT + rr] - vbase);
+          const float4 y = *reinterpret_cast<const float4*>(all + (w * RT + rr) * LD + d);
+          acc.x += y.x * f;
+          acc.y += y.y * f;
+          acc.z += y.z * f;
+          acc.w += y.w * f;
+        }
+        *reinterpret_cast<float4*>(place + rr * HD + d) = acc;
+        if (d < 32) {  // the row's statistics, and the other warps' places marked empty, by eight threads
+          const int w = d / 4;
+          float* st = place + w * C::PARTIAL + RT * HD + 3 * rr;
+          st[0] = w ? -INFINITY : mm;
+          st[1] = w ? -INFINITY : bb;
+          st[2] = w ? 0.f : ll;
+        }
       }
+    }
     g = stop;
     c.seek(a, g);
   }
@@ -690,8 +751,12 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
   const Desc d = reinterpret_cast<const Desc*>(a.descs)[blockIdx.x];
   const int r0 = blockIdx.y * RB;
   if ((int)blockIdx.x >= items || r0 >= d.rows) return;
-  const int n = d.n;
-  const float* part = a.partials + (int64_t)d.first * C::PARTIAL;
+  // Every CTA but the last left one partial (it went on to no other item), the last one eight, if only one that counts.
+  const int n = d.ctas ? d.ctas - 1 + C::WARPS : 0;
+  auto place = [&](int q) -> const float* {
+    const int c = min(q, d.ctas - 1);
+    return a.partials + ((int64_t)(d.first + c) * C::WARPS + (q - c)) * C::PARTIAL;
+  };
   const int here = min(RB, d.rows - r0);
   const int wpr = here * 2 > RB ? 1 : here * 4 > RB ? 2 : here * 8 > RB ? 4 : 8;  // warps of a row's columns
   const int unit = warp / CW, col = (warp % CW) * 128 + lane * V;
@@ -710,12 +775,11 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
   if (live) {
-    const float* stats = part + RT * HD + 3 * row;
     for (int q0 = lane; q0 < n; q0 += 128) {  // four loads in flight
       float x[4], y[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float* st = stats + (int64_t)(q0 + 32 * u) * C::PARTIAL;
+        const float* st = place(min(q0 + 32 * u, n - 1)) + RT * HD + 3 * row;
         x[u] = q0 + 32 * u < n ? st[0] : -INFINITY;
         y[u] = q0 + 32 * u < n ? st[1] : -INFINITY;
       }
@@ -735,7 +799,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
       float x[4], y[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float* st = stats + (int64_t)(q0 + 32 * u) * C::PARTIAL;
+        const float* st = place(min(q0 + 32 * u, n - 1)) + RT * HD + 3 * row;
         x[u] = q0 + 32 * u < n ? st[0] : -INFINITY;
         y[u] = q0 + 32 * u < n ? st[2] : 0.f;
       }
@@ -748,7 +812,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
     for (int k0 = 0; k0 < mine; k0 += 32) {
       float f = -1.f;  // < 0: the warp that left it met no key of the row (its sums may hold anything)
       if (k0 + lane < mine) {
-        const float* st = stats + (int64_t)(sub + (k0 + lane) * wpr) * C::PARTIAL;
+        const float* st = place(sub + (k0 + lane) * wpr) + RT * HD + 3 * row;
         if (st[1] != -INFINITY || st[2] != 0.f) f = fast_exp2(st[1] - vbase);
       }
       const int some = min(32, mine - k0);
@@ -761,7 +825,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
           if (k1 + q >= some) w[q] = -1.f;
           y[q] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (!(w[q] < 0.f)) {
-            const float* src = part + (int64_t)(sub + (k0 + k1 + q) * wpr) * C::PARTIAL + row * HD + col;
+            const float* src = place(sub + (k0 + k1 + q) * wpr) + row * HD + col;
             if constexpr (V == 4) {
               y[q] = *reinterpret_cast<const float4*>(src);
             } else {
@@ -816,14 +880,13 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
     *reinterpret_cast<uint32_t*>(dst) = out[0];
 }
 
-// Whether the requests' rows per key/value head fit the row tile of this file's kernel. Both kernels are right for any
-// rows.
+// The 8-row tiles of this file's kernel for these requests, 0 for the kernel with 128-row tiles; both are right for any
+// rows. Measured (us, this file's / the other, 8 requests of 16,384 tokens, 8 key/value heads): head 64, 16 rows 54 / 63,
+// 24 rows 96 / 64; head 128, 16 rows 66 / 79; head 256, 16 rows 113 / 141. Heads of 512 hold 8 rows; 16 rows read the
+// codes twice, the second time from L2.
 static int row_tiles_of_8(int max_q, int group, int head_dim) {
   const int64_t rows = (int64_t)max_q * group;
-  if (rows <= 8) return 1;
-  if (rows <= 16 && head_dim <= 256) return 2;
-  if (rows <= 32 && head_dim == 64) return 4;
-  return 0;
+  return rows > 16 ? 0 : rows <= 8 || head_dim == 512 ? 1 : 2;
 }
 
 // Bytes of scratch: the number of items, their descriptions, the warps' partials per (item + CTA).
@@ -875,22 +938,16 @@ int launch(Args a, const void* k_codes, const void* v_codes, uint8_t* ws, int64_
   return launch_after(join_kernel<HD, NT>, dim3((unsigned)items, C::RT * HD / (HD <= 128 ? 8 * HD : 1024)), 256, stream, a, ctas);
 }
 
-// Calls f.template operator()<HD, NT>() for the kernel of a head dim and a number of 8-row tiles.
+// f(head dim, 8-row tiles) with both as constants.
 template <typename F>
 auto with_kernel(int head_dim, int nt, F f) {
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
   switch (head_dim) {
-    case 64:
-      return nt == 1 ? f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{})
-             : nt == 2 ? f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{})
-                       : f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
-    case 128:
-      return nt == 1 ? f(std::integral_constant<int, 128>{}, std::integral_constant<int, 1>{})
-                     : f(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{});
-    case 256:
-      return nt == 1 ? f(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{})
-                     : f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
-    default:
-      return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 1>{});
+    case 64: return nt == 1 ? f(std::integral_constant<int, 64>{}, one) : f(std::integral_constant<int, 64>{}, two);
+    case 128: return nt == 1 ? f(std::integral_constant<int, 128>{}, one) : f(std::integral_constant<int, 128>{}, two);
+    case 256: return nt == 1 ? f(std::integral_constant<int, 256>{}, one) : f(std::integral_constant<int, 256>{}, two);
+    default: return f(std::integral_constant<int, 512>{}, one);
   }
 }
 

@@ -54,7 +54,7 @@ struct Cfg {
   static constexpr int QS_BYTES = Q_TMEM ? 0 : 2 * Q_BYTES;  // queries in shared memory
   static constexpr int KST = HD <= 128 ? 3 : HD == 256 ? 4 : 2, VST = HD <= 128 ? 3 : HD == 256 ? 4 : 1;  // ring stages
   static constexpr int TILES = QS_BYTES + KST * K_BYTES + VST * V_BYTES + (Q_TMEM ? BM * ROW : 0);  // of 1,024 bytes
-  static constexpr int SMEM = TILES + 3072;
+  static constexpr int SMEM = TILES + 3 * 1024;
   static constexpr int CTAS_PER_SM = (2 * (SMEM + 1024) <= 227 * 1024 && 2 * TMEM_COLS <= 512) ? 2 : 1;
   static constexpr int SOFT = 4;  // softmax warps, a thread a row
   static constexpr int CONV_WARPS = HD <= 128 ? 2 : 4;
