@@ -74,14 +74,14 @@ def store(x, other, cu, slots, codes, scale, is_key):
 
 def attention(q, k, v, ks, vs, table, cu, kv_len, scale, window, gate=None):
     """(out, spread, size): the definition in float64; per output the sum of p |v| / sum of p (times the gate), which
-    bounds what relative errors of the probabilities do to it; the largest sum |q k| * scale of a visible pair. ``k``,
-    ``v``: codes' values; rows outside every request are NaN."""
+    bounds what relative errors of the probabilities do to it; the largest sum |q k| * scale of a visible pair and the
+    largest max |q| * sum |k| * scale. ``k``, ``v``: codes' values; rows outside every request are NaN."""
     tq, hq, hd = q.shape
     hkv = k.shape[1]
     group = hq // hkv
     out = torch.full((tq, hq, hd), math.nan, dtype=torch.float64, device=q.device)
     spread = torch.zeros_like(out)
-    size = 0.0
+    size = reach = 0.0
     blocks = k.shape[0]
     for i in range(len(kv_len)):
         a, b, lk = cu[i], cu[i + 1], kv_len[i]
@@ -110,6 +110,8 @@ def attention(q, k, v, ks, vs, table, cu, kv_len, scale, window, gate=None):
             kk = k[ids, g, pos % BLOCK] * ks[ids, g].double()[:, None]
             vv = v[ids, g, pos % BLOCK] * vs[ids, g].double()[:, None]
             size = max(size, float((q[a:b, h].double().abs() @ kk.abs().T * scale)[see].max()))
+            top = q[a:b, h].double().abs().amax(1, keepdim=True)
+            reach = max(reach, float((top * kk.abs().sum(1) * scale)[see].max()))
             x = torch.where(see, q[a:b, h].double() @ kk.T * scale, -math.inf)
             x = torch.where(some[:, None], x, 0.0)
             p = torch.softmax(x, -1)
@@ -122,4 +124,4 @@ def attention(q, k, v, ks, vs, table, cu, kv_len, scale, window, gate=None):
         s = torch.sigmoid(gate.double())
         live = spread > 0
         out, spread = torch.where(live, out * s, out), spread * s
-    return out, spread, size
+    return out, spread, (size, reach)

@@ -239,17 +239,19 @@ def make(lens, new, hq, hkv, hd, seed=0, spread=1.0, pad=0):
 
 
 def tolerance(want, spread, size, hd, keys):
-    """What the definition's value may move by (derived, not fitted); spread = sum p |v| / sum p, size = the largest
-    sum |q k| * scale:
+    """What the definition's value may move by (derived, not fitted); spread = sum p |v| / sum p, size = (the largest
+    sum |q k| * scale, the largest max |q| * sum |k| * scale):
     - the output's rounding to bf16: 2^-8 |o|;
     - the probabilities' rounding to f16: 2^-11 relative each, so 2^-11 spread; those below f16's normal numbers, 2^-29
       of the row's largest scaled probability, lose at most 2^-40 of it each: keys * 2^-40 of 448 block units, which the
       largest one's own term in spread covers unless its codes are all under 2^-6;
-    - a score's error d moves every probability by at most 2 d relative: d <= (hd / 8) 2^-23 size for the products'
-      float32 sums (hd / 16 products of 16 terms, each added with an error of one unit) and 2^-22 size for its scaling,
-      the subtraction of the maximum and the exponential;
+    - a score's error d moves every probability by at most 2 d relative: d <= (hd / 8) 2^-23 size[0] for the products'
+      float32 sums (hd / 16 products of 16 terms, each added with an error of one unit), 2^-22 size[0] for its scaling,
+      the subtraction of the maximum and the exponential, and 2^-17 size[1] for the queries: as two e4m3 values of a row
+      scaled to more than 224, an element is off by half of e4m3's least step, 2^-10 (one f16 value of a row scaled to
+      at least 1 is off by 2^-25 at most);
     - the float32 sums over keys: keys / 16 additions of 2^-23 relative at most, in numerator and denominator."""
-    d = (hd / 8 * 2.0 ** -23 + 2.0 ** -22) * size
+    d = (hd / 8 * 2.0 ** -23 + 2.0 ** -22) * size[0] + 2.0 ** -17 * size[1]
     return 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -14 + keys / 8 * 2.0 ** -23 + 2 * d) * spread + 1e-30
 
 
@@ -303,6 +305,25 @@ def test_attention_of_many_requests():
     lens = g.integers(1, 400, 300).tolist()
     check_attention(lens, [1] * 300, 8, 4, 64)
     check_attention(lens, [min(n, 3) for n in lens], 8, 4, 128, window=(100, 0))
+
+
+@pytest.mark.parametrize("hd,hq,hkv", [(64, 8, 8), (128, 8, 4), (256, 8, 4), (512, 8, 2)])
+def test_attention_of_long_states_with_few_rows(hd, hq, hkv):
+    """Some hundred tiles a block: every slot of its ring is used many times over, by warps that run ahead of one another.
+    Two runs are equal bit by bit."""
+    lens = [40000, 1, 52345, 30017, 64, 47111, 38000, 20000]
+    first = check_attention(lens, [1] * 8, hq, hkv, hd)
+    assert torch.equal(first, check_attention(lens, [1] * 8, hq, hkv, hd))
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+def test_attention_of_more_requests_than_threads(rows):
+    """900 requests, empty ones and ones without new rows among them, single tokens and rows for the 128-row tiles."""
+    g = np.random.default_rng(4)
+    lens = g.integers(0, 150, 900).tolist()
+    new = [min(n, int(r)) for n, r in zip(lens, g.integers(0, rows + 1, 900))]
+    check_attention(lens, new, 4, 2, 64)
+    check_attention(lens, new, 4, 4, 128, window=(30, 0), gated=True)
 
 
 def test_rows_that_see_nothing_are_zero():
