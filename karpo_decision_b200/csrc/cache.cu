@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(TABLE_THREADS) release_kernel(ReleaseArgs a) {
 
 // ------------------------------------------------------------------------------------------------ the write
 
-constexpr int STORE_THREADS = 256;
+constexpr int store_threads(int head_dim) { return 2 * head_dim; }  // a thread holds 4 pieces of k and of v
 constexpr int E_MIN = -100, E_MAX = 120;  // the scales' exponents (E_MAX holds the largest bf16 value)
 
 // The least exponent e with a 2^-e <= 448 = 1.75 * 2^8, within [E_MIN, E_MAX]; a >= 0, finite.
@@ -262,17 +262,47 @@ KD_DEVICE float2 from_e4m3x2(uint32_t codes) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+KD_DEVICE uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+// The larger of the even and of the odd elements' magnitudes.
+KD_DEVICE uint32_t largest(const uint4& x) {
+  return max_u16x2(max_u16x2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), max_u16x2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+}
+// Raises `top` to the largest finite magnitude's pattern; whether there is a NaN.
+KD_DEVICE bool finite_max(const uint4& x, uint32_t& top) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t y = (w[e / 2] >> (16 * (e & 1))) & 0x7fffu;
+    nan |= y > 0x7f80u;
+    top = max(top, y < 0x7f80u ? y : 0u);
+  }
+  return nan;
+}
+
 // One CTA writes the new rows of one block for one key/value head: loads them (16 bytes a thread and step, all loads in
 // flight at once), takes the largest finite magnitude of the keys and of the values, and writes codes of 8 bytes a
 // thread, so that a row of 128 codes is one line. A block whose first new row is not its first row keeps the larger of
 // its old scale and the new rows' own; where it grows, the old codes are brought to it (code * 2^(old - new), rounded
 // to nearest even). Requests' blocks are laid over the grid by f(i) = cu[i] / 64 + 2 i, which leaves every request
 // enough places (its rows touch at most rows / 64 + 2 blocks) without a scan; each warp finds its request by probing 32
-// requests at a time. Bound by the reads of k and v; the smallest launches by its chain of dependent loads.
+// requests at a time.
+//
+// Bound by the reads of k and v, next to it by the instructions per element (magnitudes as two 16-bit integers to a word,
+// elements one by one only where one is not finite: 46.5 -> 38 us), then by the loads in flight: 1,280 threads an SM at 48
+// registers (38 -> 35.9 us; at 40 they spill, 40 us). 48,000 rows of 8 heads of 128: 35.9 us, 5.72 TB/s; one CTA with
+// several heads one after another, the next one's loads in flight, was slower (39 us), as were neighbouring heads first.
+// The smallest launches are a chain of dependent loads, 5.6 us.
 template <int HD>
-__global__ void __launch_bounds__(STORE_THREADS) store_kernel(StoreArgs a) {
+__global__ void __launch_bounds__(store_threads(HD), 1280 / store_threads(HD))
+    store_kernel(StoreArgs a) {
+  constexpr int THREADS = store_threads(HD);
   constexpr int VEC = HD / 8;                            // 8-element pieces of a row
-  constexpr int STEPS = BLOCK * VEC / STORE_THREADS;     // pieces a thread holds of k and of v
+  constexpr int STEPS = BLOCK * VEC / THREADS;     // pieces a thread holds of k and of v
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const int64_t place = blockIdx.x;
   // the last request i with f(i) <= place
@@ -303,10 +333,16 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(StoreArgs a) {
   const int live = (int)min((int64_t)(BLOCK - off), end - row0);
   const int head = blockIdx.y;
 
+  const int64_t at = block * a.heads + head;
+  float old_scale[2] = {};
+  if (off > 0) {
+    old_scale[0] = a.k_scale[at];
+    old_scale[1] = a.v_scale[at];
+  }
   uint4 kx[STEPS], vx[STEPS];
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
-    const int p = s * STORE_THREADS + threadIdx.x, r = p / VEC, c = (p % VEC) * 8;
+    const int p = s * THREADS + threadIdx.x, r = p / VEC, c = (p % VEC) * 8;
     if (r < live) {
       kx[s] = *reinterpret_cast<const uint4*>(a.k + (row0 + r) * a.ldk + head * HD + c);
       vx[s] = *reinterpret_cast<const uint4*>(a.v + (row0 + r) * a.ldv + head * HD + c);
@@ -314,25 +350,27 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(StoreArgs a) {
       kx[s] = vx[s] = make_uint4(0, 0, 0, 0);
     }
   }
-  __shared__ float s_max[2][STORE_THREADS / 32];
+  __shared__ float s_max[2][THREADS / 32];
   __shared__ unsigned s_nan[2];  // bit r: row r holds a NaN in its key or value
   if (threadIdx.x < 2) s_nan[threadIdx.x] = 0;
   __syncthreads();
-  // Magnitudes as bf16 bit patterns (they order as integers); inf and NaN are at or above 0x7f80.
+  // Magnitudes as bf16 bit patterns (they order as integers), two to a word; inf and NaN are at or above 0x7f80.
   uint32_t mk = 0, mv = 0;
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
-    const uint32_t kw[4] = {kx[s].x, kx[s].y, kx[s].z, kx[s].w}, vw[4] = {vx[s].x, vx[s].y, vx[s].z, vx[s].w};
-    bool nan = false;
+    mk = max_u16x2(mk, largest(kx[s]));
+    mv = max_u16x2(mv, largest(vx[s]));
+  }
+  mk = max(mk & 0xffffu, mk >> 16);
+  mv = max(mv & 0xffffu, mv >> 16);
+  if (max(mk, mv) >= 0x7f80u) {  // element by element: the largest finite one, and the rows with a NaN
+    mk = mv = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t x = (kw[e / 2] >> (16 * (e & 1))) & 0x7fffu, y = (vw[e / 2] >> (16 * (e & 1))) & 0x7fffu;
-      nan |= x > 0x7f80u || y > 0x7f80u;
-      mk = max(mk, x < 0x7f80u ? x : 0u);
-      mv = max(mv, y < 0x7f80u ? y : 0u);
+    for (int s = 0; s < STEPS; ++s) {
+      const bool nan_k = finite_max(kx[s], mk), nan_v = finite_max(vx[s], mv);
+      const int r = (s * THREADS + (int)threadIdx.x) / VEC;
+      if (nan_k || nan_v) atomicOr(&s_nan[r / 32], 1u << (r & 31));
     }
-    const int r = (s * STORE_THREADS + (int)threadIdx.x) / VEC;
-    if (nan) atomicOr(&s_nan[r / 32], 1u << (r & 31));
   }
   mk = __reduce_max_sync(0xffffffffu, mk);
   mv = __reduce_max_sync(0xffffffffu, mv);
@@ -343,21 +381,20 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(StoreArgs a) {
   __syncthreads();
   float ak = 0.f, av = 0.f;
 #pragma unroll
-  for (int w = 0; w < STORE_THREADS / 32; ++w) {
+  for (int w = 0; w < THREADS / 32; ++w) {
     ak = fmaxf(ak, s_max[0][w]);
     av = fmaxf(av, s_max[1][w]);
   }
-  const int64_t at = block * a.heads + head;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     float* scale = which ? a.v_scale : a.k_scale;
     uint8_t* codes = (which ? a.v_codes : a.k_codes) + at * BLOCK * HD;
     int e = scale_exponent(which ? av : ak);
     if (off > 0) {
-      const int old = min(max((int)((__float_as_uint(scale[at]) >> 23) & 255u) - 127, E_MIN), E_MAX);
+      const int old = min(max((int)((__float_as_uint(old_scale[which]) >> 23) & 255u) - 127, E_MIN), E_MAX);
       if (e > old) {
         const float f = power_of_two(max(old - e, -126));
-        for (int p = threadIdx.x; p < off * HD / 4; p += STORE_THREADS) {
+        for (int p = threadIdx.x; p < off * HD / 4; p += THREADS) {
           uint32_t w = reinterpret_cast<uint32_t*>(codes)[p];
           const float2 x = from_e4m3x2(w), y = from_e4m3x2(w >> 16);
           reinterpret_cast<uint32_t*>(codes)[p] = e4m3x2(x.x * f, x.y * f) | (e4m3x2(y.x * f, y.y * f) << 16);
@@ -365,21 +402,20 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(StoreArgs a) {
       } else {
         e = old;
       }
-      __syncthreads();  // every thread has read the old scale
     }
     if (threadIdx.x == 0) scale[at] = power_of_two(e);
     const float inv = power_of_two(-e);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      const int p = s * STORE_THREADS + threadIdx.x, r = p / VEC, c = (p % VEC) * 8;
+      const int p = s * THREADS + threadIdx.x, r = p / VEC, c = (p % VEC) * 8;
       if (r >= live) continue;
       const uint4 x4 = which ? vx[s] : kx[s];
       const uint32_t w[4] = {x4.x, x4.y, x4.z, x4.w};
       uint32_t o[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float2 x = unpack_bf16x2(w[q]);
-        o[q] = e4m3x2(x.x * inv, x.y * inv);
+        const float2 x = __fmul2_rn(unpack_bf16x2(w[q]), make_float2(inv, inv));
+        o[q] = e4m3x2(x.x, x.y);
       }
       uint2 out = make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
       // A token with a NaN anywhere is a NaN key and a zero value: its scores are NaN wherever it is seen and its
@@ -475,16 +511,16 @@ extern "C" int kd_kv_store_e4m3(const void* k, int64_t ldk, const void* v, int64
   const dim3 grid((unsigned)(rows / kv::BLOCK + 2 * (int64_t)num_requests), num_heads_kv);
   switch (head_dim) {
     case 64:
-      kv::store_kernel<64><<<grid, kv::STORE_THREADS, 0, stream>>>(a);
+      kv::store_kernel<64><<<grid, kv::store_threads(64), 0, stream>>>(a);
       break;
     case 128:
-      kv::store_kernel<128><<<grid, kv::STORE_THREADS, 0, stream>>>(a);
+      kv::store_kernel<128><<<grid, kv::store_threads(128), 0, stream>>>(a);
       break;
     case 256:
-      kv::store_kernel<256><<<grid, kv::STORE_THREADS, 0, stream>>>(a);
+      kv::store_kernel<256><<<grid, kv::store_threads(256), 0, stream>>>(a);
       break;
     default:
-      kv::store_kernel<512><<<grid, kv::STORE_THREADS, 0, stream>>>(a);
+      kv::store_kernel<512><<<grid, kv::store_threads(512), 0, stream>>>(a);
   }
   return record_cuda_error(cudaGetLastError(), "kv_store: launch");
 }
