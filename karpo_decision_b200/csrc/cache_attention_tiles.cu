@@ -196,6 +196,15 @@ struct Work {
 struct Split {
   int64_t begin, end, total;  // its weights, and the launch's
   int q0, h, slice, r0, rows, tiles, last, np;  // `last`: the CTA that finishes it
+  uint32_t left;  // bit p: the p-th CTA from the beginning one leaves a partial; for the first 32
+  int pad;
+  // Whether the p-th CTA from CTA `first` has any of the item's key tiles.
+  KD_DEVICE bool leaves(int first, int p) const {
+    const int64_t x0 = quotient(total * (first + p), np), x1 = quotient(total * (first + p + 1), np);
+    int t0, t1;
+    portion(begin, end, max(x0, begin), min(x1, end), tiles, t0, t1);
+    return t0 < t1;
+  }
 };
 
 // block * heads + head of an item's tile j, < 0: absent. Roles look up 32 tiles at a time, one a lane.
@@ -399,7 +408,7 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         const bool whole = x0 == it.begin && x1 == it.end;
         if (it.end > hi) {
           begun = Split{it.begin, it.end, total, it.s.q0, it.h, it.slice, it.tile * 128,
-                        (int)min((int64_t)128, (int64_t)it.s.lq * a.group - it.tile * 128), v.n, 0, np};
+                        (int)min((int64_t)128, (int64_t)it.s.lq * a.group - it.tile * 128), v.n, 0, np, 0, 0};
         }
         if (whole || t0 < t1) {
           w.q0 = it.s.q0;
@@ -461,16 +470,21 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
       }
       g += w.n;
     }
-    if (lane == 0) {
+    {
       // the item this CTA begins and the next ones finish, for the launch that joins them; share p holds weight y when
       // floor(p total / np) <= y
       Split* d = reinterpret_cast<Split*>(a.descs) + blockIdx.x;
       const bool split = lo < hi && begun.begin >= lo && begun.end > hi;
       if (split) {
         begun.last = (int)min((int64_t)np - 1, quotient(begun.end * np - 1, total));
-        *d = begun;
-      } else {
-        d->rows = 0;
+        const bool leaves = lane <= begun.last - (int)blockIdx.x && begun.leaves(blockIdx.x, lane);
+        begun.left = __ballot_sync(0xffffffffu, leaves);
+      }
+      if (lane == 0) {
+        if (split)
+          *d = begun;
+        else
+          d->rows = 0;
       }
     }
     if (!ok && lane == 0) {
@@ -934,10 +948,14 @@ done:
   }
 }
 
-// Joins the partials of the item that CTA blockIdx.x began and later ones finished, 8 of its 128 rows a block. The
-// partials' statistics first, all at once, to a weight for each; then a thread sums 4 columns of a row over the partials
-// in key order, eight loads in flight.
+// Joins the partials of the item that CTA blockIdx.x began and later ones finished, 8 of its 128 rows a block, a thread 4
+// columns of a row. Up to JOIN_FEW partials (what a pack of requests leaves): every thread reads its row's statistics and
+// its columns of four partials at once, in key order, with a running maximum; nothing waits for another thread, and the
+// beginning CTA has worked out which shares hold tiles (8 requests of 20 to 200 rows: 162 -> 150 us with it). More (one
+// long state): the statistics first, shared out among the threads, to a weight for each partial, then the columns, eight
+// loads in flight.
 constexpr int JOIN_MOST = 320;  // partials of an item: at most the CTAs
+constexpr int JOIN_FEW = 16;
 template <int HD, int DV>
 __global__ void __launch_bounds__(2 * DV) join_tiles_kernel(Args a, int ctas) {
   using C = Cfg<HD, DV>;
@@ -948,79 +966,121 @@ __global__ void __launch_bounds__(2 * DV) join_tiles_kernel(Args a, int ctas) {
   const int first = blockIdx.x, n = it.last - first + 1;
   const int sub = threadIdx.x & 7, c4 = threadIdx.x >> 3, r = blockIdx.y * 8 + sub;
   const bool live = r < it.rows;
-  __shared__ float s_w[JOIN_MOST][8];
-  __shared__ float s_red[3][2 * DV / 32][8];
-  __shared__ int s_slot[JOIN_MOST];  // < 0: the share holds none of the item's tiles
-  for (int p = threadIdx.x; p < n; p += 2 * DV) {
-    const int64_t x0 = quotient(it.total * (first + p), it.np), x1 = quotient(it.total * (first + p + 1), it.np);
-    int t0, t1;
-    portion(it.begin, it.end, max(x0, it.begin), min(x1, it.end), it.tiles, t0, t1);
-    s_slot[p] = t0 < t1 ? 2 * (first + p) + (p == 0 ? 1 : 0) : -1;
-  }
-  __syncthreads();
-  float m = -INFINITY, big = -INFINITY;
-  for (int p = c4; p < n; p += GROUPS) {
-    const int slot = s_slot[p];
-    if (slot < 0 || !live) continue;
-    const float* st = a.partials + (int64_t)slot * C::PARTIAL + C::BM * DV + r;
-    m = fmaxf(m, st[0]);
-    big = fmaxf(big, st[128]);
-  }
-  auto across = [&](float v, int which, auto op) -> float {  // over the threads of a row
-    v = op(v, __shfl_xor_sync(0xffffffffu, v, 8));
-    v = op(v, __shfl_xor_sync(0xffffffffu, v, 16));
-    if ((threadIdx.x & 31) < 8) s_red[which][threadIdx.x / 32][sub] = v;
-    __syncthreads();
-    v = s_red[which][0][sub];
-#pragma unroll
-    for (int q = 1; q < 2 * DV / 32; ++q) v = op(v, s_red[which][q][sub]);
-    return v;
-  };
-  m = across(m, 0, [](float x, float y) { return fmaxf(x, y); });
-  big = across(big, 1, [](float x, float y) { return fmaxf(x, y); });
-  const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
-  float l = 0.f;
-  for (int p = c4; p < n; p += GROUPS) {
-    const int slot = s_slot[p];
-    float f = -1.f;
-    if (slot >= 0 && live) {
-      const float* st = a.partials + (int64_t)slot * C::PARTIAL + C::BM * DV + r;
-      l += st[256] * fast_exp2(st[0] - base);
-      if (st[128] != -INFINITY || st[256] != 0.f) f = fast_exp2(st[128] - vbase);
-    }
-    s_w[p][sub] = f;  // < 0: no key of the row (its sums may hold anything)
-  }
-  l = across(l, 2, [](float x, float y) { return x + y; });
-  if (!live) return;
+  const int gr = it.r0 + r, tok = gr / a.group;
+  const int64_t row = it.q0 + tok, col = (int64_t)(it.h * a.group + gr - tok * a.group) * HD + it.slice * DV + 4 * c4;
+  uint2 gate = make_uint2(0, 0);
+  if (a.gate && live) gate = *reinterpret_cast<const uint2*>(a.gate + row * a.ldg + col);
+  float m = -INFINITY, big = -INFINITY, l = 0.f, base = 0.f, vbase = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = 0; p0 < n; p0 += 8) {
-    float4 y[8];
-    float f[8];
+  if (n <= JOIN_FEW) {
+    for (int p0 = 0; p0 < n; p0 += 4) {
+      float x[4], y[4], z[4];
+      float4 v[4];
+      float mm = m, bb = big;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      f[q] = p0 + q < n ? s_w[p0 + q][sub] : -1.f;
-      y[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (f[q] >= 0.f || f[q] != f[q])
-        y[q] = *reinterpret_cast<const float4*>(a.partials + (int64_t)s_slot[p0 + q] * C::PARTIAL + (c4 * 128 + r) * 4);
+      for (int q = 0; q < 4; ++q) {
+        x[q] = y[q] = -INFINITY;
+        z[q] = 0.f;
+        v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (((it.left >> (p0 + q)) & 1u) && live) {
+          const float* part = a.partials + (int64_t)(2 * (first + p0 + q) + (p0 + q == 0 ? 1 : 0)) * C::PARTIAL;
+          const float* st = part + C::BM * DV + r;
+          x[q] = st[0];
+          y[q] = st[128];
+          z[q] = st[256];
+          v[q] = *reinterpret_cast<const float4*>(part + (c4 * 128 + r) * 4);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        mm = fmaxf(mm, x[q]);
+        bb = fmaxf(bb, y[q]);
+      }
+      base = mm == -INFINITY ? 0.f : mm;
+      vbase = bb == -INFINITY ? 0.f : bb;
+      l *= fast_exp2(m - base);
+      const float f = fast_exp2(big - vbase);
+      o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+      m = mm;
+      big = bb;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        l += z[q] * fast_exp2(x[q] - base);
+        const float w = fast_exp2(y[q] - vbase);
+        if (y[q] != -INFINITY || z[q] != 0.f) {  // otherwise no key of the row: its sums may hold anything
+          o.x += v[q].x * w;
+          o.y += v[q].y * w;
+          o.z += v[q].z * w;
+          o.w += v[q].w * w;
+        }
+      }
     }
+    if (!live) return;
+  } else {
+    __shared__ float s_w[JOIN_MOST][8];
+    __shared__ float s_red[3][2 * DV / 32][8];
+    __shared__ int s_slot[JOIN_MOST];  // < 0: the share holds none of the item's tiles
+    for (int p = threadIdx.x; p < n; p += 2 * DV) s_slot[p] = it.leaves(first, p) ? 2 * (first + p) + (p == 0 ? 1 : 0) : -1;
+    __syncthreads();
+    for (int p = c4; p < n; p += GROUPS) {
+      const int slot = s_slot[p];
+      if (slot < 0 || !live) continue;
+      const float* st = a.partials + (int64_t)slot * C::PARTIAL + C::BM * DV + r;
+      m = fmaxf(m, st[0]);
+      big = fmaxf(big, st[128]);
+    }
+    auto across = [&](float v, int which, auto op) -> float {  // over the threads of a row
+      v = op(v, __shfl_xor_sync(0xffffffffu, v, 8));
+      v = op(v, __shfl_xor_sync(0xffffffffu, v, 16));
+      if ((threadIdx.x & 31) < 8) s_red[which][threadIdx.x / 32][sub] = v;
+      __syncthreads();
+      v = s_red[which][0][sub];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float w = f[q] < 0.f ? 0.f : f[q];
-      o.x += y[q].x * w;
-      o.y += y[q].y * w;
-      o.z += y[q].z * w;
-      o.w += y[q].w * w;
+      for (int q = 1; q < 2 * DV / 32; ++q) v = op(v, s_red[which][q][sub]);
+      return v;
+    };
+    m = across(m, 0, [](float x, float y) { return fmaxf(x, y); });
+    big = across(big, 1, [](float x, float y) { return fmaxf(x, y); });
+    base = m == -INFINITY ? 0.f : m;
+    vbase = big == -INFINITY ? 0.f : big;
+    for (int p = c4; p < n; p += GROUPS) {
+      const int slot = s_slot[p];
+      float f = -1.f;
+      if (slot >= 0 && live) {
+        const float* st = a.partials + (int64_t)slot * C::PARTIAL + C::BM * DV + r;
+        l += st[256] * fast_exp2(st[0] - base);
+        if (st[128] != -INFINITY || st[256] != 0.f) f = fast_exp2(st[128] - vbase);
+      }
+      s_w[p][sub] = f;  // < 0: no key of the row (its sums may hold anything)
+    }
+    l = across(l, 2, [](float x, float y) { return x + y; });
+    if (!live) return;
+    for (int p0 = 0; p0 < n; p0 += 8) {
+      float4 y[8];
+      float f[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        f[q] = p0 + q < n ? s_w[p0 + q][sub] : -1.f;
+        y[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (f[q] >= 0.f || f[q] != f[q])
+          y[q] = *reinterpret_cast<const float4*>(a.partials + (int64_t)s_slot[p0 + q] * C::PARTIAL + (c4 * 128 + r) * 4);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float w = f[q] < 0.f ? 0.f : f[q];
+        o.x += y[q].x * w;
+        o.y += y[q].y * w;
+        o.z += y[q].z * w;
+        o.w += y[q].w * w;
+      }
     }
   }
   const float fin = l == 0.f ? 0.f : fast_exp2(fminf(vbase - base, 126.f)) / (l * P_SCALE);
-  const int gr = it.r0 + r, tok = gr / a.group, head = it.h * a.group + gr - tok * a.group;
-  const int64_t row = it.q0 + tok, col = (int64_t)head * HD + it.slice * DV + 4 * c4;
   float x[4] = {o.x * fin, o.y * fin, o.z * fin, o.w * fin};
   if (l == 0.f) {
     x[0] = x[1] = x[2] = x[3] = 0.f;
   } else if (a.gate) {
-    const uint2 g = *reinterpret_cast<const uint2*>(a.gate + row * a.ldg + col);
-    const float2 s0 = unpack_bf16x2(g.x), s1 = unpack_bf16x2(g.y);
+    const float2 s0 = unpack_bf16x2(gate.x), s1 = unpack_bf16x2(gate.y);
     x[0] = x_sigmoid(x[0], s0.x);
     x[1] = x_sigmoid(x[1], s0.y);
     x[2] = x_sigmoid(x[2], s1.x);
