@@ -45,11 +45,9 @@ struct Cfg {
   static constexpr bool Q_TMEM = HD == 256;
   static constexpr int NS = HD == 64 ? 3 : HD == 512 ? 4 : 2;
   static constexpr int O_COL = 0, S_COL = DV, HI_COL = S_COL + NS * BN, LO_COL = HI_COL + HD / 4;
-  // The order of the products: S_{j + 1} before P_j V_j, waiting for the P V that read its buffer; or (heads of 256, whose
-  // CTA has the tensor core to itself) S_{j + NS} queued right behind P_j V_j, over whose probabilities it writes: the
-  // tensor core takes one thread's products in order, so it needs no wait (4,096 rows against 32,768 keys: 2,057 ->
-  // 1,960 us; with two CTAs to an SM the early scores only hold up the other's products: 288 -> 336 us).
-  static constexpr bool QUEUED = HD == 256;
+  // The order of the products: S_{j + 1} before P_j V_j, after a wait for the P V that read its buffer. (Scores queued
+  // right behind P_j V_j without that wait took 3% off heads of 256, but only products into one accumulator are
+  // documented to run in the order they were issued in.)
   static constexpr int USED_COLS = HI_COL + (Q_TMEM ? HD / 2 : 0), TMEM_COLS = USED_COLS <= 256 ? 256 : 512;
   static constexpr int QS_BYTES = Q_TMEM ? 0 : 2 * Q_BYTES;  // queries in shared memory
   static constexpr int KST = HD <= 128 ? 3 : HD == 256 ? 4 : 2, VST = HD <= 128 ? 3 : HD == 256 ? 4 : 1;  // ring stages
@@ -514,7 +512,7 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         auto issue_s = [&](int j) -> bool {
           const uint32_t G = g + j;
           const int st = G % KST;
-          if (!C::QUEUED && G >= NS && !mbar_wait(&pv_done[G % NS], ((G - NS) / NS) & 1, a.status)) return false;
+          if (G >= NS && !mbar_wait(&pv_done[G % NS], ((G - NS) / NS) & 1, a.status)) return false;
           if (!mbar_wait(&k_full[st], (G / KST) & 1, a.status)) return false;
           tc_fence_after();
           const uint32_t sk = smem_u32(s_k + st * C::K_BYTES);
@@ -535,11 +533,9 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
           mma_commit(&s_full[G % NS]);
           return true;
         };
-        constexpr int LOOK = C::QUEUED ? NS : 1;  // tiles that the scores run ahead
-        for (int j = 0; j < min(LOOK, n); ++j)
-          if (!issue_s(j)) goto done;
+        if (!issue_s(0)) goto done;
         for (int j = 0; j < n; ++j) {
-          if (!C::QUEUED && j + LOOK < n && !issue_s(j + LOOK)) goto done;
+          if (j + 1 < n && !issue_s(j + 1)) goto done;
           const uint32_t G = g + j;
           const int st = G % VST;
           if (!mbar_wait(&p_full[G % NS], (G / NS) & 1, a.status)) goto done;
@@ -553,7 +549,6 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
                        (j | kk) != 0);
           mma_commit(&v_empty[st]);
           mma_commit(&pv_done[G % NS]);
-          if (C::QUEUED && j + LOOK < n && !issue_s(j + LOOK)) goto done;
         }
         g += n;
       }
