@@ -226,11 +226,13 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
   // key/value head; with ITEM_TILES for each item before it, that is the weight that the shares divide.
   int64_t w_mine = 0, w_before = 0, tiles = 0;
   int items_mine = 0, items_before = 0, items = 0;
+  bool falls = false;
   auto scan = [&](int i0, int64_t carry, int carry_items) {
     const int i = i0 + tid;
     w_mine = 0;
     items_mine = 0;
     if (i < a.n) {
+      falls |= a.cu[i + 1] < a.cu[i];
       const Rows r = rows_of<RT>(a, i);
       w_mine = (int64_t)r.nrt * r.r.tiles;
       items_mine = r.nrt;
@@ -267,6 +269,11 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
     items = carry_items;
   };
   for (int i0 = 0; i0 < a.n; i0 += C::THREADS) scan(i0, tiles, items);
+  // Bounds that fall name rows twice: more items than the workspace holds. Such a launch has no work.
+  if (__syncthreads_or(falls)) {
+    if (tid == 0 && blockIdx.x == 0) *a.items = 0;
+    return;
+  }
   const int64_t total = (tiles + (int64_t)ITEM_TILES * items) * a.hkv;
   const int np = (int)shares(total, gridDim.x);
   const int64_t v_lo = quotient(total * blockIdx.x, np);

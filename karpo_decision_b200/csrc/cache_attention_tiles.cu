@@ -337,10 +337,12 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
   // ---- this CTA's share: a scan of the requests' weights for the total, then (a second scan if the requests outnumber
   // the threads) for the share's first request
   int64_t w_mine = 0, w_before = 0;
+  bool falls = false;
   auto scan = [&](int i0, int64_t carry) -> int64_t {  // the sum past this chunk; the thread's own weight and prefix
     const int i = i0 + tid;
     w_mine = 0;
     if (i < a.n) {
+      falls |= a.cu[i + 1] < a.cu[i];
       const Shape s = shape(a, i);
       w_mine = s.before(s.tiles) * SL * a.hkv;
     }
@@ -363,6 +365,7 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
   };
   int64_t total = 0;
   for (int i0 = 0; i0 < a.n; i0 += C::THREADS) total = scan(i0, total);
+  if (__syncthreads_or(falls)) total = 0;  // bounds that fall name rows twice, for CTAs at once: no work
   const int np = parts(total, a.group, gridDim.x);
   const int64_t share_lo = quotient(total * blockIdx.x, np);
   const int64_t share_hi = (int)blockIdx.x < np ? quotient(total * (blockIdx.x + 1), np) : 0;

@@ -569,7 +569,8 @@ def attention_cache(q: torch.Tensor, cache: KVBlocks, table: torch.Tensor, cu_q:
                     out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the new rows ``q`` (Tq, Hq, hd) over their requests' cached tokens (``kv_len`` of them, the new ones
     included, in the blocks ``table`` names), with ``attention_varlen``'s end-aligned window; returns (Tq, Hq * hd),
-    gated by sigmoid(gate) when given. Rows of ``out`` outside every request are left as they were."""
+    gated by sigmoid(gate) when given. Rows of ``out`` outside every request are left as they were; all of them when the
+    bounds ``cu_q`` fall anywhere (``kv_assign`` reports those)."""
     index, hkv, hd = cache.index, cache.heads, cache.head_dim
     _require(index >= 0, "the cache must be on a CUDA device")
     _require(q.dim() == 3, "q: bf16 (rows, heads, head_dim)")

@@ -1,6 +1,7 @@
 """The state cache's operators on the GPU against their float64 restatement (tests/cache_reference.py): block tables and
 slot maps, the e4m3 block write, attention over the blocks, and the three of them together."""
 
+import ctypes
 import math
 
 import numpy as np
@@ -8,7 +9,7 @@ import pytest
 import torch
 
 import cache_reference as ref
-from karpo_decision_b200 import ops
+from karpo_decision_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda")
@@ -422,6 +423,36 @@ def test_repeated_calls_are_equal_and_streams_do_not_mix(new):
             got.append(ops.attention_cache(q, *args, gate=gate))
     torch.cuda.synchronize()
     assert all(torch.equal(x, want) for x in got)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("max_q", [1, 2, 10])
+@pytest.mark.parametrize("n", [3, 900])
+def test_bounds_that_fall_compute_nothing(hd, max_q, n):
+    """Bounds that name rows twice (0, 10, 0, 10): nothing is computed, nothing is written behind the workspace, and the
+    same buffers serve a good call next. 900 requests are more than a block's threads, the fall is in the last part."""
+    hq, rows = 8, 10
+    cache, table, q, _ = make([70] * n, [0] * n, hq, 1, hd, pad=rows)
+    cu = ints([0, 10] + [10] * (n - 3) + [0, 10])
+    lens, out = ints([70] * n), torch.full((rows, hq * hd), 5.0, dtype=torch.bfloat16, device=DEV)
+    size = ctypes.c_int64()
+    _lib.call("kd_attention_cache_workspace", n, max_q, rows, hq, 1, hd, ctypes.addressof(size))
+    scratch = torch.full((size.value + (1 << 24),), 0xab, dtype=torch.uint8, device=DEV)
+
+    def run(bounds_):
+        _lib.call("kd_attention_cache", q.data_ptr(), hq * hd, cache.k.data_ptr(), cache.v.data_ptr(),
+                  cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cache.blocks, table.data_ptr(), table.stride(0),
+                  table.shape[1], bounds_.data_ptr(), lens.data_ptr(), n, max_q, rows, out.data_ptr(), hq * hd, None, 0,
+                  hq, 1, hd, hd ** -0.5, -1, 0, scratch.data_ptr(), size.value, ops.status_word(DEV).data_ptr(),
+                  torch.cuda.current_stream().cuda_stream)
+
+    run(cu)
+    ops.check_status(DEV)
+    assert (out == 5).all() and (scratch[size.value:] == 0xab).all()
+    good = ints([0] * (n - 1) + [5, 10])
+    run(good)
+    assert torch.equal(out, ops.attention_cache(q, cache, table, good, lens, max_q, hd ** -0.5, (-1, 0)))
+    assert (scratch[size.value:] == 0xab).all()
 
 
 # ------------------------------------------------------------------------------------------------ together
