@@ -255,8 +255,9 @@ int kd_gated_norm(const void* x, int64_t ldx, const void* z, int64_t ldz, const 
  * further blocks are taken from the top in request order and written to its table row; kv_len[i] = lens[i] + new rows
  * (kv_len may be lens), seqpos[t] the row's position in its request, slots[t] = block * KD_KV_BLOCK + place. Rows
  * outside every request (padding) get position 0 and slot -1. All or nothing: when blocks are missing nothing is taken,
- * every slot is -1 and kv_len = lens. free_count[1]: 0, the number of missing blocks, or KD_KV_TABLE_FULL /
- * KD_KV_MALFORMED. At most 16,384 requests. */
+ * every slot is -1 and kv_len = lens; so too when an id that the rows would use, a half-filled block's or a new one's,
+ * lies outside the pool. free_count[1]: 0, the number of missing blocks, or KD_KV_TABLE_FULL / KD_KV_MALFORMED. At most
+ * 16,384 requests. */
 int kd_kv_assign(const int32_t* lens, const int32_t* cu, int num_requests, int64_t rows, int32_t* table,
                  int64_t ld_table, int table_width, const int32_t* free_blocks, int capacity, int32_t* free_count,
                  int32_t* kv_len, int64_t* seqpos, int64_t* slots, cudaStream_t stream);

@@ -45,6 +45,8 @@ KD_DEVICE int block_exclusive_sum(int v, int* warp_sums, int& total) {
   return before + x - v;
 }
 
+KD_DEVICE bool in_pool(int id, int capacity) { return (uint32_t)id < (uint32_t)capacity; }
+
 // The last i in [0, n) with keys[i] <= x (keys ascending, keys[0] <= x).
 KD_DEVICE int last_at_most(const int* keys, int n, int x) {
   int lo = 0, hi = n - 1;
@@ -80,7 +82,9 @@ struct AssignArgs {
 // taking its share of the rows. The k-th new block of the launch is the k-th from the top of the free stack, so every
 // CTA knows the new blocks without reading the table that others write; a new block's table entry is written by the
 // thread of the block's first row. The stack's count and kv_len (which may be `lens` itself)
-// change after a cluster barrier, when every CTA has read them.
+// change after a cluster barrier, when every CTA has read them. Every CTA also looks at the ids that the rows will use,
+// the half-filled blocks' table entries during the scan and the new blocks' on the stack after it: one outside the pool
+// refuses the call before anything is written.
 // Bound by latency: dependent reads of the lengths, one of the stack or the table, and the launch.
 __global__ void __launch_bounds__(TABLE_THREADS) assign_kernel(AssignArgs a) {
   extern __shared__ int smem[];
@@ -94,11 +98,14 @@ __global__ void __launch_bounds__(TABLE_THREADS) assign_kernel(AssignArgs a) {
   const int have_free = a.count[0];
   for (int i = tid; i <= a.n; i += TABLE_THREADS) s_cu[i] = a.cu[i];
   for (int i = tid; i < a.n; i += TABLE_THREADS) s_len[i] = a.lens[i];
+  const bool stack_ok = have_free >= 0 && have_free <= a.capacity;
+  const int top = stack_ok && tid < have_free ? a.free_ids[have_free - 1 - tid] : -1;  // here when the scan is done
   __syncthreads();
   int carry = 0;
   for (int i0 = 0; i0 < a.n; i0 += TABLE_THREADS) {
     const int i = i0 + tid;
-    int add = 0;
+    int add = 0, part = -1;
+    bool half = false;  // new rows go on in the half-filled block `part`
     if (i < a.n) {
       const int len = s_len[i];
       const int64_t grown = (int64_t)s_cu[i + 1] - s_cu[i];
@@ -109,16 +116,23 @@ __global__ void __launch_bounds__(TABLE_THREADS) assign_kernel(AssignArgs a) {
         atomicMin(&s_bad, KD_KV_TABLE_FULL);
       } else {
         add = (int)((len + grown + BLOCK - 1) / BLOCK) - blocks_of(len);
+        half = grown > 0 && len % BLOCK > 0;
+        if (half) part = a.table[(int64_t)i * a.ldt + len / BLOCK];
       }
     }
     int total;
     const int base = block_exclusive_sum(add, warp_sums, total);
     if (i < a.n) s_base[i] = carry + base;
+    if (half && !in_pool(part, a.capacity)) atomicMin(&s_bad, KD_KV_MALFORMED);
     carry += total;
   }
-  __syncthreads();
   const int needed = carry;
-  const bool stack_ok = have_free >= 0 && have_free <= a.capacity;
+  if (stack_ok && needed <= have_free) {
+    for (int j = tid; j < needed; j += TABLE_THREADS)
+      if (!in_pool(j < TABLE_THREADS ? top : a.free_ids[have_free - 1 - j], a.capacity))
+        atomicMin(&s_bad, KD_KV_MALFORMED);
+  }
+  __syncthreads();
   const int bad = !stack_ok ? KD_KV_MALFORMED : s_bad;
   const bool ok = bad == 0 && needed <= have_free;
   const bool positions = bad != KD_KV_MALFORMED;
@@ -140,7 +154,7 @@ __global__ void __launch_bounds__(TABLE_THREADS) assign_kernel(AssignArgs a) {
           id = a.free_ids[have_free - 1 - (s_base[i] + b - had)];
           if (pos % BLOCK == 0) a.table[(int64_t)i * a.ldt + b] = id;
         }
-        if (id >= 0 && id < a.capacity) slot = (int64_t)id * BLOCK + pos % BLOCK;
+        slot = (int64_t)id * BLOCK + pos % BLOCK;
       }
     }
     a.seqpos[t] = pos;
@@ -206,7 +220,7 @@ __global__ void __launch_bounds__(TABLE_THREADS) release_kernel(ReleaseArgs a) {
     for (int j = tid; j < dropped; j += TABLE_THREADS) {
       const int i = last_at_most(s_base, a.n, j);
       const int id = a.table[(int64_t)i * a.ldt + s_from[i] + j - s_base[i]];
-      if (id < 0 || id >= a.capacity) atomicMin(&s_bad, KD_KV_MALFORMED);
+      if (!in_pool(id, a.capacity)) atomicMin(&s_bad, KD_KV_MALFORMED);
     }
   }
   __syncthreads();

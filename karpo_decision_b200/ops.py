@@ -479,7 +479,7 @@ def kv_assign(lens: torch.Tensor, cu: torch.Tensor, table: torch.Tensor, free: t
     stack ``free`` (``count`` int32[2]: its height, the outcome), extends ``table`` in place and returns (kv_len int32
     (n,), seqpos int64 (rows,), slots int64 (rows,)), or writes them to ``out`` (whose kv_len may be ``lens``). When
     blocks are missing nothing is taken, every slot is -1 and ``count[1]`` says how many (or KV_TABLE_FULL /
-    KV_MALFORMED)."""
+    KV_MALFORMED, block ids outside the pool among them)."""
     n, index = lens.numel(), lens.get_device()
     _require(index >= 0, "lens must be on a CUDA device")
     _int32s(lens, n, "lens", index)

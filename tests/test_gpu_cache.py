@@ -92,6 +92,46 @@ def test_assign_refuses_on_the_device(lens, cu, width, outcome):
     assert kv_len.tolist() == lens and set(slots.tolist()) == {-1}
 
 
+@pytest.mark.parametrize("bad", [-1, 40, -2 ** 31, 2 ** 31 - 1])
+@pytest.mark.parametrize("where", ["half-filled block", "top of the stack", "deep in the stack"])
+def test_assign_refuses_ids_outside_the_pool(bad, where):
+    """An id the rows would use: all or nothing, as for missing blocks. The same call with the id put right succeeds."""
+    # 40 blocks: requests hold 5 (4 full ones, 6 tokens in the last) and 0 tokens; 1,500 more for the deep entry
+    deep = 1500 if where == "deep in the stack" else 0
+    capacity = 40 + deep
+    lens, new = [262, 0], [100, 64 * (deep or 2)]
+    width = 2 + new[1] // BLOCK + 5
+    rows, free, count = dealt(lens, new, width, capacity - 5)
+    need = 1 + new[1] // BLOCK
+    table, stack, height = ints(rows), ints(free), ints([count, 0])
+    wrong = bad if bad != 40 else capacity
+    entry = {"half-filled block": (table, (0, 4)), "top of the stack": (stack, (count - 1,)),
+             "deep in the stack": (stack, (count - need,))}[where]
+    right = entry[0][entry[1]].item()
+    entry[0][entry[1]] = wrong
+    before = table.clone(), stack.clone()
+    args = ints(lens), ints(bounds(new)), table, stack, height, sum(new)
+    kv_len, _, slots = ops.kv_assign(*args)
+    assert height.tolist() == [count, ops.KV_MALFORMED] and kv_len.tolist() == lens and (slots == -1).all()
+    assert torch.equal(table, before[0]) and torch.equal(stack, before[1])
+    entry[0][entry[1]] = right
+    got = ops.kv_assign(*args)
+    want = ref.assign(lens, new, rows, free, count, width)
+    assert [x.tolist() for x in got] == list(want[:3]) and table.tolist() == want[3] and height.tolist() == [want[4], 0]
+
+
+def test_assign_looks_at_the_ids_it_uses_only():
+    """Holes in earlier blocks, a half-filled block without new rows and stack entries below the new blocks' harm nobody."""
+    lens, new = [262, 70, 64], [100, 0, 1]
+    rows, free, count = dealt(lens, new, 9, 6)
+    rows[0][1], rows[0][3], rows[1][1], rows[2][0] = -1, 10 ** 9, -5, 99
+    free[:count - 2] = [-3] * (count - 2)
+    table, stack, height = ints(rows), ints(free), ints([count, 0])
+    got = ops.kv_assign(ints(lens), ints(bounds(new)), table, stack, height, sum(new))
+    want = ref.assign(lens, new, rows, free, count, 9)
+    assert [x.tolist() for x in got] == list(want[:3]) and table.tolist() == want[3] and height.tolist() == [want[4], 0]
+
+
 def test_assign_in_place_and_release_to_a_length():
     """kv_len may be lens; a release keeps each request's first tokens and the blocks that hold them."""
     lens, new, keep = ints([100, 0, 64]), [300, 70, 1], [130, 0, 500]
