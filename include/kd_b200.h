@@ -248,7 +248,7 @@ int kd_gated_norm(const void* x, int64_t ldx, const void* z, int64_t ldz, const 
  * computes every request from its first token (decider.py:110-123). */
 #define KD_KV_BLOCK 64
 #define KD_KV_TABLE_FULL (-1) /* free_count[1]: a request's blocks exceed the table's width */
-#define KD_KV_MALFORMED (-2)  /* free_count[1]: lengths, bounds, count or block ids outside their ranges */
+#define KD_KV_MALFORMED (-2)  /* free_count[1]: lengths, bounds, count or block ids outside their ranges, an id twice */
 
 /* Blocks, positions and slots of new rows. Request i holds lens[i] tokens and gets the rows [cu[i], cu[i+1]); free_blocks
  * int32 [capacity] is a stack of free block ids (capacity: blocks in the pool), free_count[0] its height. The request's
@@ -256,7 +256,8 @@ int kd_gated_norm(const void* x, int64_t ldx, const void* z, int64_t ldz, const 
  * (kv_len may be lens), seqpos[t] the row's position in its request, slots[t] = block * KD_KV_BLOCK + place. Rows
  * outside every request (padding) get position 0 and slot -1. All or nothing: when blocks are missing nothing is taken,
  * every slot is -1 and kv_len = lens; so too when an id that the rows would use, a half-filled block's or a new one's,
- * lies outside the pool. free_count[1]: 0, the number of missing blocks, or KD_KV_TABLE_FULL / KD_KV_MALFORMED. At most
+ * lies outside the pool or is met twice: requests may share blocks that get no rows (a state that ends with its block),
+ * not one that does. free_count[1]: 0, the number of missing blocks, or KD_KV_TABLE_FULL / KD_KV_MALFORMED. At most
  * 16,384 requests. */
 int kd_kv_assign(const int32_t* lens, const int32_t* cu, int num_requests, int64_t rows, int32_t* table,
                  int64_t ld_table, int table_width, const int32_t* free_blocks, int capacity, int32_t* free_count,
@@ -264,8 +265,8 @@ int kd_kv_assign(const int32_t* lens, const int32_t* cu, int num_requests, int64
 
 /* The inverse: the blocks that hold none of request i's first keep[i] tokens (of lens[i]) return to the stack, the last
  * request's last block first, and their table entries become -1. lens is not written. free_count[1]: 0, or
- * KD_KV_MALFORMED (an entry outside the pool, a stack without room: nothing is given back). A block named by two
- * requests would be given back twice: no two may share one. */
+ * KD_KV_MALFORMED (an entry outside the pool, one block named twice among those given back, a stack without room: nothing
+ * is given back). A block that another request keeps must not be given back. */
 int kd_kv_release(int32_t* table, int64_t ld_table, int table_width, const int32_t* lens, const int32_t* keep,
                   int num_requests, int32_t* free_blocks, int capacity, int32_t* free_count, cudaStream_t stream);
 

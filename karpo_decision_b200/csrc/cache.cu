@@ -47,6 +47,19 @@ KD_DEVICE int block_exclusive_sum(int v, int* warp_sums, int& total) {
 
 KD_DEVICE bool in_pool(int id, int capacity) { return (uint32_t)id < (uint32_t)capacity; }
 
+// Ids met so far, a bit each: SEEN_BLOCKS ids from `from` on at a time (one pass for pools up to that size, so that
+// nothing waits for it), in shared memory.
+constexpr int SEEN_BLOCKS = 1 << 18;
+__host__ __device__ constexpr int seen_words(int capacity) {
+  return (capacity < SEEN_BLOCKS ? capacity : SEEN_BLOCKS) / 32 + 1;
+}
+// Marks an id of the pool; whether it was marked before.
+KD_DEVICE bool met_before(uint32_t* seen, int id, int from) {
+  const uint32_t at = (uint32_t)id - (uint32_t)from;
+  if (at >= (uint32_t)SEEN_BLOCKS) return false;
+  return (atomicOr(&seen[at / 32], 1u << (at & 31)) >> (at & 31)) & 1u;
+}
+
 // The last i in [0, n) with keys[i] <= x (keys ascending, keys[0] <= x).
 KD_DEVICE int last_at_most(const int* keys, int n, int x) {
   int lo = 0, hi = n - 1;
@@ -83,14 +96,16 @@ struct AssignArgs {
 // CTA knows the new blocks without reading the table that others write; a new block's table entry is written by the
 // thread of the block's first row. The stack's count and kv_len (which may be `lens` itself)
 // change after a cluster barrier, when every CTA has read them. Every CTA also looks at the ids that the rows will use,
-// the half-filled blocks' table entries during the scan and the new blocks' on the stack after it: one outside the pool
-// refuses the call before anything is written.
+// the half-filled blocks' table entries during the scan and the new blocks' on the stack after it: one outside the pool,
+// or one met twice, whose rows two requests would write, refuses the call before anything is written.
 // Bound by latency: dependent reads of the lengths, one of the stack or the table, and the launch.
 __global__ void __launch_bounds__(TABLE_THREADS) assign_kernel(AssignArgs a) {
   extern __shared__ int smem[];
   int* s_cu = smem;                // [n + 1]
   int* s_len = s_cu + a.n + 1;     // [n]
   int* s_base = s_len + a.n;       // [n]: the request's first new block, counted over the launch
+  uint32_t* s_seen = reinterpret_cast<uint32_t*>(s_base + a.n);  // [seen_words]
+  const int words = seen_words(a.capacity);
   __shared__ int warp_sums[32];
   __shared__ int s_bad;
   const int tid = threadIdx.x;
@@ -98,6 +113,7 @@ __global__ void __launch_bounds__(TABLE_THREADS) assign_kernel(AssignArgs a) {
   const int have_free = a.count[0];
   for (int i = tid; i <= a.n; i += TABLE_THREADS) s_cu[i] = a.cu[i];
   for (int i = tid; i < a.n; i += TABLE_THREADS) s_len[i] = a.lens[i];
+  for (int w = tid; w < words; w += TABLE_THREADS) s_seen[w] = 0;
   const bool stack_ok = have_free >= 0 && have_free <= a.capacity;
   const int top = stack_ok && tid < have_free ? a.free_ids[have_free - 1 - tid] : -1;  // here when the scan is done
   __syncthreads();
@@ -123,16 +139,34 @@ __global__ void __launch_bounds__(TABLE_THREADS) assign_kernel(AssignArgs a) {
     int total;
     const int base = block_exclusive_sum(add, warp_sums, total);
     if (i < a.n) s_base[i] = carry + base;
-    if (half && !in_pool(part, a.capacity)) atomicMin(&s_bad, KD_KV_MALFORMED);
+    if (half && (!in_pool(part, a.capacity) || met_before(s_seen, part, 0))) atomicMin(&s_bad, KD_KV_MALFORMED);
     carry += total;
   }
   const int needed = carry;
   if (stack_ok && needed <= have_free) {
-    for (int j = tid; j < needed; j += TABLE_THREADS)
-      if (!in_pool(j < TABLE_THREADS ? top : a.free_ids[have_free - 1 - j], a.capacity))
-        atomicMin(&s_bad, KD_KV_MALFORMED);
+    for (int j = tid; j < needed; j += TABLE_THREADS) {
+      const int id = j < TABLE_THREADS ? top : a.free_ids[have_free - 1 - j];
+      if (!in_pool(id, a.capacity) || met_before(s_seen, id, 0)) atomicMin(&s_bad, KD_KV_MALFORMED);
+    }
   }
   __syncthreads();
+  if (a.capacity > SEEN_BLOCKS && s_bad == 0 && stack_ok && needed <= have_free) {  // the ids past the first pass's
+    for (int from = SEEN_BLOCKS; from < a.capacity && from > 0; from += SEEN_BLOCKS) {
+      __syncthreads();
+      for (int w = tid; w < words; w += TABLE_THREADS) s_seen[w] = 0;
+      __syncthreads();
+      bool twice = false;
+      for (int i = tid; i < a.n; i += TABLE_THREADS)
+        if (s_cu[i + 1] > s_cu[i] && s_len[i] % BLOCK > 0)
+          twice |= met_before(s_seen, a.table[(int64_t)i * a.ldt + s_len[i] / BLOCK], from);
+      for (int j = tid; j < needed; j += TABLE_THREADS) twice |= met_before(s_seen, a.free_ids[have_free - 1 - j], from);
+      if (__syncthreads_or(twice)) {
+        if (tid == 0) s_bad = KD_KV_MALFORMED;
+        break;
+      }
+    }
+    __syncthreads();
+  }
   const int bad = !stack_ok ? KD_KV_MALFORMED : s_bad;
   const bool ok = bad == 0 && needed <= have_free;
   const bool positions = bad != KD_KV_MALFORMED;
@@ -184,11 +218,13 @@ struct ReleaseArgs {
 
 // The blocks past each request's first `keep` tokens go back on the stack, the last request's last block first: an
 // assignment followed by its release leaves the stack as it was. One CTA: the first pass checks every entry, so a table
-// with an id outside the pool gives nothing back.
+// with an id outside the pool, or with one named twice among those given back, gives nothing back.
 __global__ void __launch_bounds__(TABLE_THREADS) release_kernel(ReleaseArgs a) {
   extern __shared__ int smem[];
   int* s_base = smem;           // [n]
   int* s_from = s_base + a.n;   // [n]: the first block given back
+  uint32_t* s_seen = reinterpret_cast<uint32_t*>(s_from + a.n);  // [seen_words]
+  const int words = seen_words(a.capacity);
   __shared__ int warp_sums[32];
   __shared__ int s_bad;
   const int tid = threadIdx.x;
@@ -217,13 +253,17 @@ __global__ void __launch_bounds__(TABLE_THREADS) release_kernel(ReleaseArgs a) {
   const int dropped = carry;
   const bool sized = s_bad == 0 && have_free >= 0 && (int64_t)have_free + dropped <= a.capacity;
   if (sized) {
-    for (int j = tid; j < dropped; j += TABLE_THREADS) {
-      const int i = last_at_most(s_base, a.n, j);
-      const int id = a.table[(int64_t)i * a.ldt + s_from[i] + j - s_base[i]];
-      if (!in_pool(id, a.capacity)) atomicMin(&s_bad, KD_KV_MALFORMED);
+    for (int from = 0; from < a.capacity && from >= 0; from += SEEN_BLOCKS) {
+      for (int w = tid; w < words; w += TABLE_THREADS) s_seen[w] = 0;
+      __syncthreads();
+      for (int j = tid; j < dropped; j += TABLE_THREADS) {
+        const int i = last_at_most(s_base, a.n, j);
+        const int id = a.table[(int64_t)i * a.ldt + s_from[i] + j - s_base[i]];
+        if (!in_pool(id, a.capacity) || met_before(s_seen, id, from)) atomicMin(&s_bad, KD_KV_MALFORMED);
+      }
+      __syncthreads();
     }
   }
-  __syncthreads();
   const bool ok = sized && s_bad == 0;
   if (ok) {
     for (int j = tid; j < dropped; j += TABLE_THREADS) {
@@ -467,7 +507,7 @@ extern "C" int kd_kv_assign(const int32_t* lens, const int32_t* cu, int num_requ
     return set_error(KD_ERR_ARGUMENT, "kv_assign: null pointer");
   const kv::AssignArgs a{lens, cu, num_requests, rows, table, ld_table, table_width, free_blocks, capacity, free_count,
                          kv_len, seqpos, slots};
-  const int ints = 3 * num_requests + 1;
+  const int ints = 3 * num_requests + 1 + kv::seen_words(capacity);
   if (int rc = kv::table_smem(ints, (const void*)kv::assign_kernel, "kv_assign: shared memory")) return rc;
   int ctas = 1;  // a cluster's worth of rows: 1,024 rows a CTA and pass
   while (ctas < 8 && rows > (int64_t)ctas * kv::TABLE_THREADS) ctas *= 2;
@@ -494,7 +534,7 @@ extern "C" int kd_kv_release(int32_t* table, int64_t ld_table, int table_width, 
   if (!table || !lens || !keep || !free_blocks || !free_count)
     return set_error(KD_ERR_ARGUMENT, "kv_release: null pointer");
   const kv::ReleaseArgs a{table, ld_table, table_width, lens, keep, num_requests, free_blocks, capacity, free_count};
-  const int ints = 2 * num_requests;
+  const int ints = 2 * num_requests + kv::seen_words(capacity);
   if (int rc = kv::table_smem(ints, (const void*)kv::release_kernel, "kv_release: shared memory")) return rc;
   kv::release_kernel<<<1, kv::TABLE_THREADS, ints * 4, stream>>>(a);
   return record_cuda_error(cudaGetLastError(), "kv_release: launch");

@@ -479,7 +479,7 @@ def kv_assign(lens: torch.Tensor, cu: torch.Tensor, table: torch.Tensor, free: t
     stack ``free`` (``count`` int32[2]: its height, the outcome), extends ``table`` in place and returns (kv_len int32
     (n,), seqpos int64 (rows,), slots int64 (rows,)), or writes them to ``out`` (whose kv_len may be ``lens``). When
     blocks are missing nothing is taken, every slot is -1 and ``count[1]`` says how many (or KV_TABLE_FULL /
-    KV_MALFORMED, block ids outside the pool among them)."""
+    KV_MALFORMED, block ids outside the pool and two requests with rows for one block among them)."""
     n, index = lens.numel(), lens.get_device()
     _require(index >= 0, "lens must be on a CUDA device")
     _int32s(lens, n, "lens", index)
@@ -505,7 +505,8 @@ def kv_assign(lens: torch.Tensor, cu: torch.Tensor, table: torch.Tensor, free: t
 def kv_release(table: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor, free: torch.Tensor, count: torch.Tensor
                ) -> None:
     """Gives the blocks past each request's first ``keep`` tokens (of ``lens``) back to the stack, undoing a
-    ``kv_assign`` exactly; ``lens`` is not written. No two requests may share a block given back."""
+    ``kv_assign`` exactly; ``lens`` is not written. No two requests may share a block given back (KV_MALFORMED, and nothing
+    is), nor may another request keep one."""
     n, index = lens.numel(), lens.get_device()
     _require(index >= 0, "lens must be on a CUDA device")
     _int32s(lens, n, "lens", index)

@@ -132,6 +132,60 @@ def test_assign_looks_at_the_ids_it_uses_only():
     assert [x.tolist() for x in got] == list(want[:3]) and table.tolist() == want[3] and height.tolist() == [want[4], 0]
 
 
+@pytest.mark.parametrize("capacity", [40, 700000])  # ids in one part of the kernel's bitmap, and in three
+@pytest.mark.parametrize("twice", ["half-filled blocks", "half-filled block and stack", "stack"])
+def test_assign_refuses_a_block_twice(capacity, twice):
+    """Two requests' rows for one block: neither gets a slot. The same call with another id succeeds."""
+    lens, new, width = [70, 200, 0], [5, 60, 130], 6
+    high = capacity - 1
+    rows = [[1, high] + [-1] * 4, [2, 3, 4, 5, -1, -1], [-1] * 6]
+    free = list(range(6, 30)) + [-1] * (capacity - 24)  # 1 + 3 new blocks: 29, 28, 27, 26
+    count = 24
+    if twice == "half-filled blocks":
+        at, rows[1][3] = (0, (1, 3)), high
+    elif twice == "half-filled block and stack":
+        at, free[21] = (1, (21,)), high
+    else:
+        at, free[20], free[22] = (1, (22,)), high - 1, high - 1
+    table, stack, height = ints(rows), ints(free), ints([count, 0])
+    args = ints(lens), ints(bounds(new)), table, stack, height, sum(new)
+    kv_len, _, slots = ops.kv_assign(*args)
+    assert height.tolist() == [count, ops.KV_MALFORMED] and kv_len.tolist() == lens and (slots == -1).all()
+    assert table.tolist() == rows and stack.tolist() == free
+    (table, stack)[at[0]][at[1]] = 33
+    rows, free = table.tolist(), stack.tolist()
+    got = ops.kv_assign(*args)
+    want = ref.assign(lens, new, rows, free, count, width)
+    assert [x.tolist() for x in got] == list(want[:3]) and table.tolist() == want[3] and height.tolist() == [want[4], 0]
+
+
+def test_requests_share_blocks_that_get_no_rows():
+    """Two questions on a state that ends with its block, and on a half-filled one that only one of them goes on in;
+    release to the state's length gives back their own blocks only."""
+    lens, new = [128, 128, 100, 100], [70, 3, 0, 9]
+    rows = [[1, 2, -1, -1], [1, 2, -1, -1], [3, 4, -1, -1], [3, 4, -1, -1]]
+    free = [9, 8, 7, 6, 5, -1, -1, -1, -1, -1]
+    table, stack, height = ints(rows), ints(free), ints([5, 0])
+    got = ops.kv_assign(ints(lens), ints(bounds(new)), table, stack, height, sum(new))
+    want = ref.assign(lens, new, rows, free, 5, 4)
+    assert [x.tolist() for x in got] == list(want[:3]) and table.tolist() == want[3] and height.tolist() == [2, 0]
+    ops.kv_release(table, got[0], ints(lens), stack, height)
+    assert table.tolist() == rows and stack.tolist() == free and height.tolist() == [5, 0]
+
+
+@pytest.mark.parametrize("capacity", [40, 700000])
+def test_release_of_a_block_twice_gives_nothing_back(capacity):
+    high = capacity - 1
+    rows, free = [[3, high, 5], [4, high, 6]], [0, 1, 2] + [-1] * (capacity - 3)
+    table, stack, height = ints(rows), ints(free), ints([3, 0])
+    ops.kv_release(table, ints([150, 150]), ints([0, 0]), stack, height)
+    assert height.tolist() == [3, ops.KV_MALFORMED] and table.tolist() == rows and stack.tolist() == free
+    table[1, 1] = 7
+    ops.kv_release(table, ints([150, 150]), ints([0, 100]), stack, height)
+    assert height.tolist()[0] == 7 and table.tolist() == [[-1] * 3, [4, 7, -1]]
+    assert stack.tolist()[:7] == [0, 1, 2, 6, 5, high, 3]
+
+
 def test_assign_in_place_and_release_to_a_length():
     """kv_len may be lens; a release keeps each request's first tokens and the blocks that hold them."""
     lens, new, keep = ints([100, 0, 64]), [300, 70, 1], [130, 0, 500]
