@@ -226,13 +226,13 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
   // key/value head; with ITEM_TILES for each item before it, that is the weight that the shares divide.
   int64_t w_mine = 0, w_before = 0, tiles = 0;
   int items_mine = 0, items_before = 0, items = 0;
-  bool falls = false;
   auto scan = [&](int i0, int64_t carry, int carry_items) {
     const int i = i0 + tid;
     w_mine = 0;
     items_mine = 0;
+    bool falls = false;
     if (i < a.n) {
-      falls |= a.cu[i + 1] < a.cu[i];
+      falls = a.cu[i + 1] < a.cu[i];
       const Rows r = rows_of<RT>(a, i);
       w_mine = (int64_t)r.nrt * r.r.tiles;
       items_mine = r.nrt;
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
       s_warp_tiles[warp] = x;
       s_warp_items[warp] = y;
     }
-    __syncthreads();
+    falls = __syncthreads_or(falls) || carry < 0;
     w_before = carry + x - w_mine;
     items_before = carry_items + y - items_mine;
 #pragma unroll
@@ -265,12 +265,12 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
       carry_items += s_warp_items[v];
     }
     __syncthreads();
-    tiles = carry;
+    tiles = falls ? -1 : carry;
     items = carry_items;
   };
   for (int i0 = 0; i0 < a.n; i0 += C::THREADS) scan(i0, tiles, items);
   // Bounds that fall name rows twice: more items than the workspace holds. Such a launch has no work.
-  if (__syncthreads_or(falls)) {
+  if (tiles < 0) {
     if (tid == 0 && blockIdx.x == 0) *a.items = 0;
     return;
   }

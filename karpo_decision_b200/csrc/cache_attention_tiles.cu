@@ -337,12 +337,14 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
   // ---- this CTA's share: a scan of the requests' weights for the total, then (a second scan if the requests outnumber
   // the threads) for the share's first request
   int64_t w_mine = 0, w_before = 0;
-  bool falls = false;
-  auto scan = [&](int i0, int64_t carry) -> int64_t {  // the sum past this chunk; the thread's own weight and prefix
+  // The sum past this chunk (-1 once bounds fall: they name rows twice, for CTAs at once, and such a launch has no work);
+  // the thread's own weight and prefix.
+  auto scan = [&](int i0, int64_t carry) -> int64_t {
     const int i = i0 + tid;
     w_mine = 0;
+    bool falls = false;
     if (i < a.n) {
-      falls |= a.cu[i + 1] < a.cu[i];
+      falls = a.cu[i + 1] < a.cu[i];
       const Shape s = shape(a, i);
       w_mine = s.before(s.tiles) * SL * a.hkv;
     }
@@ -353,7 +355,7 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
       if (lane >= o) x += px;
     }
     if (lane == 31) s_warp[warp] = x;
-    __syncthreads();
+    falls = __syncthreads_or(falls) || carry < 0;
     w_before = carry + x - w_mine;
 #pragma unroll
     for (int v = 0; v < C::THREADS / 32; ++v) {
@@ -361,11 +363,11 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
       carry += s_warp[v];
     }
     __syncthreads();
-    return carry;
+    return falls ? -1 : carry;
   };
   int64_t total = 0;
   for (int i0 = 0; i0 < a.n; i0 += C::THREADS) total = scan(i0, total);
-  if (__syncthreads_or(falls)) total = 0;  // bounds that fall name rows twice, for CTAs at once: no work
+  total = max(total, (int64_t)0);
   const int np = parts(total, a.group, gridDim.x);
   const int64_t share_lo = quotient(total * blockIdx.x, np);
   const int64_t share_hi = (int)blockIdx.x < np ? quotient(total * (blockIdx.x + 1), np) : 0;
