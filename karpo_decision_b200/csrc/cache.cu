@@ -481,14 +481,23 @@ __global__ void __launch_bounds__(store_threads(HD), 1280 / store_threads(HD))
   }
 }
 
-static int table_smem(int ints, const void* kernel, const char* what) {
-  const int bytes = ints * 4;
-  if (bytes > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+// The kernel's limit on shared memory, raised once a device to what the most requests of the largest pool need: a limit
+// set call by call could fall between another thread's check and its launch, and 48 KB without one count the static
+// arrays too.
+static int table_smem(int most_ints, const void* kernel, bool (&configured)[64], const char* what) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return set_error(KD_ERR_ARGUMENT, "kv tables: device index");
+  if (!configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most_ints * 4);
     if (e != cudaSuccess) return record_cuda_error(e, what);
+    configured[dev] = true;
   }
   return KD_OK;
 }
+constexpr int assign_ints(int n, int capacity) { return 3 * n + 1 + seen_words(capacity); }
+constexpr int release_ints(int n, int capacity) { return 2 * n + seen_words(capacity); }
+static_assert(assign_ints(MAX_REQUESTS, 0x7fffffff) * 4 + 1024 <= 227 * 1024, "shared memory budget");
 
 }  // namespace kv
 }  // namespace kd
@@ -507,14 +516,16 @@ extern "C" int kd_kv_assign(const int32_t* lens, const int32_t* cu, int num_requ
     return set_error(KD_ERR_ARGUMENT, "kv_assign: null pointer");
   const kv::AssignArgs a{lens, cu, num_requests, rows, table, ld_table, table_width, free_blocks, capacity, free_count,
                          kv_len, seqpos, slots};
-  const int ints = 3 * num_requests + 1 + kv::seen_words(capacity);
-  if (int rc = kv::table_smem(ints, (const void*)kv::assign_kernel, "kv_assign: shared memory")) return rc;
+  static bool configured[64] = {false};
+  if (int rc = kv::table_smem(kv::assign_ints(kv::MAX_REQUESTS, 0x7fffffff), (const void*)kv::assign_kernel, configured,
+                              "kv_assign: shared memory"))
+    return rc;
   int ctas = 1;  // a cluster's worth of rows: 1,024 rows a CTA and pass
   while (ctas < 8 && rows > (int64_t)ctas * kv::TABLE_THREADS) ctas *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kv::TABLE_THREADS);
-  cfg.dynamicSmemBytes = ints * 4;
+  cfg.dynamicSmemBytes = kv::assign_ints(num_requests, capacity) * 4;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -534,9 +545,11 @@ extern "C" int kd_kv_release(int32_t* table, int64_t ld_table, int table_width, 
   if (!table || !lens || !keep || !free_blocks || !free_count)
     return set_error(KD_ERR_ARGUMENT, "kv_release: null pointer");
   const kv::ReleaseArgs a{table, ld_table, table_width, lens, keep, num_requests, free_blocks, capacity, free_count};
-  const int ints = 2 * num_requests + kv::seen_words(capacity);
-  if (int rc = kv::table_smem(ints, (const void*)kv::release_kernel, "kv_release: shared memory")) return rc;
-  kv::release_kernel<<<1, kv::TABLE_THREADS, ints * 4, stream>>>(a);
+  static bool configured[64] = {false};
+  if (int rc = kv::table_smem(kv::release_ints(kv::MAX_REQUESTS, 0x7fffffff), (const void*)kv::release_kernel,
+                              configured, "kv_release: shared memory"))
+    return rc;
+  kv::release_kernel<<<1, kv::TABLE_THREADS, kv::release_ints(num_requests, capacity) * 4, stream>>>(a);
   return record_cuda_error(cudaGetLastError(), "kv_release: launch");
 }
 

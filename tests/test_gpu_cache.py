@@ -68,6 +68,32 @@ def test_assign_and_its_inverse(name, pad):
     assert table.tolist() == rows and height.tolist() == [count, 0] and stack.tolist() == free
 
 
+def test_tables_of_the_most_requests():
+    """Counts around the 48 KB of shared memory that a launch has without asking (with its static arrays: 4,085 to 4,095
+    requests for the assignment, 6,127 to 6,143 for the release), up to the most; smaller ones first, so that no larger
+    call has asked before."""
+    for n in (4084, 4085, 4095, 4096, 6126, 6127, 6128, 6143, 6144):
+        lens, new = [0] * n, [0] * n
+        new[n // 2], new[n - 1] = 70, 3
+        table, stack, height = ints([[-1] * 2] * n), ints(list(range(32))), ints([32, 0])
+        got = ops.kv_assign(ints(lens), ints(bounds(new)), table, stack, height, 73)
+        want = ref.assign(lens, new, [[-1] * 2] * n, list(range(32)), 32, 2)
+        assert [x.tolist() for x in got] == list(want[:3]) and table.tolist() == want[3] and height.tolist() == [29, 0]
+        ops.kv_release(table, got[0], ints(lens), stack, height)
+        assert (table == -1).all() and stack.tolist() == list(range(32)) and height.tolist() == [32, 0]
+    n = 16384
+    g = np.random.default_rng(7)
+    lens, new = g.integers(0, 130, n).tolist(), g.integers(0, 70, n).tolist()
+    need = sum(-(-(a + b) // BLOCK) - -(-a // BLOCK) for a, b in zip(lens, new))
+    rows, free, count = dealt(lens, new, 4, need + 3)
+    table, stack, height = ints(rows), ints(free), ints([count, 0])
+    got = ops.kv_assign(ints(lens), ints(bounds(new)), table, stack, height, sum(new))
+    want = ref.assign(lens, new, rows, free, count, 4)
+    assert [x.tolist() for x in got] == list(want[:3]) and table.tolist() == want[3] and height.tolist() == [3, 0]
+    ops.kv_release(table, got[0], ints(lens), stack, height)
+    assert table.tolist() == rows and stack.tolist() == free and height.tolist() == [count, 0]
+
+
 def test_assign_takes_nothing_when_blocks_are_missing():
     lens, new = [70, 0, 10], [200, 65, 4]
     rows, free, count = dealt(lens, new, 8, 4)  # 3 + 2 + 0 new blocks, 4 free
