@@ -264,9 +264,10 @@ int kd_kv_assign(const int32_t* lens, const int32_t* cu, int num_requests, int64
                  int32_t* kv_len, int64_t* seqpos, int64_t* slots, cudaStream_t stream);
 
 /* The inverse: the blocks that hold none of request i's first keep[i] tokens (of lens[i]) return to the stack, the last
- * request's last block first, and their table entries become -1. lens is not written. free_count[1]: 0, or
+ * request's last block first, and their table entries become -1. lens is not written. free_count[1] becomes
  * KD_KV_MALFORMED (an entry outside the pool, one block named twice among those given back, a stack without room: nothing
- * is given back). A block that another request keeps must not be given back. */
+ * is given back) or stays what the assignment before it left, so that a step of assignment, write, attention and release
+ * still shows its failure at the end. A block that another request keeps must not be given back. */
 int kd_kv_release(int32_t* table, int64_t ld_table, int table_width, const int32_t* lens, const int32_t* keep,
                   int num_requests, int32_t* free_blocks, int capacity, int32_t* free_count, cudaStream_t stream);
 

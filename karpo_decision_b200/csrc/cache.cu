@@ -218,7 +218,8 @@ struct ReleaseArgs {
 
 // The blocks past each request's first `keep` tokens go back on the stack, the last request's last block first: an
 // assignment followed by its release leaves the stack as it was. One CTA: the first pass checks every entry, so a table
-// with an id outside the pool, or with one named twice among those given back, gives nothing back.
+// with an id outside the pool, or with one named twice among those given back, gives nothing back. The outcome word keeps
+// what the assignment before it left there, so that a failure survives the sequence of one step.
 __global__ void __launch_bounds__(TABLE_THREADS) release_kernel(ReleaseArgs a) {
   extern __shared__ int smem[];
   int* s_base = smem;           // [n]
@@ -274,8 +275,10 @@ __global__ void __launch_bounds__(TABLE_THREADS) release_kernel(ReleaseArgs a) {
     }
   }
   if (tid == 0) {
-    if (ok) a.count[0] = have_free + dropped;
-    a.count[1] = ok ? 0 : KD_KV_MALFORMED;
+    if (ok)
+      a.count[0] = have_free + dropped;
+    else
+      a.count[1] = KD_KV_MALFORMED;
   }
 }
 

@@ -506,7 +506,7 @@ def kv_release(table: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor, free
                ) -> None:
     """Gives the blocks past each request's first ``keep`` tokens (of ``lens``) back to the stack, undoing a
     ``kv_assign`` exactly; ``lens`` is not written. No two requests may share a block given back (KV_MALFORMED, and nothing
-    is), nor may another request keep one."""
+    is), nor may another request keep one. Otherwise ``count[1]`` stays what the ``kv_assign`` before left there."""
     n, index = lens.numel(), lens.get_device()
     _require(index >= 0, "lens must be on a CUDA device")
     _int32s(lens, n, "lens", index)

@@ -245,6 +245,21 @@ def test_release_onto_a_full_stack_gives_nothing_back():
     assert height.tolist() == [4, ops.KV_MALFORMED] and table.tolist() == [[3, 4, 5]]
 
 
+@pytest.mark.parametrize("free,outcome", [(2, 1), (9, ops.KV_TABLE_FULL)])
+def test_a_failed_assignment_shows_after_its_release(free, outcome):
+    """A step of assignment and release that takes nothing and gives nothing back; the next assignment clears the word."""
+    lens, width = ints([70, 10]), 3 if outcome > 0 else 2
+    rows = [[20, 21] + [-1] * (width - 2), [22] + [-1] * (width - 1)]
+    table, stack, height = ints(rows), ints(list(range(free)) + [-1] * (30 - free)), ints([free, 0])
+    kv_len, _, slots = ops.kv_assign(lens, ints([0, 100, 230]), table, stack, height, 230)
+    ops.kv_release(table, kv_len, lens, stack, height)
+    assert (slots == -1).all() and height.tolist() == [free, outcome] and table.tolist() == rows
+    ops.kv_release(table[:0], kv_len[:0], lens[:0], stack, height)
+    assert height.tolist() == [free, outcome]
+    kv_len, _, _ = ops.kv_assign(lens, ints([0, 50, 60]), table, stack, height, 60)
+    assert height.tolist() == [free, 0]
+
+
 # ------------------------------------------------------------------------------------------------ the write
 
 
