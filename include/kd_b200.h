@@ -291,9 +291,11 @@ int kd_attention_cache_workspace(int num_requests, int max_q, int64_t total_q, i
 /* Attention of new rows over their requests' cached tokens, the visibility rule and the gate of kd_attention_varlen with
  * Lk = kv_len[i] (new rows stored first: a causal row sees itself). q (total_q, heads_q, head_dim) bf16; cu_q int32
  * [requests + 1], kv_len int32 [requests] and the table are read when the kernel runs; max_q bounds every request's
- * rows. out rows outside every request are left as they were; a row that sees no key is 0. Bounds that fall anywhere
- * (kd_kv_assign reports them) make a launch that computes nothing. A table entry outside the pool hides its block's
- * tokens. out = bf16(o * sigmoid(gate)) with a gate (one rounding). head_dim 64, 128, 256, 512. */
+ * rows. out rows outside every request are left as they were; a row that sees no key is 0, and one with an infinity or a
+ * NaN in its query is NaN where it sees any. Finite scores (scale q.k log2 e) must stay within 2^22, where float32 still
+ * tells them apart by a half. Bounds that fall anywhere (kd_kv_assign reports them) make a launch that computes nothing.
+ * A table entry outside the pool hides its block's tokens. out = bf16(o * sigmoid(gate)) with a gate (one rounding).
+ * head_dim 64, 128, 256, 512. */
 int kd_attention_cache(const void* q, int64_t ldq, const void* k_codes, const void* v_codes, const float* k_scale,
                        const float* v_scale, int64_t num_blocks, const int32_t* table, int64_t ld_table,
                        int table_width, const int32_t* cu_q, const int32_t* kv_len, int num_requests, int max_q,

@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
       const int tok = r / a.group;
       const __nv_bfloat16* src = a.q + (int64_t)(c.x.r.q0 + tok) * a.ldq + (int64_t)(c.h * a.group + r - tok * a.group) * HD;
       uint4 w[PIECES];
-      uint32_t top = 0;  // the largest finite magnitude as a bf16 pattern
+      uint32_t top = 0;  // the largest magnitude as a bf16 pattern
 #pragma unroll
       for (int u = 0; u < PIECES; ++u) {
         const int d8 = u * LPR + first;
@@ -437,15 +437,14 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
       for (int u = 0; u < PIECES; ++u) {
         const uint32_t x[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t v0 = x[e] & 0x7fffu, v1 = (x[e] >> 16) & 0x7fffu;
-          top = max(top, max(v0 < 0x7f80u ? v0 : 0u, v1 < 0x7f80u ? v1 : 0u));
-        }
+        for (int e = 0; e < 4; ++e) top = max(top, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
       }
 #pragma unroll
       for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       const int e = max((int)(top >> 7) - 127, -120);
-      const float inv = pow2i(-e);
+      // An infinity or a NaN makes every element NaN, so that the row is NaN wherever it sees a key: an infinity's own
+      // scores may all be -inf, which would read as nothing seen.
+      const float inv = top >= 0x7f80u ? __int_as_float(0x7fffffff) : pow2i(-e);
       if (first == 0) s_qscale[team][rr] = pow2i(e) * a.scale_log2;
 #pragma unroll
       for (int u = 0; u < PIECES; ++u) {

@@ -647,7 +647,6 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
       const int n = w.n;
       const bool live = r < w.rows, warp_live = warp * 32 < w.rows;
       float q_scale = 1.f;
-      bool bad = false;  // an infinity or a NaN among the row's queries: NaN wherever it sees a key
       if (n > 0) {
         // The row's queries as hi + lo. The last item's products have read theirs: its last scores were waited for.
         if (warp_live) {
@@ -669,11 +668,11 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
               for (int e = 0; e < 4; ++e) top = max(top, max(v[e] & 0x7fffu, (v[e] >> 16) & 0x7fffu));
             }
           }
-          bad = top >= 0x7f80u;
           // the least e with the largest magnitude within 448 = 1.75 * 2^8
           const int e = min(max((int)(top >> 7) - 127 - 8 + ((top & 0x7fu) > 0x60u ? 1 : 0), -120), 120);
           q_scale = pow2i(e);
-          const float inv = pow2i(-e);
+          // An infinity or a NaN makes every element NaN: the row is NaN wherever it sees a key.
+          const float inv = top >= 0x7f80u ? __int_as_float(0x7fffffff) : pow2i(-e);
 #pragma unroll
           for (int c0 = 0; c0 < PIECES; c0 += HELD) {
             if (c0 > 0) {
@@ -843,7 +842,6 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
         tc_fence_after();
       }
       if (warp_live) {
-        if (bad && l != 0.f) l = __int_as_float(0x7fffffff);
         const float base = m == -INFINITY ? 0.f : m, vbase = big == -INFINITY ? 0.f : big;
         const int gr = w.r0 + (live ? r : 0), tok = gr / a.group, head = w.h * a.group + gr - tok * a.group;
         const uint32_t o_addr = lane_base + C::O_COL;

@@ -527,6 +527,35 @@ def test_a_nan_token_reaches_only_rows_that_see_it():
     assert nan[120:161].all() and not nan[:120].any() and not nan[161:].any()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("rows", [1, 3, 40])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_a_query_that_is_not_finite_makes_its_row_nan(hd, rows, value):
+    """Also where every score is -inf (the keys are positive at that place); rows that see nothing stay 0, others are not
+    touched. The cases span the tiles of 8 and 16 rows and of 128, states of one tile and of several shares."""
+    for lens in ([rows, 5, 30], [70, 64, 9001], [1, 1, 300]):
+        cache, table, q, _ = make(lens, [rows] * 3, 4, 1, hd)
+        for codes in (cache.k[..., 3], cache.k[..., hd - 1]):
+            codes.view(torch.uint8)[:] = 0x40  # 2
+        q[::2, 1, 3], q[::2, 3, hd - 1] = value, value
+        out = ops.attention_cache(q, cache, table, ints(bounds([rows] * 3)), ints(lens), rows, 0.1, (-1, 0))
+        ops.check_status(DEV)
+        out = out.float().unflatten(1, (4, hd))
+        clean = q.clone()
+        clean[::2, 1::2] = 0
+        want = ops.attention_cache(clean, cache, table, ints(bounds([rows] * 3)), ints(lens), rows, 0.1, (-1, 0))
+        want = want.float().unflatten(1, (4, hd))
+        for i, n in enumerate(lens):
+            for r in range(rows):
+                at = i * rows + r
+                seen = r + n - rows >= 0
+                assert torch.equal(out[at, ::2], want[at, ::2])
+                if at % 2 == 0 and seen:
+                    assert out[at, 1::2].isnan().all(), (lens, i, r)
+                else:
+                    assert torch.equal(out[at, 1::2], want[at, 1::2]) and (seen or not out[at].any())
+
+
 def test_strides_and_rows_behind_the_last_request():
     """q, gate and out as columns of wider buffers, a table with a row stride, rows of padding left as they were."""
     lens, new = [300, 77], [5, 20]
