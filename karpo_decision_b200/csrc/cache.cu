@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(TABLE_THREADS) assign_kernel(AssignArgs a) {
     if (i < a.n) {
       const int len = s_len[i];
       const int64_t grown = (int64_t)s_cu[i + 1] - s_cu[i];
-      const bool malformed = len < 0 || grown < 0 || s_cu[i] < 0 || s_cu[i + 1] > a.rows;
+      const bool malformed = len < 0 || grown < 0 || s_cu[i] < 0 || s_cu[i + 1] > a.rows || len + grown > 0x7fffffff;
       if (malformed) {
         atomicMin(&s_bad, KD_KV_MALFORMED);
       } else if ((len + grown + BLOCK - 1) / BLOCK > a.width) {

@@ -118,6 +118,21 @@ def test_assign_refuses_on_the_device(lens, cu, width, outcome):
     assert kv_len.tolist() == lens and set(slots.tolist()) == {-1}
 
 
+@pytest.mark.parametrize("rows,outcome", [(7, 0), (8, ops.KV_MALFORMED)])
+def test_assign_to_the_last_length_an_int32_holds(rows, outcome):
+    """A table wide enough for 2^31 tokens: up to 2^31 - 1 of them, the next one is refused."""
+    n = 2 ** 31 - 8
+    table = torch.full((1, 2 ** 25), 3, dtype=torch.int32, device=DEV)
+    stack, height = ints([0, 1, 2, -1, -1]), ints([3, 0])
+    kv_len, seqpos, slots = ops.kv_assign(ints([n]), ints([0, rows]), table, stack, height, rows)
+    assert height.tolist() == [3, outcome]
+    if outcome == 0:
+        assert kv_len.item() == n + rows and seqpos.tolist() == list(range(n, n + rows))
+        assert slots.tolist() == [3 * BLOCK + 56 + i for i in range(rows)]
+    else:
+        assert kv_len.item() == n and (slots == -1).all()
+
+
 @pytest.mark.parametrize("bad", [-1, 40, -2 ** 31, 2 ** 31 - 1])
 @pytest.mark.parametrize("where", ["half-filled block", "top of the stack", "deep in the stack"])
 def test_assign_refuses_ids_outside_the_pool(bad, where):
