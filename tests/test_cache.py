@@ -82,6 +82,30 @@ def test_the_wrappers_check_types_shapes_and_devices():
         ops.KVBlocks(cache.k[:, :, :32], cache.v[:, :, :32], cache.k_scale, cache.v_scale)
 
 
+@pytest.mark.parametrize("current,switched", [(0, []), (1, [0])])
+def test_a_call_goes_to_its_tensors_device(monkeypatch, current, switched):
+    """With another device current, the wrapper's call runs with the tensors' one current, on that one's stream."""
+    device, seen, calls = [current], [], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            seen.append(self.index)
+            self.before, device[0] = device[0], self.index
+
+        def __exit__(self, *error):
+            device[0] = self.before
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: device[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 1000 + index, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(ops, "call", lambda name, *args: calls.append((name, args, device[0])))
+    ops._call_on(0, "kd_kv_release", 7, 8)
+    assert calls == [("kd_kv_release", (7, 8, 1000), 0)] and seen == switched and device == [current]
+
+
 def test_the_restatement_rounds_as_torch_does():
     x = torch.cat([torch.linspace(-460, 460, 4001, dtype=torch.float64), torch.logspace(-4, 2, 3001, dtype=torch.float64)])
     want = x.float().clamp(-448, 448).to(torch.float8_e4m3fn).double()

@@ -495,6 +495,98 @@ def test_absent_blocks_are_not_seen():
     check_attention([500, 130], [3, 40], 4, 2, 128, table=holes)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("hq,hkv", [(4, 1), (2, 2), (6, 3)])
+@pytest.mark.parametrize("window", [(-1, -1), (20, 0), (0, 0), (0, 3), (63, 5), (200, -1), (5000, 5000)])
+def test_few_rows_and_their_windows(hd, hq, hkv, window):
+    """The kernel for up to 16 rows a head, under the windows that questions are tested with: whole, to both sides."""
+    check_attention([40, 129, 700, 64, 1500, 2], [2, 1, 4, 0, 3, 4], hq, hkv, hd, window, gated=hq == 4)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("window", [(-1, 0), (7, 0)])
+def test_few_rows_that_see_nothing_are_zero(hd, window):
+    """As for questions: no cached token, fewer cached tokens than rows, a state whose blocks are all absent."""
+    got = check_attention([0, 3, 70, 65], [2, 4, 1, 1], 4, 1, hd, window, gated=True,
+                          table=lambda t: torch.cat([t[:2], torch.full_like(t[2:3], -1), t[3:]]))
+    assert not got[:3].any() and not got[6].any() and got[3:6].any(1).all() and got[7].any()
+    assert not check_attention([0, 0], [1, 3], 4, 1, hd, window).any()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+def test_few_rows_do_not_see_absent_blocks(hd):
+    """Holes in the middle of a state, at its end (where the rows are), and in one that several CTAs share."""
+    def holes(t):
+        t = t.clone()
+        t[0, 1], t[0, 4], t[1, 0], t[2, 0] = -1, 10 ** 9, -5, t.max() + 100
+        t[3, ::3], t[3, 1::7] = -1, 2 ** 31 - 1
+        return t
+
+    check_attention([500, 130, 65, 30000], [3, 1, 1, 2], 4, 1, hd, table=holes)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("more", [0, 9000])
+def test_a_nan_token_reaches_only_the_few_rows_that_see_it(hd, more):
+    """A NaN in a value, seen by the first of two rows through its window; head 0 has none. Also in a longer state, whose
+    other tiles are finite."""
+    n = 200 + more
+    cache = ops.kv_blocks(n // BLOCK + 3, 2, hd, DEV)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(2)
+    k, v = (torch.randn(n, 2, hd, generator=g, device=DEV).bfloat16() for _ in range(2))
+    q = torch.randn(2, 2, hd, generator=g, device=DEV).bfloat16()
+    v[120, 1, 7] = math.nan
+    table = torch.randperm(n // BLOCK + 1, generator=g, device=DEV).int()[None, :]
+    t = torch.arange(n, device=DEV)
+    ops.kv_store_e4m3(k, v, ints([0, n]), table[0].long()[t // 64] * 64 + t % 64, cache)
+    # the rows' positions are n - 2 and n - 1; the window's first key is 120 for the first of them, 121 for the second
+    out = ops.attention_cache(q, cache, table, ints([0, 2]), ints([n]), 2, 0.1, (n - 122, 0)).float()
+    assert torch.isfinite(out[:, :hd]).all() and out[0, hd:].isnan().all() and torch.isfinite(out[1, hd:]).all()
+
+
+def test_few_rows_strides_and_rows_behind_the_last_request():
+    """q, gate and out as columns of wider buffers, a table with a row stride, rows of padding left as they were."""
+    lens, new = [300, 77], [1, 4]
+    cache, table, q, gate = make(lens, new, 4, 1, 64, pad=7)
+    wide = torch.zeros(2, 40, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    qs = torch.zeros(12, 768, dtype=torch.bfloat16, device=DEV)
+    gs, outs = torch.zeros_like(qs), torch.full_like(qs, 5.0)
+    qs[:, 256:512], gs[:, 512:] = q.reshape(12, 256), gate
+    args = (ints(bounds(new)), ints(lens), 4, 0.125, (-1, 0))
+    want = ops.attention_cache(q, cache, table, *args, gate=gate)
+    got = ops.attention_cache(qs[:, 256:512].unflatten(1, (4, 64)), cache, wide[:, :table.shape[1]], *args,
+                              gate=gs[:, 512:], out=outs[:, 256:512])
+    assert torch.equal(got[:5], want[:5])
+    assert (outs[5:] == 5).all() and (outs[:, :256] == 5).all() and (outs[:, 512:] == 5).all()
+
+
+@pytest.mark.parametrize("rows", [1, 30])
+def test_a_pool_past_four_gigabytes(rows):
+    """Blocks whose codes lie past 2^32 bytes: written and read as in a small pool, bit by bit."""
+    blocks, heads, hd, n = 70000, 8, 128, 300
+    shape = (blocks, heads, BLOCK, hd)
+    k, v = (torch.empty(shape, dtype=torch.float8_e4m3fn, device=DEV) for _ in range(2))
+    big = ops.KVBlocks(k, v, *(torch.ones(blocks, heads, device=DEV) for _ in range(2)))
+    small = ops.kv_blocks(5, heads, hd, DEV)
+    ids = torch.tensor([69999, 3, 66000, 69998, 32768], device=DEV)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(3)
+    rows_k, rows_v = (torch.randn(n, heads, hd, generator=g, device=DEV).bfloat16() for _ in range(2))
+    q = torch.randn(rows, 2 * heads, hd, generator=g, device=DEV).bfloat16()
+    at = torch.arange(n, device=DEV)
+    outs = []
+    for cache, order in ((big, ids), (small, torch.arange(5, device=DEV))):
+        ops.kv_store_e4m3(rows_k, rows_v, ints([0, n]), order[at // BLOCK] * BLOCK + at % BLOCK, cache)
+        outs.append(ops.attention_cache(q, cache, order.int()[None, :], ints([0, rows]), ints([n]), rows, 0.1, (-1, 0)))
+    held = torch.arange(5 * BLOCK, device=DEV).reshape(5, 1, BLOCK, 1) < n
+    for x, y in ((big.k, small.k), (big.v, small.v)):
+        assert torch.equal(torch.where(held, x[ids].view(torch.uint8), 0), torch.where(held, y.view(torch.uint8), 0))
+    assert torch.equal(big.k_scale[ids], small.k_scale) and torch.equal(big.v_scale[ids], small.v_scale)
+    assert torch.equal(*outs) and torch.isfinite(outs[0]).all()
+
+
 @pytest.mark.parametrize("new", [[1, 1], [30, 41]])
 def test_scales_far_apart(new):
     """Blocks whose value scales differ by up to 2^40 or so: the largest values need not have the largest probability."""
@@ -716,3 +808,123 @@ def test_a_captured_step_follows_the_lengths_on_the_device():
                                          [0, 1, 2, 3], [i + 1] * n, hd ** -0.5, (-1, 0))
             tol = tolerance(want, spread, size, hd, 130)
             assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+def test_captured_questions_follow_the_bounds_on_the_device(hd):
+    """One graph of assign, store, attend and release for up to 64 rows of 3 requests, padding behind them: replayed with
+    other questions each time, and with one too many for the pool, whose failure shows at the end."""
+    hq, hkv, rows, width = 4, 2, 64, 12
+    lens0 = [100, 640, 64]
+    cache, table, _, _ = make(lens0, [0, 0, 0], hq, hkv, hd)
+    have = [-(-n // BLOCK) for n in lens0]
+    blocks = cache.blocks
+    rows_ = [table[i, :h].tolist() for i, h in enumerate(have)]
+    taken = {x for r in rows_ for x in r}
+    free = [i for i in range(blocks) if i not in taken]  # three blocks
+    table = ints([r + [-1] * (width - len(r)) for r in rows_])
+    stack, height = ints(free + [-1] * (blocks - len(free))), ints([len(free), 0])
+    lens, cu, kv_len = ints(lens0), ints([0, 20, 20, 45]), ints(lens0)
+    q = torch.zeros(rows, hq, hd, dtype=torch.bfloat16, device=DEV)
+    k, v = (torch.zeros(rows, hkv, hd, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    seqpos, slots = (torch.zeros(rows, dtype=torch.int64, device=DEV) for _ in range(2))
+    out = torch.zeros(rows, hq * hd, dtype=torch.bfloat16, device=DEV)
+
+    def step():
+        ops.kv_assign(lens, cu, table, stack, height, rows, out=(kv_len, seqpos, slots))
+        ops.kv_store_e4m3(k, v, cu, slots, cache)
+        ops.attention_cache(q, cache, table, cu, kv_len, 40, hd ** -0.5, (-1, 0), out=out)
+        during.copy_(table)
+        ops.kv_release(table, kv_len, lens, stack, height)
+
+    during = torch.zeros_like(table)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    g = torch.Generator(device=DEV)
+    g.manual_seed(5)
+    for new, fails in (([20, 0, 25], 0), ([1, 1, 1], 0), ([40, 20, 4], 0), ([0, 40, 1], 0), ([0, 0, 0], 0),
+                       ([64, 0, 0], 0), ([30, 33, 1], 0)):
+        cu.copy_(ints(bounds(new)))
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=g, device=DEV))
+        out.fill_(7.0)
+        graph.replay()
+        n = sum(new)
+        grown = [a + b for a, b in zip(lens0, new)]
+        assert kv_len.tolist() == grown and height.tolist() == [len(free), fails] and stack.tolist()[:len(free)] == free
+        want, spread, size = ref.attention(q, cache.k.double(), cache.v.double(), cache.k_scale, cache.v_scale, during,
+                                     bounds(new), grown, hd ** -0.5, (-1, 0))
+        err, tol = (out.double() - want).abs(), tolerance(want, spread, size, hd, max(grown))
+        assert (err[:n] <= tol[:n]).all() and (out[n:] == 7).all()
+    height[0] = 1
+    cu.copy_(ints([0, 30, 60, 64]))  # three blocks: 100 + 30, 640 + 30 and 64 + 4 tokens
+    graph.replay()
+    assert height.tolist() == [1, 2] and kv_len.tolist() == lens0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_questions_on_one_state(hd):
+    """Four questions on one state in one pack. The state ends with its block, so its blocks are shared and stay as they
+    are bit by bit; the tokens behind its last whole block go in front of each question. The same questions one to a pack,
+    too: each pack's answers against the definition."""
+    hq, hkv, whole, tail, asks = 4, 2, 256, 37, [5, 20, 1, 64]
+    g = torch.Generator(device=DEV)
+    g.manual_seed(6)
+
+    def normal(n, heads):
+        return torch.randn(n, heads, hd, generator=g, device=DEV).bfloat16()
+
+    state_k, state_v = normal(whole, hkv), normal(whole, hkv)
+    new = [tail + n for n in asks]
+    q, k, v = normal(sum(new), hq), normal(sum(new), hkv) * 3, normal(sum(new), hkv) * 100
+    cache = pool(40, hkv, hd, 9)
+    table, stack, height = ints([[-1] * 6] * 4), ints(list(range(40))), ints([40, 0])
+    none = ints([0])
+    state, _, slots = ops.kv_assign(none, ints([0, whole]), table[:1], stack, height, whole)
+    ops.kv_store_e4m3(state_k, state_v, ints([0, whole]), slots, cache)
+    table[1:] = table[0]
+    lens, before = ints([whole] * 4), table.clone()
+    ids = table[0, :whole // BLOCK].long()
+    held = [x[ids].clone().view(torch.uint8) for x in (cache.k, cache.v)] + [cache.k_scale[ids], cache.v_scale[ids]]
+    outs = []
+    for picks in ([0, 1, 2, 3], [0], [1], [2], [3]):
+        sizes = [new[i] for i in picks]
+        at = torch.cat([torch.arange(bounds(new)[i], bounds(new)[i + 1], device=DEV) for i in picks])
+        cu, t = ints(bounds(sizes)), table[picks[0]:picks[-1] + 1]
+        kv_len, _, slots = ops.kv_assign(lens[picks[0]:picks[-1] + 1], cu, t, stack, height, sum(sizes))
+        assert height[1].item() == 0
+        ops.kv_store_e4m3(k[at], v[at], cu, slots, cache)
+        outs.append(ops.attention_cache(q[at], cache, t, cu, kv_len, 101, 0.1, (-1, 0)))
+        want, spread, size = ref.attention(q[at], cache.k.double(), cache.v.double(), cache.k_scale, cache.v_scale, t,
+                                           bounds(sizes), kv_len.tolist(), 0.1, (-1, 0))
+        assert ((outs[-1].double() - want).abs() <= tolerance(want, spread, size, hd, whole + 101)).all()
+        ops.kv_release(t, kv_len, lens[picks[0]:picks[-1] + 1], stack, height)
+        assert torch.equal(table, before)
+        after = [x[ids].view(torch.uint8) for x in (cache.k, cache.v)] + [cache.k_scale[ids], cache.v_scale[ids]]
+        assert all(torch.equal(x, y) for x, y in zip(held, after))
+
+
+def test_a_question_leaves_its_scale_in_a_half_filled_block():
+    """What a release does not give back: rows that share a state's last block may have made its scale grow, and the
+    state's codes there stay rounded to it, each once (to nearest even), until the block is written anew."""
+    cache = ops.kv_blocks(2, 1, 64, DEV)
+    table, stack, height = ints([[-1, -1]]), ints([0, 1]), ints([2, 0])
+    g = torch.Generator(device=DEV)
+    g.manual_seed(7)
+    small = torch.randn(40, 1, 64, generator=g, device=DEV).bfloat16()
+    lens, _, slots = ops.kv_assign(ints([0]), ints([0, 40]), table, stack, height, 40)
+    ops.kv_store_e4m3(small, small, ints([0, 40]), slots, cache)
+    block = table[0, 0].item()
+    values, scale = cache.k[block, 0, :40].double(), cache.k_scale[block, 0].item()
+    kv_len, _, slots = ops.kv_assign(lens, ints([0, 10]), table, stack, height, 10)
+    ops.kv_store_e4m3(small[:10] * 64, small[:10] * 64, ints([0, 10]), slots, cache)
+    ops.kv_release(table, kv_len, lens, stack, height)
+    grown = cache.k_scale[block, 0].item()
+    assert grown > scale and height.tolist() == [1, 0]
+    assert torch.equal(cache.k[block, 0, :40].double(), ref.to_e4m3(values * scale / grown))
