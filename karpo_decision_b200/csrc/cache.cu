@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(TABLE_THREADS) release_kernel(ReleaseArgs a) {
   const int tid = threadIdx.x;
   if (tid == 0) s_bad = 0;
   const int have_free = a.count[0];
+  for (int w = tid; w < words; w += TABLE_THREADS) s_seen[w] = 0;
   __syncthreads();
   int carry = 0;
   for (int i0 = 0; i0 < a.n; i0 += TABLE_THREADS) {
@@ -255,8 +256,10 @@ __global__ void __launch_bounds__(TABLE_THREADS) release_kernel(ReleaseArgs a) {
   const bool sized = s_bad == 0 && have_free >= 0 && (int64_t)have_free + dropped <= a.capacity;
   if (sized) {
     for (int from = 0; from < a.capacity && from >= 0; from += SEEN_BLOCKS) {
-      for (int w = tid; w < words; w += TABLE_THREADS) s_seen[w] = 0;
-      __syncthreads();
+      if (from > 0) {
+        for (int w = tid; w < words; w += TABLE_THREADS) s_seen[w] = 0;
+        __syncthreads();
+      }
       for (int j = tid; j < dropped; j += TABLE_THREADS) {
         const int i = last_at_most(s_base, a.n, j);
         const int id = a.table[(int64_t)i * a.ldt + s_from[i] + j - s_base[i]];

@@ -748,7 +748,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
 // fewer, several warps share a row and each takes every WPR-th partial. The lanes read all the partials' statistics of the
 // row together, then four columns each of the partials, in key order, eight loads in flight.
 template <int HD, int NT>
-__global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
+__global__ void __launch_bounds__(256) join_kernel(Args a) {
   using C = Cfg<HD, NT>;
   constexpr int RT = C::RT, CW = HD <= 128 ? 1 : HD / 128, RB = 8 / CW, V = HD == 64 ? 2 : 4;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
@@ -941,7 +941,8 @@ int launch(Args a, const void* k_codes, const void* v_codes, uint8_t* ws, int64_
   kernel<<<ctas, C::THREADS, C::SMEM, stream>>>(mk, mv, a);
   rc = record_cuda_error(cudaGetLastError(), "attention_cache: launch");
   if (rc) return rc;
-  return launch_after(join_kernel<HD, NT>, dim3((unsigned)items, C::RT * HD / (HD <= 128 ? 8 * HD : 1024)), 256, stream, a, ctas);
+  return launch_after(join_kernel<HD, NT>, dim3((unsigned)items, C::RT * HD / (HD <= 128 ? 8 * HD : 1024)), 256, stream,
+                      a);
 }
 
 // f(head dim, 8-row tiles) with both as constants.

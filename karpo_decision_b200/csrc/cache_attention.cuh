@@ -114,7 +114,7 @@ KD_DEVICE void set_registers_down() {
 // Launches the joining kernel so that its blocks are in place when the kernel before it in the stream ends (it waits for
 // that itself, by griddepcontrol.wait).
 template <typename K>
-int launch_after(K kernel, dim3 grid, int threads, cudaStream_t stream, const Args& a, int ctas) {
+int launch_after(K kernel, dim3 grid, int threads, cudaStream_t stream, const Args& a) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -124,7 +124,7 @@ int launch_after(K kernel, dim3 grid, int threads, cudaStream_t stream, const Ar
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return record_cuda_error(cudaLaunchKernelEx(&cfg, kernel, a, ctas), "attention_cache: join launch");
+  return record_cuda_error(cudaLaunchKernelEx(&cfg, kernel, a), "attention_cache: join launch");
 }
 
 // The kernel for many rows per key/value head (cache_attention_tiles.cu).

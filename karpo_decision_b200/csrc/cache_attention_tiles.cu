@@ -955,7 +955,7 @@ done:
 constexpr int JOIN_MOST = 320;  // partials of an item: at most the CTAs
 constexpr int JOIN_FEW = 16;
 template <int HD, int DV>
-__global__ void __launch_bounds__(2 * DV) join_tiles_kernel(Args a, int ctas) {
+__global__ void __launch_bounds__(2 * DV) join_tiles_kernel(Args a) {
   using C = Cfg<HD, DV>;
   constexpr int GROUPS = 2 * DV / 8;  // threads that share a row
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the partials are there after this
@@ -1123,7 +1123,7 @@ int launch(Args a, const void* k_codes, const uint8_t* v_codes, uint8_t* ws, int
     return rc;
   kernel<<<ctas, C::THREADS, C::SMEM, stream>>>(mk, a, v_codes);
   if (int rc = record_cuda_error(cudaGetLastError(), "attention_cache: launch")) return rc;
-  return launch_after(join_tiles_kernel<HD, DV>, dim3(ctas, 16), 2 * DV, stream, a, ctas);
+  return launch_after(join_tiles_kernel<HD, DV>, dim3(ctas, 16), 2 * DV, stream, a);
 }
 
 }  // namespace ct
