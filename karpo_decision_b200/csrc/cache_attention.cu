@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
     }
     // This producer's k-th tile is lo + k PRODUCERS + me; each lane looks up one tile's block and scales, 32 ahead.
     const uint32_t mine = hi - lo > me ? (uint32_t)((hi - lo - me + C::PRODUCERS - 1) / C::PRODUCERS) : 0;
-    uint32_t failed = 0;
+    uint32_t issued = mine;
     int z = -1, next_z = -1, ve = 0, next_ve = 0;
     float ks = 0.f, next_ks = 0.f;
     auto look_up = [&](uint32_t k) {
@@ -376,18 +376,17 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::THREADS, 1)
           }
         }
         if (!__shfl_sync(0xffffffffu, ok, 0)) {
-          failed = k0 + j;
+          issued = k0 + j;  // a consumer gave up
           goto drain;
         }
       }
     }
-    return;
   drain:
-    // A consumer gave up: wait (bounded) for this producer's copies in flight before the shared memory goes away: the last
-    // tile of each of its slots, of the `failed` that it issued.
+    // Wait (bounded) for this producer's copies in flight, the last one into each of its slots: consumers that gave up do
+    // not wait for them before the shared memory goes away.
     if (lane == 0) {
       const uint64_t start = globaltimer();
-      for (uint32_t k = failed > SLOTS / C::PRODUCERS ? failed - SLOTS / C::PRODUCERS : 0; k < failed; ++k) {
+      for (uint32_t k = issued > SLOTS / C::PRODUCERS ? issued - SLOTS / C::PRODUCERS : 0; k < issued; ++k) {
         const uint32_t at = k * C::PRODUCERS + me;
         while (!mbar_try_wait(smem_u32(&full[at % SLOTS]), (at / SLOTS) & 1) && globaltimer() - start < 1000000000ull) {
         }

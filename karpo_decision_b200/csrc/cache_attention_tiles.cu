@@ -274,7 +274,7 @@ template <int HD, int DV>
 struct Shared {
   using C = Cfg<HD, DV>;
   uint64_t q_full, k_full[C::KST], v_full[C::VST], k_empty[C::KST], v_empty[C::VST];
-  uint64_t s_full[C::NS], p_full[C::NS], pv_done[C::NS], item_full[2], item_empty[2];
+  uint64_t s_full[C::NS], p_full[C::NS], pv_done[C::NS], item_full[2], item_empty[2], drained;
   int64_t warp[C::THREADS / 32], start;
   Work works[2];
   Info info[8];           // by key tile: at most KST + NS tiles are between their load and their softmax
@@ -311,6 +311,7 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
   if (tid == 0) {
     mbar_init(&q_full, SOFT);
+    mbar_init(&sh.drained, 1);
     for (int s = 0; s < KST; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
@@ -490,8 +491,8 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
           d->rows = 0;
       }
     }
-    if (!ok && lane == 0) {
-      // another role gave up: wait (bounded) for the copies in flight before the shared memory goes away
+    if (lane == 0) {
+      // wait (bounded) for the copies in flight: roles that gave up do not before the shared memory goes away
       const uint64_t start = globaltimer();
       for (int s = 0; s < KST; ++s)
         while (issued[s] >= 0 && !mbar_try_wait(smem_u32(&k_full[s]), (uint32_t)issued[s] & 1) &&
@@ -506,13 +507,13 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
       const uint32_t sq = smem_u32(s_q);
       uint32_t g = 0, nq = 0;  // key tiles and items so far
       for (uint32_t k = 0;; ++k) {
-        if (!mbar_wait(&item_full[k & 1], (k >> 1) & 1, a.status)) goto done;
+        if (!mbar_wait(&item_full[k & 1], (k >> 1) & 1, a.status)) goto gave_up;
         const int n = works[k & 1].n;
         const bool end = works[k & 1].i < 0;
         mbar_arrive(&item_empty[k & 1]);
         if (end) break;
         if (n == 0) continue;
-        if (!mbar_wait(&q_full, nq & 1, a.status)) goto done;
+        if (!mbar_wait(&q_full, nq & 1, a.status)) goto gave_up;
         ++nq;
         auto issue_s = [&](int j) -> bool {
           const uint32_t G = g + j;
@@ -538,13 +539,13 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
           mma_commit(&s_full[G % NS]);
           return true;
         };
-        if (!issue_s(0)) goto done;
+        if (!issue_s(0)) goto gave_up;
         for (int j = 0; j < n; ++j) {
-          if (j + 1 < n && !issue_s(j + 1)) goto done;
+          if (j + 1 < n && !issue_s(j + 1)) goto gave_up;
           const uint32_t G = g + j;
           const int st = G % VST;
-          if (!mbar_wait(&p_full[G % NS], (G / NS) & 1, a.status)) goto done;
-          if (!mbar_wait(&v_full[st], (G / VST) & 1, a.status)) goto done;
+          if (!mbar_wait(&p_full[G % NS], (G / NS) & 1, a.status)) goto gave_up;
+          if (!mbar_wait(&v_full[st], (G / VST) & 1, a.status)) goto gave_up;
           tc_fence_after();
           const uint32_t sv = smem_u32(s_v + st * C::V_BYTES);
           const uint32_t p = tmem + C::S_COL + (G % NS) * BN;
@@ -556,6 +557,12 @@ __global__ void __launch_bounds__(Cfg<HD, DV>::THREADS, Cfg<HD, DV>::CTAS_PER_SM
           mma_commit(&pv_done[G % NS]);
         }
         g += n;
+      }
+    gave_up:
+      // wait (bounded) for the products in flight: roles that gave up do not before the tiles and tensor memory go away
+      mma_commit(&sh.drained);
+      const uint64_t start = globaltimer();
+      while (!mbar_try_wait(smem_u32(&sh.drained), 0) && globaltimer() - start < 1000000000ull) {
       }
     }
   } else {

@@ -726,6 +726,28 @@ def test_bounds_that_fall_compute_nothing(hd, max_q, n):
     assert (scratch[size.value:] == 0xab).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("new", [[1, 1, 2], [40, 9, 60]])
+def test_a_launch_that_gives_up_ends_by_itself(hd, new):
+    """With an error already in the status word every wait that is not over at once gives up. The launches end, write
+    nothing behind their buffers, and the next ones are right."""
+    lens = [900, 64, 30000]
+    cache, table, q, gate = make(lens, new, 8, 2, hd, pad=3)
+    args = (cache, table, ints(bounds(new)), ints(lens), max(new), 0.1, (-1, 0))
+    want = ops.attention_cache(q, *args, gate=gate)
+    word = ops.status_word(DEV)
+    for _ in range(3):
+        out = torch.full_like(want, 5.0)
+        word.fill_(_lib.KD_DEVICE_TIMEOUT)
+        ops.attention_cache(q, *args, gate=gate, out=out)
+        with pytest.raises(_lib.KernelError, match="gave up"):
+            ops.check_status(DEV)
+        assert (out[sum(new):] == 5).all()
+        got = ops.attention_cache(q, *args, gate=gate)
+        ops.check_status(DEV)
+        assert torch.equal(got[:sum(new)], want[:sum(new)])
+
+
 # ------------------------------------------------------------------------------------------------ together
 
 
