@@ -243,9 +243,10 @@ int kd_gated_norm(const void* x, int64_t ldx, const void* z, int64_t ldz, const 
 /* ---------------------------------------------------------------------------------------------- cache of states
  * Keys and values of earlier tokens kept in blocks of KD_KV_BLOCK tokens, so that a state that is asked about again runs
  * only its new rows. One layer's pool: codes k, v e4m3 [blocks][heads_kv][KD_KV_BLOCK][head_dim] (contiguous) and one
- * float32 scale per (block, head) for each, a power of two with exponent in [-100, 120]: value = code * scale. Block
- * tables int32 [requests][width] name each request's blocks in order (-1: none). No counterpart in the reference, which
- * computes every request from its first token (decider.py:110-123). */
+ * float32 scale per (block, head) for each, a power of two with exponent in [-100, 120]: value = code * scale (of a
+ * value's scale only the exponent is read). No value code of a request's tokens is NaN, as kd_kv_store_e4m3 writes them.
+ * Block tables int32 [requests][width] name each request's blocks in order (-1: none). No counterpart in the reference,
+ * which computes every request from its first token (decider.py:110-123). */
 #define KD_KV_BLOCK 64
 #define KD_KV_TABLE_FULL (-1) /* free_count[1]: a request's blocks exceed the table's width */
 #define KD_KV_MALFORMED (-2)  /* free_count[1]: lengths, bounds, count or block ids outside their ranges, an id twice */
@@ -256,29 +257,32 @@ int kd_gated_norm(const void* x, int64_t ldx, const void* z, int64_t ldz, const 
  * (kv_len may be lens), seqpos[t] the row's position in its request, slots[t] = block * KD_KV_BLOCK + place. Rows
  * outside every request (padding) get position 0 and slot -1. All or nothing: when blocks are missing nothing is taken,
  * every slot is -1 and kv_len = lens; so too when an id that the rows would use, a half-filled block's or a new one's,
- * lies outside the pool or is met twice: requests may share blocks that get no rows (a state that ends with its block),
- * not one that does. free_count[1]: 0, the number of missing blocks, or KD_KV_TABLE_FULL / KD_KV_MALFORMED. At most
- * 16,384 requests. */
+ * lies outside the pool or is met twice. Requests may share the blocks of a state that ends with its block; a half-filled
+ * block belongs to the one request that goes on in it. free_count[1]: 0, the number of missing blocks, or
+ * KD_KV_TABLE_FULL / KD_KV_MALFORMED. At most 16,384 requests. */
 int kd_kv_assign(const int32_t* lens, const int32_t* cu, int num_requests, int64_t rows, int32_t* table,
                  int64_t ld_table, int table_width, const int32_t* free_blocks, int capacity, int32_t* free_count,
                  int32_t* kv_len, int64_t* seqpos, int64_t* slots, cudaStream_t stream);
 
-/* The inverse: the blocks that hold none of request i's first keep[i] tokens (of lens[i]) return to the stack, the last
- * request's last block first, and their table entries become -1. lens is not written. free_count[1] becomes
- * KD_KV_MALFORMED (an entry outside the pool, one block named twice among those given back, a stack without room: nothing
- * is given back) or stays what the assignment before it left, so that a step of assignment, write, attention and release
- * still shows its failure at the end. A block that another request keeps must not be given back. */
+/* The inverse for tables and stack (not for codes and scales, see the write): the blocks that hold none of request i's
+ * first keep[i] tokens (of lens[i]) return to the stack, the last request's last block first, and their table entries
+ * become -1. lens is not written. free_count[1] becomes KD_KV_MALFORMED (an entry outside the pool, one block named
+ * twice among those given back, a stack without room: nothing is given back) or stays what the assignment before it
+ * left, so that a step of assignment, write, attention and release still shows its failure at the end. A block that
+ * another request keeps must not be given back. */
 int kd_kv_release(int32_t* table, int64_t ld_table, int table_width, const int32_t* lens, const int32_t* keep,
                   int num_requests, int32_t* free_blocks, int capacity, int32_t* free_count, cudaStream_t stream);
 
-/* The rows' keys and values (bf16 [rows][heads_kv][head_dim], row strides in elements) into their blocks. Per block and
- * head the scale is the least power of two that keeps the largest finite magnitude within 448 scale units; a block that
- * held earlier tokens of the request (its first new row is not the block's first) keeps the larger of its scale and the
- * new rows' own, and where it grows its earlier codes are brought to it, each rounded once to nearest even. Values
- * saturate at 448 * scale (infinities too). A token with a NaN in its key or value is stored as a NaN key (code 0x7f) and
- * a zero value: exactly the query rows that see it become NaN. A request's rows take consecutive places, as
- * kd_kv_assign makes them; requests whose first slot is negative, and rows outside every request, are not written. No
- * two requests may write one block in one call. head_dim 64, 128, 256 or 512. */
+/* The rows' keys and values (bf16 [rows][heads_kv][head_dim], row strides in elements) into their blocks. Per block
+ * and head the scale is the least power of two that keeps the largest finite magnitude within 448 scale units; a block
+ * that held earlier tokens of the request (its first new row is not the block's first) keeps the larger of its scale
+ * and the new rows' own, and where it grows its earlier codes are brought to it, each rounded once to nearest even.
+ * Giving the new rows' blocks back does not undo that: a state that has to stay as it is ends with its block, and the
+ * tokens past its last whole block go in front of the new rows each time. Values saturate at 448 * scale (infinities
+ * too). A token with a NaN in its key or value is stored as a NaN key (code 0x7f) and a zero value: exactly the query
+ * rows that see it become NaN. A request's rows take consecutive places, as kd_kv_assign makes them; requests whose
+ * first slot is negative, and rows outside every request, are not written. No two requests may write one block in one
+ * call (kd_kv_assign refuses such tables). head_dim 64, 128, 256 or 512. */
 int kd_kv_store_e4m3(const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t rows, const int32_t* cu,
                      int num_requests, const int64_t* slots, int num_heads_kv, int head_dim, void* k_codes,
                      void* v_codes, float* k_scale, float* v_scale, int64_t num_blocks, cudaStream_t stream);

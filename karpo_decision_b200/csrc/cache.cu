@@ -98,7 +98,8 @@ struct AssignArgs {
 // change after a cluster barrier, when every CTA has read them. Every CTA also looks at the ids that the rows will use,
 // the half-filled blocks' table entries during the scan and the new blocks' on the stack after it: one outside the pool,
 // or one met twice, whose rows two requests would write, refuses the call before anything is written.
-// Bound by latency: dependent reads of the lengths, one of the stack or the table, and the launch.
+// Bound by latency: dependent reads of the lengths, of the stack and of the table, and the launch. With the release after
+// it, as graph replays: one request 7.5 us, 512 requests of 45,473 rows 15.1 us (0.6 of each for the ids' checks).
 __global__ void __launch_bounds__(TABLE_THREADS) assign_kernel(AssignArgs a) {
   extern __shared__ int smem[];
   int* s_cu = smem;                // [n + 1]
@@ -352,11 +353,13 @@ KD_DEVICE bool finite_max(const uint4& x, uint32_t& top) {
 // enough places (its rows touch at most rows / 64 + 2 blocks) without a scan; each warp finds its request by probing 32
 // requests at a time.
 //
-// Bound by the reads of k and v, next to it by the instructions per element (magnitudes as two 16-bit integers to a word,
-// elements one by one only where one is not finite: 46.5 -> 38 us), then by the loads in flight: 1,280 threads an SM at 48
-// registers (38 -> 35.9 us; at 40 they spill, 40 us). 48,000 rows of 8 heads of 128: 35.9 us, 5.72 TB/s; one CTA with
-// several heads one after another, the next one's loads in flight, was slower (39 us), as were neighbouring heads first.
-// The smallest launches are a chain of dependent loads, 5.6 us.
+// Bound by the reads of k and v, next to it by the instructions per element (magnitudes as two 16-bit integers to a
+// word, elements one by one only where one is not finite: 46.5 -> 38 us), then by the loads in flight: for heads of 64
+// and 128 1,280 threads an SM at 48 registers (38 -> 35.9 us; at 40 they spill, 40 us), for heads of 256 and 512 the
+// two and the one CTA that fit, 1,024. 33,349 rows of 8 heads of 128 (205 MB): 36.1 us, 5.68 TB/s; as many bytes in 16
+// heads of 64 39 us, in 4 of 256 41 us, in 2 of 512 52 us. One CTA with several heads one after another, the next
+// one's loads in flight, was slower (39 us), as were neighbouring heads first. The smallest launches are a chain of
+// dependent loads, 5.6 us.
 template <int HD>
 __global__ void __launch_bounds__(store_threads(HD), 1280 / store_threads(HD))
     store_kernel(StoreArgs a) {

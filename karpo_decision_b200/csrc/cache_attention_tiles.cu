@@ -6,7 +6,8 @@
 // tensor memory, as in attention.cu; what differs is the operands. The keys' codes go to the tensor cores as they are
 // (kind::f8f6f4, tiles by TMA): a query row is split into two e4m3 rows, its rounding and the rest, q 2^-e = hi + lo with
 // the row's largest magnitude in (224, 448]. That is exact for every bf16 element within 2^-10 of the row's largest and
-// off by at most 2^-10 (2^-17 of the largest) below, and two products at the 8-bit rate cost what one in 16 bits does.
+// off by at most 2^-10 (2^-17 of the largest) below, and two products at the 8-bit rate cost what one in 16 bits does. (The
+// kernel for few rows holds queries in f16, 2^-25: a row with one large element may differ there in its last bits.)
 // The values meet probabilities, which need more range than e4m3 has: converter warps load a block's value codes (16
 // bytes a thread and piece, the next tile's loads in flight while one is converted, later tiles on their way into L2) and
 // write them as f16 (exact, two per instruction) into the 128-byte swizzled tiles that the descriptors name. So the codes

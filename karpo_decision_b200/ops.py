@@ -411,8 +411,8 @@ def gated_norm(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, heads: in
 
 class KVBlocks:
     """One layer's pool of cached keys and values: e4m3 codes ``k``, ``v`` (blocks, Hkv, 64, hd) and float32 power-of-two
-    scales ``k_scale``, ``v_scale`` (blocks, Hkv); value = code * scale. Checked here, once, for every call that takes
-    it."""
+    scales ``k_scale``, ``v_scale`` (blocks, Hkv); value = code * scale. Types and shapes are checked here, once, for every
+    call that takes it; that scales are powers of two is not (of a value's scale only the exponent is read)."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "blocks", "heads", "head_dim", "index")
 
@@ -505,7 +505,8 @@ def kv_assign(lens: torch.Tensor, cu: torch.Tensor, table: torch.Tensor, free: t
 def kv_release(table: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor, free: torch.Tensor, count: torch.Tensor
                ) -> None:
     """Gives the blocks past each request's first ``keep`` tokens (of ``lens``) back to the stack, undoing a
-    ``kv_assign`` exactly; ``lens`` is not written. No two requests may share a block given back (KV_MALFORMED, and nothing
+    ``kv_assign`` exactly in ``table`` and the stack (a half-filled block's scale and codes stay as its rows left them);
+    ``lens`` is not written. No two requests may share a block given back (KV_MALFORMED, and nothing
     is), nor may another request keep one. Otherwise ``count[1]`` stays what the ``kv_assign`` before left there."""
     n, index = lens.numel(), lens.get_device()
     _require(index >= 0, "lens must be on a CUDA device")
