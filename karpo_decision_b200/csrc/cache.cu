@@ -359,7 +359,7 @@ KD_DEVICE bool finite_max(const uint4& x, uint32_t& top) {
 // two and the one CTA that fit, 1,024. 33,349 rows of 8 heads of 128 (205 MB): 36.1 us, 5.68 TB/s; as many bytes in 16
 // heads of 64 39 us, in 4 of 256 41 us, in 2 of 512 52 us. One CTA with several heads one after another, the next
 // one's loads in flight, was slower (39 us), as were neighbouring heads first. The smallest launches are a chain of
-// dependent loads, 5.6 us.
+// dependent loads, 6.1 us.
 template <int HD>
 __global__ void __launch_bounds__(store_threads(HD), 1280 / store_threads(HD))
     store_kernel(StoreArgs a) {

@@ -663,6 +663,39 @@ def test_a_query_that_is_not_finite_makes_its_row_nan(hd, rows, value):
                     assert torch.equal(out[at, 1::2], want[at, 1::2]) and (seen or not out[at].any())
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("new", [[1, 2, 1], [40, 9, 60]])
+@pytest.mark.parametrize("spread", [0.0, 8.0])
+def test_scores_near_their_limit(hd, new, spread):
+    """Every row's query along one key, so that its score is about 2^21.5 in log2 units and the others' far lower: the row
+    is that key's value. Off by the output's rounding, 2^-8, and the one probability's to f16, 2^-11 (its exponent may be
+    off by a half here, in numerator and sum alike up to a float32 rounding)."""
+    lens, hkv, group = [300, 64, 9000], 2, 2
+    cache, table, q, _ = make(lens, new, hkv * group, hkv, hd, spread=spread)
+    cache.k_scale.fill_(2.0 ** -6)
+    scale, cu = hd ** -0.5, bounds(new)
+    g = np.random.default_rng(hd)
+    want = torch.zeros(sum(new), hkv * group, hd, dtype=torch.float64, device=DEV)
+    for i, (n, rows) in enumerate(zip(lens, new)):
+        pos = torch.arange(n, device=DEV)
+        ids, at = table[i].long()[pos // BLOCK], pos % BLOCK
+        for h in range(hkv * group):
+            k = cache.k[ids, h // group, at].double() * 2.0 ** -6
+            v = cache.v[ids, h // group, at].double() * cache.v_scale[ids, h // group].double()[:, None]
+            for r in range(rows):
+                key = int(g.integers(0, n - rows + r + 1))
+                x = k[key] * 2.0 ** 21.5 / (scale * math.log2(math.e) * (k[key] @ k[key]))
+                q[cu[i] + r, h] = x.bfloat16()
+                scores = k[:n - rows + r + 1] @ q[cu[i] + r, h].double() * scale * math.log2(math.e)
+                assert scores.argmax() == key and scores.abs().max() < 2 ** 22
+                assert scores.numel() == 1 or scores.topk(2).values.diff().item() < -2.0 ** 17
+                want[cu[i] + r, h] = v[key]
+    out = ops.attention_cache(q, cache, table, ints(cu), ints(lens), max(new), scale, (-1, 0)).double()
+    ops.check_status(DEV)
+    want = want.flatten(1)
+    assert ((out - want).abs() <= (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -14) * want.abs()).all()
+
+
 def test_strides_and_rows_behind_the_last_request():
     """q, gate and out as columns of wider buffers, a table with a row stride, rows of padding left as they were."""
     lens, new = [300, 77], [5, 20]
