@@ -94,6 +94,25 @@ def test_tables_of_the_most_requests():
     assert table.tolist() == rows and stack.tolist() == free and height.tolist() == [count, 0]
 
 
+def test_tables_of_the_most_requests_on_a_large_pool():
+    """The largest shared memory a call can ask for, in a cluster of eight: 16,384 requests, ids in two parts."""
+    n, capacity = 16384, 2 ** 18 + 70000
+    lens, new = [5] * n, [1] * n
+    for i in range(0, n, 7):
+        new[i] = 64
+    need = len(range(0, n, 7))
+    ids = np.random.default_rng(8).permutation(capacity).tolist()
+    rows, free = [[x, -1] for x in ids[:n]], ids[n:] + [-1] * n
+    count = capacity - n
+    table, stack, height = ints(rows), ints(free), ints([count, 0])
+    got = ops.kv_assign(ints(lens), ints(bounds(new)), table, stack, height, sum(new))
+    want = ref.assign(lens, new, rows, free, count, 2)
+    assert [x.tolist() for x in got] == list(want[:3]) and table.tolist() == want[3]
+    assert height.tolist() == [count - need, 0]
+    ops.kv_release(table, got[0], ints(lens), stack, height)
+    assert table.tolist() == rows and stack.tolist() == free and height.tolist() == [count, 0]
+
+
 def test_assign_takes_nothing_when_blocks_are_missing():
     lens, new = [70, 0, 10], [200, 65, 4]
     rows, free, count = dealt(lens, new, 8, 4)  # 3 + 2 + 0 new blocks, 4 free
